@@ -68,6 +68,17 @@ _SIGS = {
     "cuinf_moe_ffn_workspace_size": (c_size_t, [c_int, c_int, c_int]),
     "cuinf_moe_ffn": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
                               c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "cuinf_attn_varlen_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "cuinf_attn_varlen": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_int,
+                                  c_float, c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "cuinf_kv_paged_append": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int,
+                                      c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p,
+                                      c_void_p, c_int, c_void_p]),
+    "cuinf_attn_paged_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "cuinf_attn_paged": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_int,
+                                 c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_float,
+                                 c_void_p, c_int, c_int, c_void_p, c_size_t, c_void_p]),
+    "cuinf_paged_error": (c_int, [ctypes.POINTER(ctypes.c_uint)]),
     "cuinf_quantize_int4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
     "cuinf_quantize_int4_host": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
     "cuinf_default_config": (None, [ctypes.POINTER(CuinfConfig)]),

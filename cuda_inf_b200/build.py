@@ -20,7 +20,7 @@ BUILD = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libcuinf.so")
 BUILD_TRACE = os.path.join(PKG, "_build_trace")
 LIB_TRACE = os.path.join(PKG, "libcuinf_trace.so")
-SOURCES = ["ops.cu", "engine.cu", "batch.cu", "tokenizer.cpp"]
+SOURCES = ["ops.cu", "engine.cu", "batch.cu", "serve.cu", "tokenizer.cpp"]
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith((".cuh", ".h")))
 
 NVCC = os.environ.get("NVCC", "nvcc")

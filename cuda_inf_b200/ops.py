@@ -3,7 +3,8 @@
 Names and argument meaning follow the kernels of src/engine.cu in
 g023/cuda_inf (gemv_int4, rmsnorm, rope, kv_commit_group, ...); each call goes
 through the C ABI of libcuinf.so on the current torch CUDA stream.  Tensors
-must be CUDA and contiguous; fp16 activations, u8 packed INT4 / FP8, fp32
+must be CUDA and contiguous (the serving operators at the end also take
+strided token rows, and run on their tensors' device); fp16 activations, u8 packed INT4 / FP8, fp32
 GEMV outputs.  Errors raise CuinfError; nothing falls back to the CPU.
 """
 import ctypes
@@ -17,6 +18,7 @@ __all__ = [
     "kv_commit_group", "attn_decode", "attn_decode_noalloc", "conv_pre", "conv_apply", "conv_update_state", "swiglu",
     "acc_scaled", "add_inplace", "add_f32_inplace", "f32_to_f16", "embed_gather", "argmax",
     "moe_route", "moe_ffn", "quantize_int4", "expert_table",
+    "attn_varlen", "kv_paged_append", "attn_paged", "paged_error",
 ]
 
 
@@ -247,3 +249,172 @@ def quantize_int4(w):
     scales = torch.empty((N, K // 128), dtype=torch.float16, device=w.device)
     check(lib().cuinf_quantize_int4(_p(w), N, K, _p(packed), _p(scales), _stream()))
     return packed, scales
+
+
+# --------------------------------------------------------------------------
+# serving attention: packed prompts, and a paged FP8 cache
+# --------------------------------------------------------------------------
+def _heads(t, name, dev=None):
+    """(pointer, elements between tokens, heads) of fp16 rows [T, heads, 64]; the
+    tokens may be apart (a part of a wider row), a token's heads not."""
+    _dt(t, torch.float16, name)
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor")
+    if dev is not None and t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if t.dim() != 3 or t.shape[2] != 64 or t.shape[1] == 0:
+        raise ValueError(f"{name} must be [tokens, heads, 64], got {tuple(t.shape)}")
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 64):
+        raise ValueError(f"{name}: a token's heads must be contiguous")
+    stride = t.stride(0) if t.shape[0] > 1 else t.shape[1] * 64
+    return ctypes.c_void_p(t.data_ptr()), stride, t.shape[1]
+
+
+def _ints(t, shape, name, dev):
+    _dt(t, torch.int32, name)
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+    return _p(t)
+
+
+def _cache(dev, n, table, kp8, vp8, kps, vps, ktail, vtail):
+    """Checked pointers of a paged cache, in the order of the C ABI, and its sizes."""
+    if table.dim() != 2 or table.shape[1] == 0:
+        raise ValueError("table must be [sequences, pages]")
+    if kp8.dim() != 4 or tuple(kp8.shape[2:]) != (64, 64) or kp8.shape[0] == 0 or kp8.shape[1] == 0:
+        raise ValueError(f"kp8 must be [pages, kv heads, 64, 64], got {tuple(kp8.shape)}")
+    n_pages, nkv = kp8.shape[:2]
+    ptrs = [_ints(table, (n, table.shape[1]), "table", dev)]
+    for t, dtype, shape, name in ((kp8, torch.uint8, (n_pages, nkv, 64, 64), "kp8"),
+                                  (vp8, torch.uint8, (n_pages, nkv, 64, 64), "vp8"),
+                                  (kps, torch.float16, (n_pages, nkv), "kps"),
+                                  (vps, torch.float16, (n_pages, nkv), "vps"),
+                                  (ktail, torch.float16, (n, nkv, 64, 64), "ktail"),
+                                  (vtail, torch.float16, (n, nkv, 64, 64), "vtail")):
+        _dt(t, dtype, name)
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+        if tuple(t.shape) != shape:
+            raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
+        ptrs.append(_p(t))
+    return ptrs, n_pages, nkv
+
+
+def _cu(cu_seqlens, dev):
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+        raise ValueError("cu_seqlens must be [sequences + 1]")
+    return _ints(cu_seqlens, (cu_seqlens.numel(),), "cu_seqlens", dev), cu_seqlens.numel() - 1
+
+
+def _out(out, q):
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _dt(out, torch.float16, "out")
+    if out.shape != q.shape or out.device != q.device:
+        raise ValueError(f"out must be {tuple(q.shape)} on {q.device}")
+    return out
+
+
+def _scratch(workspace, size, dev):
+    """The workspace's pointer and bytes; without one, scratch of this call (from
+    torch's allocator, so it follows the stream's order and a capture's pool)."""
+    if workspace is None:
+        workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    elif workspace.device != dev:
+        raise ValueError(f"workspace is on {workspace.device}, expected {dev}")
+    nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
+    return workspace, nbytes
+
+
+def attn_varlen(q, k, v, cu_seqlens, scale=0.125, out=None, workspace=None):
+    """Causal attention of prompts packed behind one another: row t of sequence s
+    (rows cu_seqlens[s]..cu_seqlens[s+1]-1) attends that sequence's rows up to t.
+
+    q fp16 [T,nh,64], k, v fp16 [T,nkv,64] (tokens may be strided, so k and v may
+    be parts of one projection's rows), cu_seqlens int32 [n+1] on the device;
+    query head h reads kv head h // (nh // nkv).  Rows outside all sequences are
+    left as they were (undefined in a new `out`).  Nothing synchronizes."""
+    qp, qs, nh = _heads(q, "q")
+    dev = q.device
+    kp, ks, nkv = _heads(k, "k", dev)
+    vp, vs, nv = _heads(v, "v", dev)
+    if k.shape[0] != q.shape[0] or v.shape[0] != q.shape[0] or nv != nkv:
+        raise ValueError("q, k and v must have the same tokens, k and v the same heads")
+    cu, n = _cu(cu_seqlens, dev)
+    out = _out(out, q)
+    T = q.shape[0]
+    if T == 0 or n == 0:
+        return out
+    L = lib()
+    with torch.cuda.device(dev):
+        ws, nbytes = _scratch(workspace, L.cuinf_attn_varlen_workspace_size(n, T, nh, nkv), dev)
+        check(L.cuinf_attn_varlen(qp, qs, kp, ks, vp, vs, cu, n, T, scale, _p(out), nh, nkv, _p(ws), nbytes,
+                                  _stream()))
+    return out
+
+
+def kv_paged_append(k, v, cu_seqlens, ctx_lens, table, kp8, vp8, kps, vps, ktail, vtail):
+    """Append packed new rows to the paged FP8 cache, what kv_write_tail and
+    kv_commit_group do for one sequence's contiguous cache.
+
+    k, v fp16 [T,nkv,64] (tokens may be strided); sequence s holds ctx_lens[s]
+    tokens before and gets rows cu_seqlens[s]..cu_seqlens[s+1]-1.  Groups of 64
+    tokens that become complete are quantized into page table[s, group] (kp8/vp8
+    u8 [pages,nkv,64,64], kps/vps fp16 [pages,nkv]); the rest goes to
+    ktail/vtail fp16 [n,nkv,64,64].  Page indices outside the pool and lengths
+    outside their ranges are skipped and reported by paged_error()."""
+    kp, ks, nkv = _heads(k, "k")
+    dev = k.device
+    vp, vs, nv = _heads(v, "v", dev)
+    if v.shape[0] != k.shape[0] or nv != nkv:
+        raise ValueError("k and v must have the same shape")
+    cu, n = _cu(cu_seqlens, dev)
+    ctx = _ints(ctx_lens, (n,), "ctx_lens", dev)
+    (tb, *cache), n_pages, cache_kv = _cache(dev, n, table, kp8, vp8, kps, vps, ktail, vtail)
+    if cache_kv != nkv:
+        raise ValueError(f"the cache has {cache_kv} kv heads, k {nkv}")
+    if k.shape[0] == 0 or n == 0:
+        return
+    with torch.cuda.device(dev):
+        check(lib().cuinf_kv_paged_append(kp, ks, vp, vs, cu, ctx, n, k.shape[0], tb, table.shape[1], *cache[:4],
+                                          n_pages, *cache[4:], nkv, _stream()))
+
+
+def attn_paged(q, cu_seqlens, kv_lens, table, kp8, vp8, kps, vps, ktail, vtail, scale=0.125, max_q=None, out=None,
+               workspace=None):
+    """Attention of new tokens over the paged FP8 cache that already holds them
+    (kv_paged_append first): sequence s has kv_lens[s] tokens, its new rows
+    q[cu_seqlens[s]:cu_seqlens[s+1]] are the last of them, and each attends all
+    positions up to its own; a row whose position is negative is zero.
+
+    q fp16 [T,nh,64] (tokens may be strided); a chunk of a prompt, drafted
+    tokens, or one token per sequence (the decode step), mixed as they come.
+    max_q: an upper bound of the rows of one sequence (default T); a smaller
+    bound lets a pure decode step skip the chunks' kernel.  Nothing
+    synchronizes; what the device finds wrong is reported by paged_error()."""
+    qp, qs, nh = _heads(q, "q")
+    dev = q.device
+    cu, n = _cu(cu_seqlens, dev)
+    kvl = _ints(kv_lens, (n,), "kv_lens", dev)
+    (tb, *cache), n_pages, nkv = _cache(dev, n, table, kp8, vp8, kps, vps, ktail, vtail)
+    out = _out(out, q)
+    T = q.shape[0]
+    if T == 0 or n == 0:
+        return out
+    max_q = T if max_q is None else max_q
+    L = lib()
+    with torch.cuda.device(dev):
+        ws, nbytes = _scratch(workspace, L.cuinf_attn_paged_workspace_size(n, T, max_q, nh, nkv, table.shape[1]), dev)
+        check(L.cuinf_attn_paged(qp, qs, cu, kvl, n, T, max_q, tb, table.shape[1], *cache[:4], n_pages, *cache[4:],
+                                 scale, _p(out), nh, nkv, _p(ws), nbytes, _stream()))
+    return out
+
+
+def paged_error():
+    """Read and clear the current device's error word of attn_varlen,
+    kv_paged_append and attn_paged (0 = none; the bits are in cuinf.h)."""
+    flags = ctypes.c_uint(0)
+    check(lib().cuinf_paged_error(ctypes.byref(flags)))
+    return flags.value

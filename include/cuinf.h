@@ -160,6 +160,74 @@ int cuinf_moe_ffn(const void* xn, const void* gate, const void* expert_bias,
                   const void* const* experts, void* h, int H, int I, int n_exp, int topk,
                   int* idx, float* w, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* Serving attention: packed prompts, and a paged FP8 cache.  No counterpart  */
+/* in the reference, which holds one sequence in contiguous buffers           */
+/* (Buffers, engine.cu:590-623).                                               */
+/*                                                                             */
+/* Packed rows: the tokens of n_seqs sequences behind one another; sequence s  */
+/* holds rows cu_seqlens[s] .. cu_seqlens[s+1]-1 of n_rows (device int         */
+/* [n_seqs+1], non-decreasing; empty sequences are allowed).  Rows outside     */
+/* all sequences are left as they were.  A row of `heads` heads is heads*64    */
+/* contiguous fp16 values; rows are *_stride elements apart (a multiple of 8,  */
+/* at least heads*64), so keys and values may be parts of a wider row.         */
+/*                                                                             */
+/* Paged cache: pages of 64 tokens (the commit group), head-major, so that     */
+/* one head of one page is 4096 contiguous bytes: kp8/vp8 u8                   */
+/* [n_pages][nkv][64][64] FP8 E4M3 with one fp16 scale per page and kv head    */
+/* (kps/vps [n_pages][nkv]); table (device int [n_seqs][table_width]) names    */
+/* the page of each whole 64-token group of a sequence; the tokens behind its  */
+/* last whole group are fp16 in ktail/vtail [n_seqs][nkv][64][64].  Sequences  */
+/* may share pages that are only read (a common prefix).                       */
+/*                                                                             */
+/* All lengths are read on the device; nothing synchronizes, so the calls can  */
+/* be captured into a CUDA graph.  What the device finds wrong there it skips  */
+/* and reports in a word per device (cuinf_paged_error): a page index outside  */
+/* the pool (its keys count as absent, its group is not stored), lengths or    */
+/* offsets outside their ranges (the sequence is skipped).                     */
+/* ------------------------------------------------------------------------ */
+
+/* out[t,h,:] = softmax(scale * q[t,h] . k[j,h/(nh/nkv)]) v over the rows j of
+ * t's sequence up to t (causal).  q [n_rows][nh][64], k, v [n_rows][nkv][64],
+ * out fp16 [n_rows][nh][64] contiguous; nh/nkv <= 128; scale > 0.  Softmax
+ * statistics and sums in fp32.  workspace: device scratch of
+ * cuinf_attn_varlen_workspace_size bytes, 16-byte aligned, any contents; calls
+ * that may overlap need one each.  All q/k/v/out pointers 16-byte aligned. */
+size_t cuinf_attn_varlen_workspace_size(int n_seqs, int n_rows, int nh, int nkv);
+int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                      int64_t v_stride, const int* cu_seqlens, int n_seqs, int n_rows, float scale, void* out,
+                      int nh, int nkv, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Append the packed new rows k, v [n_rows][nkv][64] to the paged cache:
+ * sequence s holds ctx_lens[s] tokens (device int) before the call.  Every
+ * 64-token group that the call completes is quantized like
+ * cuinf_kv_commit_group into page table[s][group] (scale = absmax/448 + 1e-12,
+ * codes with the fp32 scale); the rows of the unfinished last group go to the
+ * tail, whose other rows stay as they were.  No page that the call writes may
+ * be shared. */
+int cuinf_kv_paged_append(const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                          const int* cu_seqlens, const int* ctx_lens, int n_seqs, int n_rows, const int* table,
+                          int table_width, uint8_t* kp8, uint8_t* vp8, void* kps, void* vps, int n_pages,
+                          void* ktail, void* vtail, int nkv, void* stream);
+
+/* Attention of the packed new rows q [n_rows][nh][64] over the paged cache
+ * that holds them: sequence s has kv_lens[s] tokens (device int), its c new
+ * rows the last c of them; row i attends positions 0 .. kv_lens[s]-c+i (none
+ * where that is negative: the row is zero).  max_q (host) is at least the
+ * rows of the longest sequence; a longer one is skipped and reported.  One
+ * token per sequence is the decode step.  workspace as above. */
+size_t cuinf_attn_paged_workspace_size(int n_seqs, int n_rows, int max_q, int nh, int nkv, int table_width);
+int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_seqlens, const int* kv_lens, int n_seqs,
+                     int n_rows, int max_q, const int* table, int table_width, const uint8_t* kp8,
+                     const uint8_t* vp8, const void* kps, const void* vps, int n_pages, const void* ktail,
+                     const void* vtail, float scale, void* out, int nh, int nkv, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Read and clear the current device's error word of these operators
+ * (synchronous): bit 0 a bounded wait gave up, bit 1 a page index outside the
+ * pool, bit 2 lengths or offsets outside their ranges. */
+int cuinf_paged_error(unsigned* flags);
+
 /* INT4 G=128 quantizer of tools/export_weights.py:64-79, bit-exact:
  * scale = amax/7 (fp32), q = rint(w/scale) clipped to [-7,7], nibble q+8,
  * scale stored fp16.  Device version (w, packed, scales device pointers) and

@@ -1,0 +1,624 @@
+"""GPU tests of the serving attention operators against plain 64-bit forms.
+
+Tolerance of the attention, per output value, from the formulas: the softmax
+weights are rounded to fp16 before they meet the values, each off by at most
+2^-11 of itself, so the sum is off by 2^-11 sum p|v|; their exponentials, the
+scores' fp32 sums and the running rescalings are together well below another
+2^-12 of each weight for scores up to 2^7; the result is rounded to fp16
+(2^-11 |o|).  Weights below fp16's normal range are off by at most 2^-25 of the
+largest weight each, in units of which the values enter with at most max|v|
+(for FP8 pages the weight carries the page's scale times a constant of at least
+16, so a value of at most 448 scales enters with 28).  Hence
+  |got - o| <= 2^-11 |o| + 1.5 * 2^-11 sum p|v| + n 2^-25 max(max|v|, 28).
+Codes, scales and tails of the cache have to be those of kv_commit_group and
+kv_write_tail, bit for bit.
+"""
+import pytest
+import torch
+
+from cuda_inf_b200 import ops
+from cuda_inf_b200._lib import CuinfError
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(autouse=True)
+def _clean(cuda):
+    ops.paged_error()
+    yield
+    torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ plain forms
+def plain_rows(q, k, v, first, scale):
+    """q [c,nh,64] at positions first.., k, v [nkv,l,64] (64 bits): (out, bound on its error)."""
+    c, nh, _ = q.shape
+    k, v = (x.repeat_interleave(nh // k.shape[0], 0) for x in (k, v))
+    s = torch.einsum("chd,hld->hcl", q.double(), k) * scale
+    pos = first + torch.arange(c, device=q.device)
+    ok = (torch.arange(k.shape[1], device=q.device)[None] <= pos[:, None])[None]
+    s = torch.where(ok, s, torch.full_like(s, -INF))
+    p = torch.where(pos[None, :, None] >= 0, torch.softmax(s, -1), torch.zeros_like(s)) if k.shape[1] else s
+    # a weight of zero takes no part, whatever its value is
+    fin = torch.isfinite(v)
+    o = torch.einsum("hcl,hld->chd", p, torch.where(fin, v, torch.zeros_like(v)))
+    mag = torch.einsum("hcl,hld->chd", p, torch.where(fin, v, torch.zeros_like(v)).abs())
+    if not bool(fin.all()):
+        seen = ok.double().expand_as(s)
+        for kind, x in ((v == INF, INF), (v == -INF, -INF), (v.isnan(), NAN)):
+            hit = torch.einsum("hcl,hld->chd", seen, kind.double()) > 0
+            o = torch.where(hit, o + x, o)
+    big = float(torch.where(fin, v, torch.zeros_like(v)).abs().max()) if v.numel() else 0.0
+    return o, 2.0**-11 * o.abs() + 1.5 * 2.0**-11 * mag + k.shape[1] * 2.0**-25 * max(big, 28.0)
+
+
+def close(got, want, tol):
+    g = got.double()
+    fin = torch.isfinite(want)
+    assert torch.equal(torch.isnan(g), torch.isnan(want))
+    assert torch.equal(g[~fin & ~want.isnan()], want[~fin & ~want.isnan()])
+    e = (g - want).abs()[fin]
+    bad = e > tol[fin]
+    assert not bool(bad.any()), (float(e.max()), float((e / tol[fin]).max()), int(bad.sum()), e.numel())
+
+
+def cum(lens, dev, start=0):
+    c = [start]
+    for x in lens:
+        c.append(c[-1] + x)
+    return torch.tensor(c, dtype=torch.int32, device=dev)
+
+
+def rnd(shape, seed, dev, scale=1.0):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=dev) * scale).half()
+
+
+# ------------------------------------------------------------------ packed prompts
+def check_varlen(q, k, v, lens, out, scale=0.125, start=0):
+    a = start
+    for x in lens:
+        if x:
+            o, tol = plain_rows(q[a:a + x], k[a:a + x].double().transpose(0, 1), v[a:a + x].double().transpose(0, 1), 0,
+                                scale)
+            close(out[a:a + x], o, tol)
+        a += x
+
+
+LENS = [[1], [2], [17], [64], [127], [128], [129], [255, 1, 0, 3], [300], [1, 1, 1, 1, 1], [513, 64, 31, 0, 0, 700],
+        [1025, 130], [2500], [40] * 37, [0, 0, 5]]
+
+
+@pytest.mark.parametrize("lens", LENS, ids=lambda x: "-".join(map(str, x[:6])))
+@pytest.mark.parametrize("nh,nkv", [(32, 8), (4, 1), (8, 8), (12, 4), (5, 1), (32, 1), (7, 7)])
+def test_varlen(cuda, lens, nh, nkv):
+    t = sum(lens)
+    q, k, v = rnd((t, nh, 64), 1 + t, cuda), rnd((t, nkv, 64), 2 + t, cuda), rnd((t, nkv, 64), 3 + t, cuda)
+    out = ops.attn_varlen(q, k, v, cum(lens, cuda))
+    assert ops.paged_error() == 0
+    check_varlen(q, k, v, lens, out)
+
+
+@pytest.mark.parametrize("grp", [96, 128, 48])
+def test_varlen_many_heads_per_kv_head(cuda, grp):
+    lens = [130, 5]
+    q, k, v = rnd((135, grp, 64), 1, cuda), rnd((135, 1, 64), 2, cuda), rnd((135, 1, 64), 3, cuda)
+    check_varlen(q, k, v, lens, ops.attn_varlen(q, k, v, cum(lens, cuda)))
+
+
+def test_varlen_strided_rows_and_out(cuda):
+    """q, k and v as parts of wider rows, out given; rows outside the sequences stay."""
+    lens, start, t = [70, 0, 200], 9, 300
+    wide = rnd((t, 20, 64), 5, cuda)
+    q, k, v = wide[:, :12], wide[:, 12:16], wide[:, 16:]
+    out = torch.full((t, 12, 64), 7.0, dtype=torch.float16, device=cuda)
+    assert ops.attn_varlen(q, k, v, cum(lens, cuda, start), out=out) is out
+    check_varlen(q, k, v, lens, out, start=start)
+    assert bool((out[:start] == 7).all()) and bool((out[start + 270:] == 7).all())
+
+
+@pytest.mark.parametrize("scale,mul", [(0.125, 8.0), (1.0, 3.0), (1e-4, 1.0), (0.125, 0.0)])
+def test_varlen_scores(cuda, scale, mul):
+    """Scores that are sharp, flat, all equal; a maximum that grows along the keys."""
+    lens = [400, 33]
+    q, k, v = rnd((433, 8, 64), 1, cuda, mul), rnd((433, 2, 64), 2, cuda), rnd((433, 2, 64), 3, cuda)
+    k = k * torch.linspace(0.1, 1.5, 433, device=cuda).half()[:, None, None]
+    check_varlen(q, k, v, lens, ops.attn_varlen(q, k, v, cum(lens, cuda), scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("at", [0, 63, 64, 190, 299])
+def test_varlen_masked_places_do_not_reach_the_rows(cuda, bad, at):
+    """A value that is no number reaches the rows that attend it, and those alone;
+    keys that are no numbers in masked places reach nothing."""
+    lens, nh, nkv = [300, 45], 8, 2
+    q, k, v = rnd((345, nh, 64), 1, cuda), rnd((345, nkv, 64), 2, cuda), rnd((345, nkv, 64), 3, cuda)
+    v[at, 1, 5] = bad
+    out = ops.attn_varlen(q, k, v, cum(lens, cuda))
+    check_varlen(q, k, v, lens, out)
+    k[at] = bad  # rows before `at` and the other sequence stay as they were
+    out2 = ops.attn_varlen(q, k, v, cum(lens, cuda))
+    assert torch.equal(out2[:at], out[:at]) and torch.equal(out2[300:], out[300:])
+    assert bool(out2[at].isnan().all())
+
+
+def test_varlen_neighbours_of_nan(cuda):
+    """Sequences of NaN on both sides of one of numbers."""
+    lens = [100, 77, 300]
+    q, k, v = rnd((477, 8, 64), 1, cuda), rnd((477, 2, 64), 2, cuda), rnd((477, 2, 64), 3, cuda)
+    want = ops.attn_varlen(q, k, v, cum(lens, cuda))
+    for t in (q, k, v):
+        t[:100] = NAN
+        t[177:] = NAN
+    out = ops.attn_varlen(q, k, v, cum(lens, cuda))
+    assert torch.equal(out[100:177], want[100:177])
+    assert bool(out[:100].isnan().all()) and bool(out[177:].isnan().all())
+
+
+def test_varlen_bad_offsets_are_reported(cuda):
+    q, k, v = rnd((50, 4, 64), 1, cuda), rnd((50, 1, 64), 2, cuda), rnd((50, 1, 64), 3, cuda)
+    want = ops.attn_varlen(q, k, v, cum([50], cuda))
+    assert ops.paged_error() == 0
+    out = torch.full_like(want, 3.0)
+    ops.attn_varlen(q, k, v, torch.tensor([0, 50, 70], dtype=torch.int32, device=cuda), out=out)
+    assert ops.paged_error() & 4
+    assert torch.equal(out, want)
+    assert ops.paged_error() == 0
+
+
+# ------------------------------------------------------------------ the paged cache
+class Cache:
+    """Pages in a shuffled order for n sequences of up to `room` tokens each."""
+
+    def __init__(self, n, nkv, room, dev, seed=0, spare=2):
+        w = max(1, -(-room // 64))
+        g = torch.Generator(device=dev).manual_seed(seed)
+        self.n, self.nkv, self.dev = n, nkv, dev
+        pages = n * w + spare
+        self.table = torch.randperm(pages, generator=g, device=dev)[:n * w].to(torch.int32).view(n, w).contiguous()
+        # free places hold codes and bits that are no numbers
+        self.kp8 = torch.full((pages, nkv, 64, 64), 0x7F, dtype=torch.uint8, device=dev)
+        self.vp8 = self.kp8.clone()
+        self.kps = torch.full((pages, nkv), NAN, dtype=torch.float16, device=dev)
+        self.vps = self.kps.clone()
+        self.ktail = torch.full((n, nkv, 64, 64), NAN, dtype=torch.float16, device=dev)
+        self.vtail = self.ktail.clone()
+        self.lens = [0] * n
+
+    @property
+    def t(self):
+        return self.table, self.kp8, self.vp8, self.kps, self.vps, self.ktail, self.vtail
+
+    def ints(self):
+        return torch.tensor(self.lens, dtype=torch.int32, device=self.dev)
+
+    def append(self, k, v, new):
+        ops.kv_paged_append(k, v, cum(new, self.dev), self.ints(), *self.t)
+        self.lens = [a + b for a, b in zip(self.lens, new)]
+
+    def values(self, i, which):
+        """[nkv, len, 64] in 64 bits."""
+        g, r = divmod(self.lens[i], 64)
+        p8, ps, tail = (self.kp8, self.kps, self.ktail) if which == "k" else (self.vp8, self.vps, self.vtail)
+        at = self.table[i, :g].long()
+        x = p8[at].view(torch.float8_e4m3fn).double() * ps[at].double()[:, :, None, None]
+        x = x.permute(1, 0, 2, 3).reshape(self.nkv, g * 64, 64)
+        return torch.cat([x, tail[i, :, :r].double()], 1)
+
+    def check(self, q, new, out, scale=0.125):
+        a = 0
+        for i, c in enumerate(new):
+            if c:
+                o, tol = plain_rows(q[a:a + c], self.values(i, "k"), self.values(i, "v"), self.lens[i] - c, scale)
+                close(out[a:a + c], o, tol)
+            a += c
+
+    def attend(self, q, new, **kw):
+        return ops.attn_paged(q, cum(new, self.dev), self.ints(), *self.t, **kw)
+
+
+def fill(cache, lens, seed, vscale=0.5):
+    """Appends `lens` random tokens in one call."""
+    t = sum(lens)
+    if t:
+        cache.append(rnd((t, cache.nkv, 64), seed, cache.dev), rnd((t, cache.nkv, 64), seed + 1, cache.dev, vscale),
+                     lens)
+
+
+APPENDS = [([0], [1]), ([0], [64]), ([0], [63]), ([63], [1]), ([63], [2]), ([5], [59]), ([5], [60]), ([0], [65]),
+           ([60], [200]), ([10, 0, 64, 127], [1, 1, 1, 1]), ([10, 0, 64, 127, 3], [300, 0, 64, 129, 0]),
+           ([1] * 300, [1] * 300), ([0, 7], [1500, 1])]
+
+
+@pytest.mark.parametrize("ctx,new", APPENDS, ids=lambda x: "-".join(map(str, x[:5])))
+@pytest.mark.parametrize("nkv", [1, 8])
+def test_append_is_write_tail_and_commit(cuda, ctx, new, nkv):
+    """Bit-equal to kv_write_tail + kv_commit_group, one sequence after another."""
+    n = len(ctx)
+    c = Cache(n, nkv, max(a + b for a, b in zip(ctx, new)) + 1, cuda, seed=len(ctx))
+    fill(c, ctx, 11)
+    kt, vt = c.ktail.clone(), c.vtail.clone()
+    p = [x.clone() for x in (c.kp8, c.vp8, c.kps, c.vps)]
+    wide = rnd((sum(new), 2 * nkv, 64), 21, cuda)
+    k, v = wide[:, :nkv], wide[:, nkv:]
+    old = list(c.lens)
+    c.append(k, v, new)
+    assert ops.paged_error() == 0
+    at = 0
+    for i in range(n):
+        t1, t2 = (x[i].transpose(0, 1).clone(memory_format=torch.contiguous_format) for x in (kt, vt))  # [64, nkv, 64]
+        done = 0
+        while done < new[i]:
+            pos = old[i] + done
+            slot, cnt = pos % 64, min(64 - pos % 64, new[i] - done)
+            ops.kv_write_tail(k[at + done:at + done + cnt].contiguous(), v[at + done:at + done + cnt].contiguous(),
+                              t1, t2, slot, cnt)
+            done += cnt
+            if slot + cnt == 64:
+                k8, v8 = (torch.empty((64, nkv, 64), dtype=torch.uint8, device=cuda) for _ in range(2))
+                s1, s2 = (torch.empty((1, nkv), dtype=torch.float16, device=cuda) for _ in range(2))
+                ops.kv_commit_group(t1, t2, k8, v8, s1, s2, 0, 0)
+                page = int(c.table[i, pos // 64])
+                p[0][page], p[1][page] = k8.transpose(0, 1), v8.transpose(0, 1)
+                p[2][page], p[3][page] = s1[0], s2[0]
+        rest = (old[i] + new[i]) % 64 if (old[i] + new[i]) // 64 > old[i] // 64 else old[i] % 64 + new[i]
+        kt[i, :, :rest], vt[i, :, :rest] = t1.transpose(0, 1)[:, :rest], t2.transpose(0, 1)[:, :rest]
+        at += new[i]
+    for got, want in zip((c.kp8, c.vp8, c.kps, c.vps, c.ktail, c.vtail), (*p, kt, vt)):
+        assert torch.equal(got.view(torch.uint8) if got.dtype != torch.uint8 else got,
+                           want.view(torch.uint8) if want.dtype != torch.uint8 else want)
+
+
+def test_append_zero_and_extreme_rows(cuda):
+    """A page of zeros, of fp16's largest values, of its smallest: codes and scales in 64 bits."""
+    c = Cache(1, 4, 64, cuda)
+    k = torch.zeros((64, 4, 64), dtype=torch.float16, device=cuda)
+    k[:, 1] = 65504.0
+    k[:, 2] = 6e-8
+    k[3, 3, 9] = -2.0
+    c.append(k, k, [64])
+    s = k.double().abs().amax((0, 2)) / 448 + 1e-12
+    page = int(c.table[0, 0])
+    assert torch.allclose(c.kps[page].double(), s, rtol=2**-10, atol=2**-25)
+    codes = c.kp8[page].view(torch.float8_e4m3fn).double()
+    want = (k.double() / s[None, :, None]).transpose(0, 1)
+    assert bool(((codes - want).abs() <= want.abs() * 2**-4 + 2**-10).all())
+    assert torch.equal(c.kp8[page], c.vp8[page])
+
+
+def test_append_bad_page_and_lengths_are_reported(cuda):
+    c = Cache(3, 2, 128, cuda)
+    fill(c, [60, 60, 60], 5)
+    c.table[1, 0] = -1
+    before = c.kp8.clone()
+    c.append(rnd((15, 2, 64), 1, cuda), rnd((15, 2, 64), 2, cuda), [5, 5, 5])
+    assert ops.paged_error() == 2
+    changed = (c.kp8 != before).flatten(1).any(1)
+    assert sorted(changed.nonzero().flatten().tolist()) == sorted([int(c.table[0, 0]), int(c.table[2, 0])])
+    # a group past the table's width, a negative length
+    c = Cache(1, 2, 64, cuda)
+    fill(c, [60], 5)
+    c.append(rnd((100, 2, 64), 1, cuda), rnd((100, 2, 64), 2, cuda), [100])
+    assert ops.paged_error() == 2
+    c = Cache(1, 2, 64, cuda)
+    c.lens = [-4]
+    before = [x.clone() for x in c.t]
+    c.append(rnd((100, 2, 64), 1, cuda), rnd((100, 2, 64), 2, cuda), [100])
+    assert ops.paged_error() == 4
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, c.t))
+
+
+TOKENS = [[1], [2], [63], [64], [65], [128], [129], [1000], [1, 64, 700, 3, 128], [4097, 5], [513] * 40, [9000],
+          list(range(1, 150))]
+
+
+@pytest.mark.parametrize("lens", TOKENS, ids=lambda x: "-".join(map(str, x[:5])))
+@pytest.mark.parametrize("nh,nkv", [(32, 8), (4, 1), (8, 8), (12, 4), (10, 2), (16, 1), (32, 1)])
+def test_single_tokens(cuda, lens, nh, nkv):
+    c = Cache(len(lens), nkv, max(lens), cuda, seed=1)
+    fill(c, lens, 3)
+    new = [1] * len(lens)
+    q = rnd((len(lens), nh, 64), 7, cuda)
+    out = c.attend(q, new, max_q=1)
+    assert ops.paged_error() == 0
+    c.check(q, new, out)
+    # the bound of the longest chunk changes the way, not the result's meaning
+    c.check(q, new, c.attend(q, new))
+
+
+CHUNKS = [([0], [1]), ([0], [64]), ([0], [300]), ([1], [2]), ([63], [2]), ([100], [28]), ([64], [64]), ([500], [33]),
+          ([130, 0, 64, 1000, 7], [5, 129, 0, 1, 300]), ([2000, 2000], [700, 1]), ([4000], [257]),
+          ([30] * 20, [3] * 20), ([1200] * 9, [1] * 8 + [400]), ([0], [1100])]
+
+
+@pytest.mark.parametrize("ctx,new", CHUNKS, ids=lambda x: "-".join(map(str, x[:5])))
+@pytest.mark.parametrize("nh,nkv", [(32, 8), (4, 1), (8, 8), (12, 4), (10, 2), (32, 1)])
+def test_chunks(cuda, ctx, new, nh, nkv):
+    c = Cache(len(ctx), nkv, max(a + b for a, b in zip(ctx, new)), cuda, seed=2)
+    fill(c, ctx, 3)
+    fill(c, new, 5)
+    wide = rnd((sum(new), nh + 2, 64), 7, cuda)
+    q = wide[:, 1:nh + 1]
+    out = c.attend(q, new, max_q=max(new))
+    assert ops.paged_error() == 0
+    c.check(q, new, out)
+
+
+def test_rows_before_the_first_key_are_zero(cuda):
+    """More new rows than the cache holds: the first ones have no key at all."""
+    c = Cache(3, 2, 128, cuda)
+    fill(c, [40, 3, 0], 3)
+    new = [100, 5, 2]
+    q = rnd((107, 8, 64), 7, cuda)
+    out = c.attend(q, new)
+    assert ops.paged_error() == 0
+    assert bool((out[:60] == 0).all()) and bool((out[100:102] == 0).all()) and bool((out[105:] == 0).all())
+    c.check(q, new, out)
+
+
+def test_rows_outside_the_sequences_stay(cuda):
+    c = Cache(2, 2, 256, cuda)
+    fill(c, [200, 90], 3)
+    q = rnd((300, 8, 64), 7, cuda)
+    for new in ([1, 1], [150, 3]):
+        out = torch.full_like(q, 7.0)
+        ops.attn_paged(q, cum(new, cuda, 20), c.ints(), *c.t, out=out, max_q=max(new))
+        a, b = 20, 20 + sum(new)
+        c.check(q[a:b], new, out[a:b])
+        assert bool((out[:a] == 7).all()) and bool((out[b:] == 7).all())
+
+
+@pytest.mark.parametrize("bad", [NAN, INF, -INF])
+@pytest.mark.parametrize("chunk", [1, 40, 200])
+def test_paged_masked_places(cuda, bad, chunk):
+    """Junk behind the last token, and a later token of the chunk that is no number."""
+    total = 333
+    c = Cache(1, 2, 448, cuda)
+    fill(c, [total], 3)
+    c.vtail[:, :, total % 64:] = bad
+    c.ktail[:, :, total % 64:] = bad
+    q = rnd((chunk, 8, 64), 7, cuda)
+    out = c.attend(q, [chunk])
+    c.check(q, [chunk], out)
+    if chunk > 1:
+        c.vtail[0, :, total % 64 - 1, 3] = bad  # the newest token: the last row alone attends it
+        got = c.attend(q, [chunk])
+        assert torch.equal(got[:-1], out[:-1])
+        c.check(q, [chunk], got)
+
+
+def test_paged_bad_pages_count_as_absent(cuda):
+    """A page index outside the pool: its keys are left out, and reported."""
+    for chunk in (1, 60):
+        c = Cache(2, 2, 512, cuda)
+        fill(c, [500, 300], 3)
+        q = rnd((2 * chunk, 8, 64), 7, cuda)
+        want = c.attend(q, [chunk, chunk])
+        for wrong in (-1, c.kp8.shape[0], 2**31 - 1, -2**31):
+            keep = int(c.table[0, 2])
+            c.table[0, 2] = wrong
+            out = c.attend(q, [chunk, chunk], max_q=chunk)
+            assert ops.paged_error() == 2
+            assert torch.equal(out[chunk:], want[chunk:])
+            c.table[0, 2] = keep
+            k, v = (torch.cat([c.values(0, x)[:, :128], c.values(0, x)[:, 192:]], 1) for x in ("k", "v"))
+            o, tol = plain_rows(q[:chunk], k, v, 500 - 64 - chunk, 0.125)
+            close(out[:chunk], o, tol)
+
+
+def test_paged_bad_lengths_are_reported(cuda):
+    c = Cache(3, 2, 128, cuda)
+    fill(c, [100, 100, 100], 3)
+    q = rnd((3, 8, 64), 7, cuda)
+    want = c.attend(q, [1, 1, 1])
+    for wrong in (-1, 192, 10000, 2**31 - 1, -2**31):
+        c.lens[1] = wrong
+        for mq in (1, 64):
+            out = torch.full_like(want, 5.0)
+            c.attend(q, [1, 1, 1], max_q=mq, out=out)
+            assert ops.paged_error() == 4
+            assert torch.equal(out[0], want[0]) and torch.equal(out[2], want[2]) and bool((out[1] == 5).all())
+    c.lens[1] = 100
+    out = torch.full((61, 8, 64), 5.0, dtype=torch.float16, device=cuda)
+    q = rnd((61, 8, 64), 7, cuda)
+    c.attend(q, [1, 59, 1], max_q=1, out=out)  # a longer sequence than the caller's bound
+    assert ops.paged_error() == 4
+    assert bool((out[1:60] == 5).all()) and not bool((out[0] == 5).any()) and not bool((out[60] == 5).any())
+
+
+def test_shared_prefix_pages(cuda):
+    c = Cache(2, 2, 640, cuda)
+    fill(c, [512, 512], 3)
+    c.table[1, :8] = c.table[0, :8]
+    fill(c, [30, 77], 9)
+    for new in ([1, 1], [30, 77]):
+        q = rnd((sum(new), 8, 64), 7, cuda)
+        c.check(q, new, c.attend(q, new, max_q=max(new)))
+
+
+def test_prefill_then_decode_as_served(cuda):
+    """Packed prompts through attn_varlen and into the cache, the rest of one prompt in chunks, then steps of
+    one token beside it; every output in 64 bits from what the cache holds."""
+    n, nh, nkv = 4, 32, 8
+    c = Cache(n, nkv, 700, cuda)
+    steps = [[130, 64, 1, 0], [1, 1, 1, 250], [1, 1, 1, 250], [1, 1, 1, 37], [1, 1, 1, 1], [1, 0, 1, 1]]
+    for i, new in enumerate(steps):
+        t = sum(new)
+        q, k, v = rnd((t, nh, 64), i, cuda), rnd((t, nkv, 64), 50 + i, cuda), rnd((t, nkv, 64), 90 + i, cuda)
+        if i == 0:
+            check_varlen(q, k, v, new, ops.attn_varlen(q, k, v, cum(new, cuda)))
+        c.append(k, v, new)
+        c.check(q, new, c.attend(q, new, max_q=max(new)))
+    assert ops.paged_error() == 0
+
+
+@pytest.mark.parametrize("total", [1, 63, 200, 4095])
+def test_matches_the_contiguous_operator(cuda, total):
+    """attn_decode on the same cache laid out contiguously."""
+    c = Cache(1, 8, total, cuda)
+    fill(c, [total], 3)
+    g = total // 64
+    at = c.table[0, :max(g, 1)].long()
+    k8, v8 = (x[at].transpose(1, 2).reshape(-1, 8, 64).contiguous() for x in (c.kp8, c.vp8))
+    ks, vs = (x[at].contiguous() for x in (c.kps, c.vps))
+    q = rnd((1, 32, 64), 7, cuda)
+    kt, vt = (x[0].transpose(0, 1).contiguous().nan_to_num(0.0) for x in (c.ktail, c.vtail))
+    want = ops.attn_decode(q[0], k8, v8, ks, vs, kt, vt, g * 64, total - 1)
+    got = c.attend(q, [1], max_q=1)[0]
+    o, tol = plain_rows(q, c.values(0, "k"), c.values(0, "v"), total - 1, 0.125)
+    close(got, o[0], tol[0])
+    assert float((got.float() - want.float()).abs().max()) <= 2e-3 * float(want.float().abs().max()) + float(tol.max())
+
+
+def test_offsets_past_32_bits(cuda):
+    """Pages whose bytes lie behind 2^32."""
+    nkv, pages = 8, 131072 + 40
+    c = Cache(1, nkv, 64 * 9, cuda)
+    for name in ("kp8", "vp8"):
+        setattr(c, name, torch.zeros((pages, nkv, 64, 64), dtype=torch.uint8, device=cuda))
+    for name in ("kps", "vps"):
+        setattr(c, name, torch.zeros((pages, nkv), dtype=torch.float16, device=cuda))
+    c.table = (pages - 1 - 2 * torch.arange(9, device=cuda, dtype=torch.int32))[None].contiguous()
+    fill(c, [530], 3)
+    assert int(c.kp8[:131000].count_nonzero()) == 0
+    for new in ([1], [70], [520]):
+        q = rnd((new[0], 32, 64), 7, cuda)
+        c.check(q, new, c.attend(q, new, max_q=new[0]))
+    assert ops.paged_error() == 0
+
+
+def test_rows_past_32_bits(cuda):
+    """q and out of more than 2^31 elements, k and v strided past 2^31."""
+    nh, nkv, t = 128, 1, 270000
+    lens = [t - 300, 300]
+    q = torch.zeros((t, nh, 64), dtype=torch.float16, device=cuda)
+    wide = torch.zeros((t, 8192), dtype=torch.float16, device=cuda)
+    k, v = wide[:, None, :64], wide[:, None, 64:128]
+    q[-300:] = rnd((300, nh, 64), 1, cuda)
+    wide[-300:, :128] = rnd((300, 128), 2, cuda)
+    out = torch.zeros_like(q)
+    # the long sequence is cut short: its rows before the last 100 are nobody's
+    cu = torch.tensor([t - 400, t - 300, t], dtype=torch.int32, device=cuda)
+    ops.attn_varlen(q, k, v, cu, out=out)
+    check_varlen(q[-300:], k[-300:], v[-300:], [300], out[-300:])
+    assert ops.paged_error() == 0
+
+
+def test_same_bits_twice(cuda):
+    c = Cache(9, 8, 5000, cuda)
+    fill(c, [5000, 1, 70, 900, 64, 3000, 2, 700, 128], 3)
+    for new in ([1] * 9, [300, 1, 5, 64, 1, 1, 1, 130, 1]):
+        q = rnd((sum(new), 32, 64), 7, cuda)
+        a = c.attend(q, new, max_q=max(new))
+        for _ in range(3):
+            assert torch.equal(a, c.attend(q, new, max_q=max(new)))
+    q, k, v = rnd((3000, 32, 64), 1, cuda), rnd((3000, 8, 64), 2, cuda), rnd((3000, 8, 64), 3, cuda)
+    a = ops.attn_varlen(q, k, v, cum([2000, 1000], cuda))
+    assert torch.equal(a, ops.attn_varlen(q, k, v, cum([2000, 1000], cuda)))
+
+
+def test_captured_step_follows_the_lengths(cuda):
+    """A step captured once (append, attention; all lengths on the device) and replayed as the sequences grow, a
+    second graph beside it on another stream."""
+    n, nh, nkv = 6, 32, 8
+    sides = []
+    for side in range(2):
+        c = Cache(n, nkv, 700, cuda, seed=side)
+        fill(c, [60 + 3 * i + 200 * side for i in range(n)], 3 + side)
+        st = torch.cuda.Stream()
+        ctx, kvl, cu = c.ints(), c.ints(), cum([1] * n, cuda)
+        q, k, v = (torch.zeros((n, h, 64), dtype=torch.float16, device=cuda) for h in (nh, nkv, nkv))
+        st.wait_stream(torch.cuda.current_stream())
+
+        def step(c=c, ctx=ctx, kvl=kvl, cu=cu, q=q, k=k, v=v):
+            ops.kv_paged_append(k, v, cu, ctx, *c.t)
+            ctx.add_(1)
+            kvl.copy_(ctx)
+            return ops.attn_paged(q, cu, kvl, *c.t, max_q=1)
+
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            out = step()
+        sides.append((c, st, g, q, k, v, out, step))  # step holds the lengths' tensors
+    for i in range(8):
+        for j, (c, st, g, q, k, v, out, _) in enumerate(sides):
+            q.copy_(rnd(q.shape, 10 * i + j, cuda)), k.copy_(rnd(k.shape, 11 * i + j, cuda))
+            v.copy_(rnd(v.shape, 12 * i + j, cuda))
+        torch.cuda.synchronize()
+        for c, st, g, *_ in sides:
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for c, st, g, q, k, v, out, _ in sides:
+            c.lens = [x + 1 for x in c.lens]
+            c.check(q, [1] * n, out)
+    assert ops.paged_error() == 0
+
+
+def test_two_streams_at_once(cuda):
+    c = Cache(3, 8, 4000, cuda)
+    fill(c, [4000, 100, 2000], 3)
+    q1, q2 = rnd((3, 32, 64), 7, cuda), rnd((600, 32, 64), 8, cuda)
+    new2 = [300, 50, 250]
+    w1, w2 = c.attend(q1, [1] * 3, max_q=1), c.attend(q2, new2)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    cu1, cu2, kvl = cum([1] * 3, cuda), cum(new2, cuda), c.ints()
+    torch.cuda.synchronize()
+    for _ in range(10):
+        with torch.cuda.stream(s1):
+            a = ops.attn_paged(q1, cu1, kvl, *c.t, max_q=1)
+        with torch.cuda.stream(s2):
+            b = ops.attn_paged(q2, cu2, kvl, *c.t)
+        torch.cuda.synchronize()
+        assert torch.equal(a, w1) and torch.equal(b, w2)
+
+
+def test_empty_calls(cuda):
+    q, k = rnd((0, 8, 64), 1, cuda), rnd((0, 2, 64), 1, cuda)
+    assert ops.attn_varlen(q, k, k, cum([], cuda)).shape == (0, 8, 64)
+    assert ops.attn_varlen(q, k, k, cum([0, 0], cuda)).shape == (0, 8, 64)
+    c = Cache(2, 2, 64, cuda)
+    c.append(k, k, [0, 0])
+    assert c.attend(q, [0, 0]).shape == (0, 8, 64)
+    q, k = rnd((5, 8, 64), 1, cuda), rnd((5, 2, 64), 1, cuda)
+    out = torch.full_like(q, 2.0)
+    ops.attn_varlen(q, k, k, cum([0, 0, 0], cuda), out=out)
+    assert bool((out == 2).all()) and ops.paged_error() == 0
+
+
+def test_refusals(cuda):
+    c = Cache(2, 2, 64, cuda)
+    q, k, cu = rnd((2, 8, 64), 1, cuda), rnd((2, 2, 64), 1, cuda), cum([1, 1], cuda)
+    kvl = torch.ones(2, dtype=torch.int32, device=cuda)
+    with pytest.raises(ValueError, match="same tokens"):
+        ops.attn_varlen(q, k[:1], k[:1], cu)
+    with pytest.raises(CuinfError, match="multiple of nkv"):
+        ops.attn_varlen(q[:, :7], k, k, cu)
+    with pytest.raises(ValueError, match="heads must be contiguous"):
+        ops.attn_varlen(q[:, ::2], k, k, cu)
+    with pytest.raises(ValueError, match="64"):
+        ops.attn_varlen(q[..., :32], k, k, cu)
+    with pytest.raises(TypeError, match="cu_seqlens"):
+        ops.attn_varlen(q, k, k, cu.long())
+    with pytest.raises(CuinfError, match="16-byte aligned"):
+        wide = rnd((2, 8 * 64 + 4), 1, cuda)
+        ops.attn_varlen(wide[:, :512].view(2, 8, 64), k, k, cu)
+    with pytest.raises(ValueError, match="out must be"):
+        ops.attn_varlen(q, k, k, cu, out=q[:1].contiguous())
+    with pytest.raises(CuinfError, match="scale"):
+        ops.attn_varlen(q, k, k, cu, scale=0.0)
+    with pytest.raises(ValueError, match="kv heads"):
+        ops.kv_paged_append(k[:, :1], k[:, :1], cu, kvl, *c.t)
+    with pytest.raises(ValueError, match="ctx_lens"):
+        ops.kv_paged_append(k, k, cu, kvl[:1], *c.t)
+    with pytest.raises(ValueError, match="table"):
+        ops.attn_paged(q, cu, kvl, c.table[:1], *c.t[1:])
+    with pytest.raises(TypeError, match="kp8"):
+        ops.attn_paged(q, cu, kvl, c.table, c.kp8.half(), *c.t[2:])
+    with pytest.raises(ValueError, match="vtail"):
+        ops.attn_paged(q, cu, kvl, *c.t[:6], c.vtail[:1])
+    with pytest.raises(CuinfError, match="max_q"):
+        ops.attn_paged(q, cu, kvl, *c.t, max_q=0)
