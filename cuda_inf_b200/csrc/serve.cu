@@ -3,7 +3,11 @@
 // over that cache.
 #include <math.h>
 
+#include <algorithm>
+#include <mutex>
+
 #include "serve.cuh"
+#include "serve_tc.cuh"
 
 #define ST(s) ((cudaStream_t)(s))
 #define REQUIRE(cond, msg) \
@@ -148,93 +152,6 @@ __global__ void __launch_bounds__(256) k_paged_append(const AppendArgs A) {
 }
 
 // ---------------------------------------------------------------------------
-// attention, simple form: one warp per (row, query head), one key per lane,
-// running maximum and sum in fp32
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(128) k_attn_rows(const AttnArgs A) {
-    __shared__ float qs[4][CUINF_HD];
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * 4 + w;
-    const long long row = item / A.nh;
-    const int h = (int)(item % A.nh), hk = h / (A.nh / A.nkv);
-    if (row >= A.rows.n_rows) return;
-    int s = -1;
-    for (int b = 0; b < A.rows.n_seqs; b += 32) {
-        const int i = b + lane;
-        int x, y;
-        if (i < A.rows.n_seqs && !packed_range(A.rows, i, x, y)) atomicOr(A.err, SERVE_ERR_RANGE);
-        s += __popc(__ballot_sync(0xffffffffu, i < A.rows.n_seqs && A.rows.cu[i] <= row));
-    }
-    if (s < 0) return;
-    int a, b;
-    if (!packed_range(A.rows, s, a, b) && lane == 0) atomicOr(A.err, SERVE_ERR_RANGE);
-    if (row >= b) return;  // behind the last sequence
-    const int kv = A.kv_lens ? A.kv_lens[s] : b - a;
-    if (A.kv_lens && (kv < 0 || kv / SERVE_PAGE > A.kv.width || b - a > A.max_q)) {
-        if (lane == 0) atomicOr(A.err, SERVE_ERR_RANGE);
-        return;
-    }
-    const int pos = kv - (b - a) + (int)(row - a);
-    for (int d = lane; d < CUINF_HD; d += 32)
-        qs[w][d] = __half2float(A.q[row * A.q_stride + h * CUINF_HD + d]) * A.scale;
-    __syncwarp();
-    float m = -INFINITY, l = 0.f, o0 = 0.f, o1 = 0.f;
-    for (int j0 = 0; j0 <= pos; j0 += 32) {
-        const int j = j0 + lane;
-        const __half *kr = nullptr, *vr = nullptr;
-        const uint8_t *k8 = nullptr, *v8 = nullptr;
-        float ks = 1.f, vs = 1.f;
-        bool ok = j <= pos;
-        if (!A.kv_lens) {
-            kr = A.k + (size_t)(a + min(j, pos)) * A.k_stride + hk * CUINF_HD;
-            vr = A.v + (size_t)(a + min(j, pos)) * A.v_stride + hk * CUINF_HD;
-        } else if (j / SERVE_PAGE < kv / SERVE_PAGE) {
-            const int page = A.kv.table[(size_t)s * A.kv.width + j / SERVE_PAGE];
-            if (page >= 0 && page < A.kv.n_pages) {
-                const size_t blk = (size_t)page * A.nkv + hk;
-                k8 = A.kv.kp8 + blk * SERVE_PAGE_HEAD + (j % SERVE_PAGE) * CUINF_HD;
-                v8 = A.kv.vp8 + blk * SERVE_PAGE_HEAD + (j % SERVE_PAGE) * CUINF_HD;
-                ks = __half2float(A.kv.kps[blk]), vs = __half2float(A.kv.vps[blk]);
-            } else {
-                if (ok) atomicOr(A.err, SERVE_ERR_PAGE);
-                ok = false;
-            }
-        } else {
-            const size_t t = ((size_t)s * A.nkv + hk) * SERVE_PAGE_HEAD + (j % SERVE_PAGE) * CUINF_HD;
-            kr = A.kv.ktail + t, vr = A.kv.vtail + t;
-        }
-        float x = 0.f;
-        if (ok)
-            for (int d = 0; d < CUINF_HD; d++)
-                x += qs[w][d] * (kr ? __half2float(kr[d]) : ks * (float)*reinterpret_cast<const __nv_fp8_e4m3*>(k8 + d));
-        x = ok ? x : -INFINITY;
-        const float mn = fmaxf(m, warp_max(x));  // NaN scores pass the maximum by, and reach the sum through p
-        const float ref = mn == -INFINITY ? 0.f : mn;
-        const float f = __expf(m - ref);
-        const float p = ok ? __expf(x - ref) : 0.f;
-        l = l * f + p, o0 *= f, o1 *= f, m = mn;
-        for (int t = 0; t < 32; t++) {
-            const float pt = __shfl_sync(0xffffffffu, p, t);
-            const float st = __shfl_sync(0xffffffffu, vs, t);
-            const __half* vt = (const __half*)__shfl_sync(0xffffffffu, (unsigned long long)vr, t);
-            const uint8_t* v8t = (const uint8_t*)__shfl_sync(0xffffffffu, (unsigned long long)v8, t);
-            if (!__shfl_sync(0xffffffffu, (int)ok, t)) continue;
-            if (vt) {
-                o0 += pt * __half2float(vt[lane]), o1 += pt * __half2float(vt[lane + 32]);
-            } else {
-                o0 += pt * st * (float)*reinterpret_cast<const __nv_fp8_e4m3*>(v8t + lane);
-                o1 += pt * st * (float)*reinterpret_cast<const __nv_fp8_e4m3*>(v8t + lane + 32);
-            }
-        }
-    }
-    l = warp_sum(l);
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    __half* o = A.out + ((size_t)row * A.nh + h) * CUINF_HD;
-    o[lane] = __float2half_rn(o0 * inv);
-    o[lane + 32] = __float2half_rn(o1 * inv);
-}
-
-// ---------------------------------------------------------------------------
 // entry points
 // ---------------------------------------------------------------------------
 static int check_rows(const void* p, int64_t stride, int heads, const char* what) {
@@ -285,15 +202,86 @@ extern "C" int cuinf_kv_paged_append(const void* k, int64_t k_stride, const void
     return cuinf_launch_status();
 }
 
-static int launch_attn(const AttnArgs& A, cudaStream_t st) {
-    const long long blocks = ((long long)A.rows.n_rows * A.nh + 3) / 4;
-    REQUIRE(blocks < (1ll << 31), "too many rows");
-    k_attn_rows<<<(unsigned)blocks, 128, 0, st>>>(A);
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static EncodeTiledFn encode_fn() {
+    static EncodeTiledFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = (EncodeTiledFn)p;
+    });
+    return fn;
+}
+// fp16 rows [n_rows][heads][64], `stride` elements apart: boxes of bh heads x bt rows, 128-byte swizzle
+static int rows_map(CUtensorMap* m, const __half* base, int64_t stride, int heads, int n_rows, int bh, int bt) {
+    EncodeTiledFn fn = encode_fn();
+    REQUIRE(fn, "cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[3] = {CUINF_HD, (cuuint64_t)heads, (cuuint64_t)n_rows};
+    const cuuint64_t strides[2] = {CUINF_HD * 2, (cuuint64_t)stride * 2};
+    const cuuint32_t box[3] = {CUINF_HD, (cuuint32_t)bh, (cuuint32_t)bt}, one[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)base, dims, strides, box, one,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled refused the rows (stride below 2^39 elements?)");
+    return CUINF_OK;
+}
+
+// One CTA per SM, at most this many: the workspace holds two partial results of each.
+#define SERVE_MAX_CTAS 148
+// Items of at most this many key tiles are not cut.
+#define SERVE_WHOLE_TILES 4
+static bool sv_cuts(long long most_keys) { return most_keys > SERVE_WHOLE_TILES * SV_KT; }
+static int check_ws(const void* ws, size_t have, size_t need) {
+    REQUIRE(need == 0 || (ws && have >= need && ((uintptr_t)ws & 15) == 0),
+            "workspace: 16-byte aligned and of the size the _workspace_size call gives");
+    return CUINF_OK;
+}
+static int num_ctas(int* n) {
+    int dev = 0, sms = 0;
+    CUINF_TRY(cudaGetDevice(&dev));
+    CUINF_TRY(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    *n = std::min(sms, SERVE_MAX_CTAS);
+    return CUINF_OK;
+}
+
+template <bool PAGED>
+static int launch_tc(const AttnArgs& A, bool cuts, void* ws, cudaStream_t st) {
+    CUtensorMap qm, km, vm;
+    const int G = A.nh / A.nkv;
+    if (int rc = rows_map(&qm, A.q, A.q_stride, A.nh, A.rows.n_rows, G, 128 / G)) return rc;
+    km = vm = qm;
+    if (!PAGED) {
+        if (int rc = rows_map(&km, A.k, A.k_stride, A.nkv, A.rows.n_rows, 1, SV_KT)) return rc;
+        if (int rc = rows_map(&vm, A.v, A.v_stride, A.nkv, A.rows.n_rows, 1, SV_KT)) return rc;
+    }
+    int ctas;
+    if (int rc = num_ctas(&ctas)) return rc;
+    const SvWs W = sv_ws(ws, ctas);
+    CUINF_TRY(cudaFuncSetAttribute(k_serve_attn<PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int)SV_SMEM_BYTES));
+    k_serve_attn<PAGED><<<ctas, SvCfg<PAGED>::WARPS * 32, SV_SMEM_BYTES, st>>>(qm, km, vm, A, cuts, W);
+    if (int rc = cuinf_launch_status()) return rc;
+    if (!cuts) return CUINF_OK;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas, 4);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_combine, A, W, ctas));
     return cuinf_launch_status();
 }
 
 extern "C" size_t cuinf_attn_varlen_workspace_size(int n_seqs, int n_rows, int nh, int nkv) {
-    return 0;
+    return sv_cuts(n_rows) ? sv_ws_bytes(SERVE_MAX_CTAS) : 0;
 }
 extern "C" int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                                  int64_t v_stride, const int* cu_seqlens, int n_seqs, int n_rows, float scale,
@@ -312,13 +300,16 @@ extern "C" int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k,
     A.q_stride = q_stride, A.k_stride = k_stride, A.v_stride = v_stride;
     A.rows = {cu_seqlens, n_seqs, n_rows};
     A.scale = scale, A.out = (__half*)out, A.nh = nh, A.nkv = nkv;
+    const bool cuts = sv_cuts(n_rows);
+    if (int rc = check_ws(workspace, workspace_bytes, cuinf_attn_varlen_workspace_size(n_seqs, n_rows, nh, nkv)))
+        return rc;
     if (int rc = serve_err_ptr(&A.err)) return rc;
-    return launch_attn(A, ST(stream));
+    return launch_tc<false>(A, cuts, workspace, ST(stream));
 }
 
 extern "C" size_t cuinf_attn_paged_workspace_size(int n_seqs, int n_rows, int max_q, int nh, int nkv,
                                                   int table_width) {
-    return 0;
+    return sv_cuts(((long long)table_width + 1) * SERVE_PAGE) ? sv_ws_bytes(SERVE_MAX_CTAS) : 0;
 }
 extern "C" int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_seqlens, const int* kv_lens,
                                 int n_seqs, int n_rows, int max_q, const int* table, int table_width,
@@ -340,6 +331,10 @@ extern "C" int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_s
     A.kv = {(uint8_t*)kp8, (uint8_t*)vp8, (__half*)kps, (__half*)vps, (__half*)ktail, (__half*)vtail,
             table, table_width, n_pages, nkv};
     A.scale = scale, A.out = (__half*)out, A.nh = nh, A.nkv = nkv;
+    const bool cuts = sv_cuts(((long long)table_width + 1) * SERVE_PAGE);
+    if (int rc = check_ws(workspace, workspace_bytes,
+                          cuinf_attn_paged_workspace_size(n_seqs, n_rows, max_q, nh, nkv, table_width)))
+        return rc;
     if (int rc = serve_err_ptr(&A.err)) return rc;
-    return launch_attn(A, ST(stream));
+    return launch_tc<true>(A, cuts, workspace, ST(stream));
 }

@@ -1,0 +1,1069 @@
+// Attention of many new rows on the 5th-generation tensor cores: packed
+// prompts (fp16 keys and values by TMA) and chunks over the paged FP8 cache
+// (pages widened to fp16 by converter warps).
+//
+// Rows of the MMA are (token, query head of one kv head), TOK = 128 / G
+// tokens x G heads, so each key tile serves all heads that share it.  A work
+// item is one (sequence, kv head, block of 2 TOK tokens): two 128-row tiles
+// t = 0, 1 that run against the same 128-key tiles, one's softmax beside the
+// other's products.  Per key tile and row tile
+//   S = Q K^T        tcgen05.mma, 128 x 128 x 64, fp32 in TMEM
+//   P = exp2(c S - m) one thread per row: its 128 scores in registers, running
+//                    reference m and sum l in fp32, P rounded to fp16 (the MMA
+//                    operand) and written over S's first half in TMEM
+//   O += P V         tcgen05.mma with P from TMEM, 128 x 64 x 128, fp32 in TMEM
+// The reference m follows the row's maximum only when that has grown by more
+// than 2^THR since, so O is rescaled seldom (P stays within fp16's range).
+//
+// S has three TMEM buffers in rotation: product n + 2 is issued before the
+// softmax of n is done, so the softmax warps find their next S ready and the
+// kernel runs at their pace.  With head_dim 64 that pace is the exponentials'
+// (128 x 128 of them at 16 a clock: 1024 clocks, against 512 of MMA).
+//
+// The row blocks' key tiles of all sequences are laid end to end, and each CTA
+// takes an equal share of that line (or, where items are short, the items that
+// begin in it).  An item that is cut is joined by k_serve_combine from at most
+// two partial results per CTA.
+//
+// Masked places: scores are replaced, not added to.  A value that is no number
+// would pass a weight of zero (0 * NaN), so in tiles where some row masks some
+// key such values are set to zero in shared memory and noted by (column, first
+// key); the epilogue adds them to the rows that do attend them.
+#pragma once
+#include <cuda.h>
+#include "serve.cuh"
+
+#define SV_KT 128        // keys per tile
+#define SV_KST 4         // K and V stages
+#define SV_SC 16         // slots of the pages' scales (more tiles than can be in flight)
+#define SV_TILE_BYTES (SV_KT * CUINF_HD * 2)
+#define SV_TMEM_COLS 512
+#define SV_O_COL 384     // S/P buffers at 0, 128, 256; O of row tile t at 384 + 64 t
+#define SV_VEXP 16.f     // FP8: weights carry scale * 16 (fp16 keeps 146 * 16 * 2^THR)
+
+// One sequence as this kernel sees it: c new rows from row a on, the first at
+// position p0 of kv keys.
+struct SvSeq {
+    int a, c, p0, kv;
+};
+// A role's place on the line of key tiles.  One per warp, in shared memory: the
+// softmax warps have no registers to spare for it.
+struct SvItem {
+    int s, h, qb, nqb;  // sequence, kv head, row block of nqb
+    SvSeq q;
+    int t0, tb, te, n;  // first token of the block; key tiles [tb, te) of n
+    long long left;     // tiles left of the CTA's share
+};
+
+struct SvSmem {
+    uint64_t q_full[2], q_empty[2], k_full[SV_KST], k_empty[SV_KST], v_full[SV_KST], v_empty[SV_KST], v_ok[SV_KST];
+    uint64_t s_full[2][3], p_full[3], o_full[2], o_free[2], epi[2], conv, done;
+    uint32_t tmem;
+    int abort_;
+    float sc[SV_SC][4];  // FP8: K scale of the tile's two pages (negative: absent), V scales
+    int bad[2][3][CUINF_HD];  // by segment parity: first key whose value is +inf, -inf, NaN
+    int any_bad[2];
+    // start of this CTA's share
+    int s, h, qb, tile;
+    long long left;
+    long long scan[32];
+    SvItem item[16];
+};
+static constexpr size_t SV_Q_BYTES = 2 * SV_TILE_BYTES;  // both row tiles of an item
+static constexpr size_t SV_SMEM_BYTES = 1024 + 2 * SV_Q_BYTES + 2 * SV_KST * (size_t)SV_TILE_BYTES + sizeof(SvSmem);
+
+// Partial results: [CTA][2] slots of 256 rows; slot 0: the CTA's share began
+// inside the item, slot 1: it began the item and did not finish it.
+struct SvPart {
+    int valid, last, row0, tokens, h, pad[3];  // first token row, tokens of the item, kv head
+};
+struct SvWs {
+    SvPart* part;  // [ctas][2]
+    float* ml;     // [ctas][2][256][2]
+    float* o;      // [ctas][2][256][64]
+};
+static inline size_t sv_ws_bytes(int ctas) { return (size_t)ctas * 2 * (sizeof(SvPart) + 256 * 2 * 4 + 256 * 64 * 4); }
+__host__ __device__ inline SvWs sv_ws(void* p, int ctas) {
+    SvWs w;
+    w.o = (float*)p;
+    w.ml = w.o + (size_t)ctas * 2 * 256 * 64;
+    w.part = (SvPart*)(w.ml + (size_t)ctas * 2 * 256 * 2);
+    return w;
+}
+
+// ---- waits (bounded; the first that gives up raises the abort word) ----
+#define SV_WAIT_LIMIT_NS 500000000ull
+__device__ __forceinline__ bool sv_wait(uint64_t* bar, uint32_t parity, SvSmem* S, unsigned* err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (int k = 1;; k++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((k & 15) == 0) {
+            if (*(volatile int*)&S->abort_) return false;
+            if (globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS) break;
+        }
+    }
+    *(volatile int*)&S->abort_ = 1;
+    atomicOr(err, SERVE_ERR_WAIT);
+    return false;
+}
+__device__ __forceinline__ void sv_drain(uint64_t* bar, uint32_t parity, unsigned* err) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity))
+        if (globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS) {
+            atomicOr(err, SERVE_ERR_WAIT);
+            return;
+        }
+}
+
+// ---- tcgen05 ----
+__device__ __forceinline__ void sv_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void sv_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void sv_commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+// Shared-memory descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart:
+// a K-major operand (rows of 64 values), and equally V [key][64], an MN-major
+// operand whose one 64-wide atom spans the head.
+__device__ __forceinline__ uint64_t sv_desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+__device__ __forceinline__ void sv_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
+            d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void sv_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
+            d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// fp16 operands, fp32 accumulate, M = 128; bit 16: B is MN-major
+#define SV_IDESC_QK ((1u << 4) | ((uint32_t)(SV_KT >> 3) << 17) | (8u << 24))
+#define SV_IDESC_PV ((1u << 4) | (1u << 16) | ((uint32_t)(CUINF_HD >> 3) << 17) | (8u << 24))
+
+#define SV_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), \
+                    "=r"(r[o + 6]), "=r"(r[o + 7])
+#define SV_I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), \
+                    "r"(r[o + 6]), "r"(r[o + 7])
+__device__ __forceinline__ void sv_ld32(uint32_t t, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
+        : SV_R8(r, 0), SV_R8(r, 8), SV_R8(r, 16), SV_R8(r, 24)
+        : "r"(t));
+}
+__device__ __forceinline__ void sv_st32(uint32_t t, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::SV_I8(r, 0),
+        SV_I8(r, 8), SV_I8(r, 16), SV_I8(r, 24), "r"(t)
+        : "memory");
+}
+__device__ __forceinline__ void sv_st16(uint32_t t, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};\n" ::
+            SV_I8(r, 0),
+        SV_I8(r, 8), "r"(t)
+        : "memory");
+}
+__device__ __forceinline__ void sv_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void sv_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void sv_tma_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];\n" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// ---- packed fp32 pairs ----
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ float sv_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t sv_pack_h2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+// ---------------------------------------------------------------------------
+// the line of key tiles
+// ---------------------------------------------------------------------------
+// False: nothing for this kernel (empty, out of range, or few enough rows for
+// the single-token kernel).
+template <bool PAGED>
+__device__ __forceinline__ bool sv_seq(const AttnArgs& A, int s, SvSeq& q, bool report) {
+    int b;
+    bool fine = packed_range(A.rows, s, q.a, b);
+    q.c = b - q.a;
+    if (PAGED) {
+        q.kv = A.kv_lens[s];
+        if (q.c > 0 && (q.kv < 0 || q.kv / SERVE_PAGE > A.kv.width || q.c > A.max_q)) {
+            fine = false;
+            q.c = 0;
+        }
+        if (q.c * (A.nh / A.nkv) <= SERVE_FEW_ROWS) q.c = 0;
+    } else {
+        q.kv = q.c;
+    }
+    q.p0 = q.kv - q.c;
+    if (report && !fine) atomicOr(A.err, SERVE_ERR_RANGE);
+    return q.c > 0;
+}
+// key tiles of a block of rows that ends before row `end` (at least one: a
+// block whose rows have no key still writes its zeros)
+__device__ __forceinline__ int sv_tiles(const SvSeq& q, int end) {
+    return max(1, (q.p0 + end + SV_KT - 1) >> 7);
+}
+// sum over i < n of floor((a i + b) / m), all non-negative
+__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
+    long long r = 0;
+    while (n > 0) {
+        r += (n - 1) * n / 2 * (a / m);
+        a %= m;
+        r += n * (b / m);
+        b %= m;
+        const long long y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const long long t = m;
+        m = a;
+        a = t;
+    }
+    return r;
+}
+// key tiles of all row blocks of one kv head of the sequence
+__device__ __forceinline__ long long sv_head_tiles(const SvSeq& q, int tq) {
+    const int m = (q.c + tq - 1) / tq - 1;  // blocks before the last
+    const int z = q.p0 < 0 ? min(m, -q.p0 / tq) : 0;  // of these, without a key
+    return z + floor_sum(m - z, SV_KT, tq, (long long)q.p0 + (long long)tq * (z + 1) + SV_KT - 1) + sv_tiles(q, q.c);
+}
+
+// Finds the CTA's share [W i / N, W (i+1) / N) of the line of W tiles and its
+// first item.  All threads call; the result is in S (left = 0: nothing to do).
+template <bool PAGED>
+__device__ void sv_start(const AttnArgs& A, SvSmem* S, int tq, int n_ctas) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
+    long long total = 0, beg = 0, end = 0, base = 0;
+    if (tid == 0) S->left = 0;
+    for (int pass = 0; pass < 2; pass++) {
+        for (int b = 0; b < A.rows.n_seqs; b += nt) {
+            const int s = b + tid;
+            SvSeq q;
+            long long w = 0;
+            if (s < A.rows.n_seqs && sv_seq<PAGED>(A, s, q, pass == 0 && blockIdx.x == 0))
+                w = sv_head_tiles(q, tq) * A.nkv;
+            long long x = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) S->scan[warp] = x;
+            __syncthreads();
+            long long before = 0, all = 0;
+            for (int i = 0; i < nw; i++) {
+                const long long y = S->scan[i];
+                if (i < warp) before += y;
+                all += y;
+            }
+            if (pass == 0) {
+                total += all;
+            } else {
+                const long long lo = base + before + x - w;
+                if (end > beg && beg >= lo && beg < lo + w) {
+                    S->s = s;
+                    S->left = end - beg;
+                    S->scan[31] = beg - lo;
+                }
+                base += all;
+            }
+        }
+        if (pass == 0) {
+            beg = total * blockIdx.x / n_ctas;
+            end = total * (blockIdx.x + 1) / n_ctas;
+        }
+    }
+    __syncthreads();
+    if (warp == 0 && S->left > 0) {
+        SvSeq q;
+        sv_seq<PAGED>(A, S->s, q, false);
+        const long long per = sv_head_tiles(q, tq);
+        long long rem = S->scan[31];
+        const int h = (int)(rem / per);
+        rem -= h * per;
+        const int nqb = (q.c + tq - 1) / tq;
+        for (int b = 0; b < nqb; b += 32) {
+            const int qb = b + lane;
+            const int w = qb < nqb ? sv_tiles(q, min((qb + 1) * tq, q.c)) : 0;
+            int x = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            const unsigned hit = __ballot_sync(0xffffffffu, rem < x);
+            if (hit) {
+                if (lane == __ffs(hit) - 1) {
+                    S->h = h;
+                    S->qb = qb;
+                    S->tile = (int)(rem - (x - w));
+                }
+                break;
+            }
+            rem -= __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+    __syncthreads();
+}
+
+// Walks the items of the CTA's share; every role runs its own (one lane calls).
+__device__ __forceinline__ void sv_item(SvItem& w, int tq, int split) {
+    w.t0 = w.qb * tq;
+    w.n = sv_tiles(w.q, min(w.t0 + tq, w.q.c));
+    w.te = split ? (int)min((long long)w.n, w.tb + w.left) : w.n;
+}
+template <bool PAGED>
+__device__ __forceinline__ void sv_advance(const AttnArgs& A, SvItem& w, int tq, int split) {
+    if (++w.qb >= w.nqb) {
+        w.qb = 0;
+        if (++w.h >= A.nkv) {
+            w.h = 0;
+            SvSeq q;
+            int s = w.s;
+            do s++;
+            while (s < A.rows.n_seqs && !sv_seq<PAGED>(A, s, q, false));
+            if (s >= A.rows.n_seqs) {
+                w.left = 0;
+                return;
+            }
+            w.s = s, w.q = q;
+            w.nqb = (q.c + tq - 1) / tq;
+        }
+    }
+    w.tb = 0;
+    sv_item(w, tq, split);
+}
+template <bool PAGED>
+__device__ __forceinline__ void sv_first(const AttnArgs& A, const SvSmem* S, SvItem& w, int tq, int split) {
+    w.s = S->s, w.h = S->h, w.qb = S->qb, w.left = S->left, w.tb = S->tile;
+    if (w.left <= 0) return;
+    SvSeq q;
+    sv_seq<PAGED>(A, w.s, q, false);
+    w.q = q;
+    w.nqb = (q.c + tq - 1) / tq;
+    sv_item(w, tq, split);
+    if (!split && w.tb > 0) {  // the item belongs to the share in which it begins
+        w.left -= w.n - w.tb;
+        if (w.left > 0) sv_advance<PAGED>(A, w, tq, split);
+    }
+}
+template <bool PAGED>
+__device__ __forceinline__ void sv_next(const AttnArgs& A, SvItem& w, int tq, int split) {
+    w.left -= w.te - w.tb;
+    if (w.left > 0) sv_advance<PAGED>(A, w, tq, split);
+}
+// the same for all lanes of a warp
+template <bool PAGED>
+__device__ __forceinline__ void sv_next_warp(const AttnArgs& A, SvItem& w, int tq, int split) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) sv_next<PAGED>(A, w, tq, split);
+    __syncwarp();
+}
+
+// ---------------------------------------------------------------------------
+// roles
+// ---------------------------------------------------------------------------
+template <bool PAGED>
+struct SvCfg {
+    // softmax warps 0-7; packed: 8 TMA, 9 MMA, 10 value check (11 idle);
+    // paged: 8-11 converters, 12 Q by TMA, 13 MMA (14, 15 idle)
+    static constexpr int WARPS = PAGED ? 16 : 12;
+    static constexpr int MMA_WARP = PAGED ? 13 : 9;
+    static constexpr int Q_WARP = PAGED ? 12 : 8;
+    // registers: 512 x 128 = 256 x 184 + 256 x 72; 384 x 168 = 256 x 208 + 128 x 88
+    static constexpr int REG_HI = PAGED ? 184 : 208;
+    static constexpr int REG_LO = PAGED ? 72 : 88;
+    static constexpr float THR = PAGED ? 3.f : 8.f;
+};
+
+// Does some row of the block mask some key of the tile?
+__device__ __forceinline__ bool sv_masked(const SvSeq& q, int t0, int tile) {
+    return (tile + 1) * SV_KT > q.p0 + t0 + 1;
+}
+
+// ---- paged: pages widened to fp16 tiles by four warps ----
+__device__ __forceinline__ uint32_t sv_e4m3x2(uint32_t two) {  // low 16 bits: two codes -> two halves, exact
+    uint32_t r;
+    asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(r) : "r"(two));
+    return r;
+}
+template <int N>
+__device__ __forceinline__ bool sv_not_finite(const uint32_t (&h)[N]) {  // 0 * x is NaN for what is no number
+    uint32_t x = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) x = hfma2_u(h[i], 0, x);
+    const __half2 y = *reinterpret_cast<const __half2*>(&x);
+    return __hisnan(y.x) || __hisnan(y.y);
+}
+// Values that are no numbers, of key `key`, columns d0..: noted and set to zero (rare).
+template <int N>
+__device__ __forceinline__ void sv_note_bad(SvSmem* S, int par, int key, int d0, uint32_t (&h)[N]) {
+#pragma unroll
+    for (int i = 0; i < 2 * N; i++) {
+        const uint32_t bits = h[i >> 1] >> (16 * (i & 1)) & 0xffffu;
+        if ((bits & 0x7c00u) == 0x7c00u) {
+            atomicMin(&S->bad[par][(bits & 0x3ffu) ? 2 : bits & 0x8000u ? 1 : 0][d0 + i], key);
+            S->any_bad[par] = 1;
+            h[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+        }
+    }
+}
+struct SvConv {
+    const AttnArgs& A;
+    SvSmem* S;
+    int tid;
+    // chunk u = tid + 128 i of a group's 256: row u / 4, 16 values from 16 (u % 4)
+    __device__ __forceinline__ void load(const uint8_t* pool, int page, int h, uint4* x) const {
+        if (page < 0) {
+            x[0] = x[1] = make_uint4(0, 0, 0, 0);
+            return;
+        }
+        const uint4* src = reinterpret_cast<const uint4*>(pool + ((size_t)page * A.nkv + h) * SERVE_PAGE_HEAD) + tid;
+        x[0] = __ldg(src);
+        x[1] = __ldg(src + 128);
+    }
+    template <bool CHECK>
+    __device__ __forceinline__ void store(unsigned char* dst, int g, const uint4* x, int par, int key0) const {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int u = tid + 128 * i, r = 64 * g + (u >> 2), c = 2 * (u & 3);
+            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+            uint32_t h[8];
+#pragma unroll
+            for (int j = 0; j < 4; j++) h[2 * j] = sv_e4m3x2(w[j]), h[2 * j + 1] = sv_e4m3x2(w[j] >> 16);
+            if (CHECK && sv_not_finite(h)) sv_note_bad(S, par, key0 + r, 8 * c, h);
+            unsigned char* row = dst + r * 128;
+            *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        }
+    }
+    // the fp16 tail (rows behind `rest` are zero)
+    template <bool CHECK>
+    __device__ __forceinline__ void tail(unsigned char* dst, int g, const __half* src, int rest, int par, int key0) const {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int u = tid + 128 * i, r = u >> 3, c = u & 7, rr = 64 * g + r;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (r < rest) x = *reinterpret_cast<const uint4*>(src + r * CUINF_HD + c * 8);
+            if (CHECK) {
+                uint32_t h[4] = {x.x, x.y, x.z, x.w};
+                if (sv_not_finite(h)) {
+                    sv_note_bad(S, par, key0 + rr, 8 * c, h);
+                    x = make_uint4(h[0], h[1], h[2], h[3]);
+                }
+            }
+            *reinterpret_cast<uint4*>(dst + rr * 128 + ((c ^ (rr & 7)) << 4)) = x;
+        }
+    }
+};
+// page of group g: -1 absent, -2 the tail
+__device__ __forceinline__ int sv_page(const AttnArgs& A, const SvSeq& q, int s, int g) {
+    const int ng = q.kv / SERVE_PAGE;
+    if (g >= ng) return g == ng && q.kv % SERVE_PAGE ? -2 : -1;
+    return __ldg(A.kv.table + (size_t)s * A.kv.width + g);
+}
+__device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq, int split, SvSmem* S,
+                                           unsigned char* Ks, unsigned char* Vs, int tid) {
+    const int lane = tid & 31, warp = tid >> 5;
+    const SvConv cv = {A, S, tid};
+    uint32_t seg = 0, kt = 0;
+    bool ok = true;
+    // an index outside the pool: reported once per use, then absent
+    auto valid = [&](int page, int g) -> int {
+        if (g < w.q.kv / SERVE_PAGE && (page < 0 || page >= A.kv.n_pages)) {
+            if (tid == 0) atomicOr(A.err, SERVE_ERR_PAGE);
+            return -3;
+        }
+        return page;
+    };
+    for (; ok && w.left > 0; sv_next_warp<true>(A, w, tq, split), seg++) {
+        const int par = seg & 1;
+        // this parity's notes were last read two segments ago
+        if (seg >= 2 && !(ok = sv_wait(&S->epi[par], ((seg >> 1) - 1) & 1, S, A.err))) break;
+        if (warp == 0) {
+            for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[par][0][0])[u] = 0x7fffffff;
+            if (lane == 0) S->any_bad[par] = 0;
+        }
+        __threadfence_block();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S->conv);
+        if (!(ok = sv_wait(&S->conv, seg & 1, S, A.err))) break;
+
+        const size_t tail = ((size_t)w.s * A.nkv + w.h) * SERVE_PAGE_HEAD;
+        const int rest = w.q.kv % SERVE_PAGE;
+        int pg[2], pn[2];  // pages of this tile and (as read) of the next
+        uint4 kx[2][2], vx[2][2];
+        float sc = 0.f, sn = 0.f;  // threads 0..3: (K, V) x (group 0, 1)
+        auto scale = [&](const int* p) -> float {
+            const int page = p[tid & 1];
+            if (page == -3) return -1.f;
+            if (page < 0) return 1.f;
+            return __half2float((tid & 2 ? A.kv.vps : A.kv.kps)[(size_t)page * A.nkv + w.h]);
+        };
+#pragma unroll
+        for (int g = 0; g < 2; g++) pg[g] = valid(sv_page(A, w.q, w.s, 2 * w.tb + g), 2 * w.tb + g);
+#pragma unroll
+        for (int g = 0; g < 2; g++) cv.load(A.kv.kp8, pg[g], w.h, kx[g]), cv.load(A.kv.vp8, pg[g], w.h, vx[g]);
+        if (tid < 4) sc = scale(pg);
+#pragma unroll
+        for (int g = 0; g < 2; g++) pn[g] = w.tb + 1 < w.te ? sv_page(A, w.q, w.s, 2 * (w.tb + 1) + g) : -1;
+        for (int i = w.tb; i < w.te; i++, kt++) {
+            const uint32_t st = kt % SV_KST, ph = ((kt / SV_KST) & 1) ^ 1;
+            const bool masked = sv_masked(w.q, w.t0, i);
+            int pq[2];  // the next tile's pages, checked
+#pragma unroll
+            for (int g = 0; g < 2; g++) pq[g] = i + 1 < w.te ? valid(pn[g], 2 * (i + 1) + g) : -1;
+            if (tid < 4) sn = scale(pq);
+#pragma unroll
+            for (int g = 0; g < 2; g++) pn[g] = i + 2 < w.te ? sv_page(A, w.q, w.s, 2 * (i + 2) + g) : -1;
+            if (!(ok = sv_wait(&S->k_empty[st], ph, S, A.err))) break;
+            unsigned char* kd = Ks + st * SV_TILE_BYTES;
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                if (pg[g] == -2)
+                    cv.tail<false>(kd, g, A.kv.ktail + tail, rest, 0, 0);
+                else
+                    cv.store<false>(kd, g, kx[g], 0, 0);
+            }
+            if (tid < 4) S->sc[kt % SV_SC][tid] = sc;
+            sc = sn;
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S->k_full[st]);
+#pragma unroll
+            for (int g = 0; g < 2; g++) cv.load(A.kv.kp8, pq[g], w.h, kx[g]);
+            if (!(ok = sv_wait(&S->v_empty[st], ph, S, A.err))) break;
+            unsigned char* vd = Vs + st * SV_TILE_BYTES;
+#pragma unroll
+            for (int g = 0; g < 2; g++) {
+                if (masked) {
+                    if (pg[g] == -2)
+                        cv.tail<true>(vd, g, A.kv.vtail + tail, rest, par, i * SV_KT);
+                    else
+                        cv.store<true>(vd, g, vx[g], par, i * SV_KT);
+                } else if (pg[g] == -2) {
+                    cv.tail<false>(vd, g, A.kv.vtail + tail, rest, 0, 0);
+                } else {
+                    cv.store<false>(vd, g, vx[g], 0, 0);
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+            __threadfence_block();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S->v_full[st]);
+#pragma unroll
+            for (int g = 0; g < 2; g++) cv.load(A.kv.vp8, pq[g], w.h, vx[g]), pg[g] = pq[g];
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&S->epi[par]);
+    }
+}
+
+template <bool PAGED>
+__global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
+    k_serve_attn(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
+                 const __grid_constant__ CUtensorMap vmap, const AttnArgs A, const int split, const SvWs W) {
+    using C = SvCfg<PAGED>;
+    extern __shared__ __align__(1024) unsigned char sv_raw[];
+    unsigned char* sm = sv_raw + ((1024 - (smem_u32(sv_raw) & 1023)) & 1023);
+    unsigned char* Qs = sm;
+    unsigned char* Ks = Qs + 2 * SV_Q_BYTES;
+    unsigned char* Vs = Ks + SV_KST * SV_TILE_BYTES;
+    SvSmem* S = reinterpret_cast<SvSmem*>(Vs + SV_KST * SV_TILE_BYTES);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = A.nh / A.nkv, TOK = 128 / G, tq = 2 * TOK;
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&S->q_full[i], 1), mbar_init(&S->q_empty[i], 1);
+            mbar_init(&S->o_full[i], 1), mbar_init(&S->o_free[i], 4), mbar_init(&S->epi[i], PAGED ? 12 : 9);
+            S->any_bad[i] = 0;
+        }
+        for (int i = 0; i < SV_KST; i++) {
+            mbar_init(&S->k_full[i], PAGED ? 4 : 1), mbar_init(&S->k_empty[i], 1);
+            mbar_init(&S->v_full[i], PAGED ? 4 : 1), mbar_init(&S->v_empty[i], 1);
+            mbar_init(&S->v_ok[i], 1);
+        }
+        for (int i = 0; i < 3; i++)
+            mbar_init(&S->s_full[0][i], 1), mbar_init(&S->s_full[1][i], 1), mbar_init(&S->p_full[i], 4);
+        mbar_init(&S->conv, 4);
+        mbar_init(&S->done, 1);
+        S->abort_ = 0;
+    }
+    if (warp == C::MMA_WARP) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&S->tmem)),
+                     "r"(SV_TMEM_COLS)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+    }
+    if (split && tid < 2) W.part[blockIdx.x * 2 + tid].valid = 0;
+    sv_start<PAGED>(A, S, tq, gridDim.x);
+    sv_fence_before();
+    __syncthreads();
+    sv_fence_after();
+    const uint32_t tmem = S->tmem;
+    SvItem& w = S->item[warp];
+    if (lane == 0) sv_first<PAGED>(A, S, w, tq, split);
+    __syncwarp();
+
+    if (warp < 8) {
+        // ---- softmax and epilogue: one thread per row of row tile t ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(C::REG_HI));
+        const int t = warp >> 2, row = tid & 127;
+        const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t o_addr = lane_base + SV_O_COL + t * CUINF_HD;
+        const float c2 = A.scale * 1.44269504088896340736f;  // scores in powers of two
+        uint32_t n = 0, ops = 0, tiles = 0, seg = 0;
+        uint32_t sbits = 0;  // phases of s_full[t] by buffer
+        bool ok = true;
+        for (; ok && w.left > 0; sv_next_warp<PAGED>(A, w, tq, split), seg++) {
+            const int nt = w.te - w.tb;
+            const bool act1 = w.t0 + TOK < w.q.c;
+            // all who arrive at a segment's epi barrier have seen the one before of the same parity complete
+            if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, S, A.err))) break;
+            if (t == 1 && !act1) {
+                n += nt, tiles += nt;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S->epi[seg & 1]);
+                continue;
+            }
+            const int tok = w.t0 + t * TOK + row / G;
+            const bool live_row = row < TOK * G && tok < w.q.c;
+            const int pos = live_row ? w.q.p0 + tok : -1;
+            float m = -INFINITY;
+            uint64_t l2 = 0;  // two partial sums
+            for (int i = w.tb; i < w.te; i++, ops++, tiles++) {
+                const uint32_t nn = n + (act1 ? 2 * (i - w.tb) + t : i - w.tb), b = nn % 3;
+                if (!(ok = sv_wait(&S->s_full[t][b], (sbits >> b) & 1, S, A.err))) break;
+                sbits ^= 1u << b;
+                sv_fence_after();
+                uint32_t sr[128];
+                const uint32_t s_addr = lane_base + b * 128;
+#pragma unroll
+                for (int j = 0; j < 4; j++) sv_ld32(s_addr + 32 * j, sr + 32 * j);
+                float kc[2] = {c2, c2}, vc[2] = {1.f, 1.f};
+                bool gone[2] = {false, false};
+                if (PAGED) {
+                    const float* sc = S->sc[tiles % SV_SC];
+#pragma unroll
+                    for (int g = 0; g < 2; g++) {
+                        gone[g] = sc[g] < 0.f;
+                        kc[g] = c2 * sc[g];
+                        if (kc[g] == 0.f) kc[g] = 1e-30f;  // a page of zeros: -inf * 0 is no number
+                        vc[g] = SV_VEXP * sc[2 + g];
+                    }
+                }
+                sv_wait_ld();
+                float* s = reinterpret_cast<float*>(sr);
+                if (sv_masked(w.q, w.t0 + t * TOK, i)) {
+                    const int lim = pos - i * SV_KT;  // last key of the tile that the row attends
+#pragma unroll
+                    for (int j = 0; j < 128; j++) s[j] = j <= lim ? s[j] : -INFINITY;
+                    if (PAGED) {  // a page's scale that is no number reaches only rows that attend the page
+                        if (lim < 0) kc[0] = c2, vc[0] = 0.f;
+                        if (lim < 64) kc[1] = c2, vc[1] = 0.f;
+                    }
+                }
+                if (PAGED) {
+#pragma unroll
+                    for (int g = 0; g < 2; g++)
+                        if (gone[g]) {
+                            kc[g] = c2, vc[g] = 0.f;
+#pragma unroll
+                            for (int j = 0; j < 64; j++) s[64 * g + j] = -INFINITY;
+                        }
+                }
+                float mx[2];
+#pragma unroll
+                for (int g = 0; g < 2; g++) {
+                    float a0 = s[64 * g], a1 = s[64 * g + 1], a2 = s[64 * g + 2], a3 = s[64 * g + 3];
+#pragma unroll
+                    for (int j = 4; j < 64; j += 4) {
+                        a0 = fmaxf(a0, s[64 * g + j]), a1 = fmaxf(a1, s[64 * g + j + 1]);
+                        a2 = fmaxf(a2, s[64 * g + j + 2]), a3 = fmaxf(a3, s[64 * g + j + 3]);
+                    }
+                    mx[g] = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)) * kc[g];
+                }
+                const float x = fmaxf(mx[0], mx[1]);
+                if (i == w.tb) {
+                    m = x;
+                } else if (__any_sync(0xffffffffu, x > m + C::THR)) {
+                    // rare: the reference follows the maximum, sum and O with it
+                    const float mn = fmaxf(m, x);
+                    const float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
+                    m = mn;
+                    l2 = f2_mul(l2, f2_pack(f, f));
+                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, S, A.err))) break;
+                    sv_fence_after();
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        uint32_t o[32];
+                        sv_ld32(o_addr + 32 * j, o);
+                        sv_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        sv_st32(o_addr + 32 * j, o);
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                const uint64_t nm = f2_pack(-ref, -ref);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const int g = j >> 1;
+                    const uint64_t cc = f2_pack(kc[g], kc[g]), vv = f2_pack(vc[g], vc[g]);
+                    uint32_t pk[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        uint64_t y = f2_fma(f2_pack(s[32 * j + 2 * e], s[32 * j + 2 * e + 1]), cc, nm);
+                        float y0, y1;
+                        f2_unpack(y, y0, y1);
+                        y0 = sv_exp2(y0), y1 = sv_exp2(y1);
+                        y = f2_pack(y0, y1);
+                        l2 = f2_add(l2, y);
+                        if (PAGED) f2_unpack(f2_mul(y, vv), y0, y1);
+                        pk[e] = sv_pack_h2(y0, y1);
+                    }
+                    sv_st16(s_addr + 16 * j, pk);
+                }
+                sv_wait_st();
+                sv_fence_before();
+                // every phase of o_full is seen (a parity tells only neighbouring phases apart); the last
+                // product is long done here
+                if (i > w.tb && !(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, S, A.err))) break;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S->p_full[b]);
+            }
+            if (!ok) break;
+            n += act1 ? 2 * nt : nt;
+            // ---- epilogue of the item (or of the CTA's part of it) ----
+            if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, S, A.err))) break;
+            sv_fence_after();
+            uint32_t o[64];
+            sv_ld32(o_addr, o);
+            sv_ld32(o_addr + 32, o + 32);
+            sv_wait_ld();
+            sv_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S->o_free[t]);
+            float la, lb;
+            f2_unpack(l2, la, lb);
+            const float l = la + lb;
+            float* of = reinterpret_cast<float*>(o);
+            const float vs = PAGED ? 1.f / SV_VEXP : 1.f;
+            if (S->any_bad[seg & 1]) {
+                const int(*bad)[CUINF_HD] = S->bad[seg & 1];
+#pragma unroll
+                for (int d = 0; d < 64; d++) {
+                    if (bad[0][d] <= pos) of[d] += INFINITY;
+                    if (bad[1][d] <= pos) of[d] -= INFINITY;
+                    if (bad[2][d] <= pos) of[d] = NAN;
+                }
+            }
+            const bool whole = w.tb == 0 && w.te == w.n;
+            if (whole) {
+                if (live_row) {
+                    const float inv = l == 0.f ? 0.f : vs / l;
+                    uint4* dst = reinterpret_cast<uint4*>(A.out + ((size_t)(w.q.a + tok) * A.nh + w.h * G + row % G) *
+                                                                      CUINF_HD);
+#pragma unroll
+                    for (int d = 0; d < 64; d += 8) {
+                        uint4 r;
+                        r.x = sv_pack_h2(of[d] * inv, of[d + 1] * inv);
+                        r.y = sv_pack_h2(of[d + 2] * inv, of[d + 3] * inv);
+                        r.z = sv_pack_h2(of[d + 4] * inv, of[d + 5] * inv);
+                        r.w = sv_pack_h2(of[d + 6] * inv, of[d + 7] * inv);
+                        dst[d / 8] = r;
+                    }
+                }
+            } else {
+                const size_t slot = (size_t)blockIdx.x * 2 + (w.tb == 0);
+                if (live_row) {
+                    const size_t r = slot * 256 + t * 128 + row;
+                    reinterpret_cast<float2*>(W.ml)[r] = make_float2(m, l);
+                    float4* dst = reinterpret_cast<float4*>(W.o + r * 64);
+#pragma unroll
+                    for (int d = 0; d < 64; d += 4)
+                        dst[d / 4] = make_float4(of[d] * vs, of[d + 1] * vs, of[d + 2] * vs, of[d + 3] * vs);
+                }
+                if (t == 0 && row == 0) {
+                    SvPart p;
+                    p.valid = 1, p.last = w.te == w.n, p.row0 = w.q.a + w.t0, p.tokens = min(tq, w.q.c - w.t0);
+                    p.h = w.h;
+                    W.part[slot] = p;
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S->epi[seg & 1]);
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(C::REG_LO));
+        if (warp == C::Q_WARP) {
+            // ---- Q (and, packed, K and V) by TMA ----
+            uint32_t seg = 0, kt = 0, nq = 0, nk = 0, nv = 0;  // copies issued
+            bool ok = true;
+            for (; ok && w.left > 0; sv_next_warp<PAGED>(A, w, tq, split), seg++) {
+                const uint32_t qsl = seg & 1;
+                bool r = true;
+                if (lane == 0) {
+                    r = sv_wait(&S->q_empty[qsl], ((seg >> 1) & 1) ^ 1, S, A.err);
+                    if (r) {
+                        const bool act1 = w.t0 + TOK < w.q.c;
+                        mbar_arrive_expect_tx(&S->q_full[qsl], (uint32_t)(TOK * G * 128) * (act1 ? 2 : 1));
+                        for (int t = 0; t < (act1 ? 2 : 1); t++)
+                            sv_tma_3d(Qs + qsl * SV_Q_BYTES + t * SV_TILE_BYTES, &qmap, 0, w.h * G,
+                                      w.q.a + w.t0 + t * TOK, &S->q_full[qsl]);
+                        nq++;
+                    }
+                }
+                if (!(ok = __shfl_sync(0xffffffffu, (int)r, 0) != 0)) break;
+                if (PAGED) continue;
+                for (int i = w.tb; i < w.te; i++, kt++) {
+                    const uint32_t st = kt % SV_KST, ph = ((kt / SV_KST) & 1) ^ 1;
+                    if (lane == 0) {
+                        r = sv_wait(&S->k_empty[st], ph, S, A.err);
+                        if (r) {
+                            mbar_arrive_expect_tx(&S->k_full[st], SV_TILE_BYTES);
+                            sv_tma_3d(Ks + st * SV_TILE_BYTES, &kmap, 0, w.h, w.q.a + i * SV_KT, &S->k_full[st]);
+                            nk++;
+                            r = sv_wait(&S->v_empty[st], ph, S, A.err);
+                        }
+                        if (r) {
+                            mbar_arrive_expect_tx(&S->v_full[st], SV_TILE_BYTES);
+                            sv_tma_3d(Vs + st * SV_TILE_BYTES, &vmap, 0, w.h, w.q.a + i * SV_KT, &S->v_full[st]);
+                            nv++;
+                        }
+                    }
+                    if (!(ok = __shfl_sync(0xffffffffu, (int)r, 0) != 0)) break;
+                }
+            }
+            // what is in flight lands before the CTA can exit
+            if (lane == 0) {
+                for (uint32_t k = nq < 2 ? 0 : nq - 2; k < nq; k++) sv_drain(&S->q_full[k & 1], (k >> 1) & 1, A.err);
+                for (uint32_t k = nk < SV_KST ? 0 : nk - SV_KST; k < nk; k++)
+                    sv_drain(&S->k_full[k % SV_KST], (k / SV_KST) & 1, A.err);
+                for (uint32_t k = nv < SV_KST ? 0 : nv - SV_KST; k < nv; k++)
+                    sv_drain(&S->v_full[k % SV_KST], (k / SV_KST) & 1, A.err);
+            }
+            __syncwarp();
+        } else if (warp == C::MMA_WARP) {
+            // ---- products: S of op n, then O of op n - 2 ----
+            if (lane == 0) {
+                uint32_t n = 0, seg = 0, kt = 0, pv = 0, vt = 0;
+                uint32_t segs[2] = {0, 0};  // segments of row tile t so far
+                // ops whose PV is still to come: bit 0 t, 1 first of its segment, 2 first and 3 last op of
+                // the key tile
+                uint32_t pend[3] = {0, 0, 0};
+                bool ok = true;
+                auto issue_pv = [&]() -> bool {
+                    const uint32_t op = pend[pv % 3], b = pv % 3, t = op & 1, st = vt % SV_KST;
+                    if ((op & 2) && segs[t] > 0 && !sv_wait(&S->o_free[t], (segs[t] - 1) & 1, S, A.err)) return false;
+                    if (op & 2) segs[t]++;
+                    if (op & 4) {
+                        if (!sv_wait(&S->v_full[st], (vt / SV_KST) & 1, S, A.err)) return false;
+                        if (!PAGED && !sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, S, A.err)) return false;
+                    }
+                    if (!sv_wait(&S->p_full[b], (pv / 3) & 1, S, A.err)) return false;
+                    sv_fence_after();
+                    const uint32_t va = smem_u32(Vs + st * SV_TILE_BYTES);
+#pragma unroll
+                    for (int k = 0; k < SV_KT / 16; k++)
+                        sv_mma_ts(tmem + SV_O_COL + t * CUINF_HD, tmem + b * 128 + 8 * k, sv_desc(va + k * 16 * 128),
+                                  SV_IDESC_PV, !((op & 2) && k == 0));
+                    sv_commit(&S->o_full[t]);
+                    if (op & 8) {
+                        sv_commit(&S->v_empty[st]);
+                        vt++;
+                    }
+                    pv++;
+                    return true;
+                };
+                // What comes next may wait for what is pending (notes of values that are no numbers are reused
+                // two segments on), so nothing stays pending while an input is awaited.
+                auto wait_input = [&](uint64_t* bar, uint32_t parity) -> bool {
+                    if (mbar_test_wait(bar, parity)) return true;
+                    while (pv < n)
+                        if (!issue_pv()) return false;
+                    return sv_wait(bar, parity, S, A.err);
+                };
+                for (; ok && w.left > 0; sv_next<PAGED>(A, w, tq, split), seg++) {
+                    const bool act1 = w.t0 + TOK < w.q.c;
+                    if (!(ok = wait_input(&S->q_full[seg & 1], (seg >> 1) & 1))) break;
+                    for (int i = w.tb; ok && i < w.te; i++, kt++) {
+                        const uint32_t st = kt % SV_KST;
+                        if (!(ok = wait_input(&S->k_full[st], (kt / SV_KST) & 1))) break;
+                        for (int t = 0; t < (act1 ? 2 : 1); t++) {
+                            const uint32_t b = n % 3;
+                            sv_fence_after();
+                            const uint32_t qa = smem_u32(Qs + (seg & 1) * SV_Q_BYTES + t * SV_TILE_BYTES);
+                            const uint32_t ka = smem_u32(Ks + st * SV_TILE_BYTES);
+#pragma unroll
+                            for (int k = 0; k < CUINF_HD / 16; k++)
+                                sv_mma_ss(tmem + b * 128, sv_desc(qa + 32 * k), sv_desc(ka + 32 * k), SV_IDESC_QK,
+                                          k != 0);
+                            sv_commit(&S->s_full[t][b]);
+                            const bool last_t = t == (act1 ? 1 : 0);
+                            if (last_t) {
+                                sv_commit(&S->k_empty[st]);
+                                if (i == w.te - 1) sv_commit(&S->q_empty[seg & 1]);
+                            }
+                            pend[b] = (uint32_t)t | (i == w.tb ? 2u : 0u) | (t == 0 ? 4u : 0u) | (last_t ? 8u : 0u);
+                            n++;
+                            if (n - pv > 2 && !(ok = issue_pv())) break;
+                        }
+                    }
+                }
+                while (ok && pv < n) ok = issue_pv();
+                sv_commit(&S->done);
+            }
+            __syncwarp();
+        } else if (!PAGED && warp == 10) {
+            // ---- values that are no numbers, in tiles with masked places ----
+            uint32_t seg = 0, kt = 0;
+            bool ok = true;
+            for (; ok && w.left > 0; sv_next_warp<PAGED>(A, w, tq, split), seg++) {
+                // this parity's notes were last read two segments ago
+                if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, S, A.err))) break;
+                for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[seg & 1][0][0])[u] = 0x7fffffff;
+                if (lane == 0) S->any_bad[seg & 1] = 0;
+                __syncwarp();
+                for (int i = w.tb; i < w.te; i++, kt++) {
+                    const uint32_t st = kt % SV_KST;
+                    // every tile passes here, so that no phase of v_full goes unseen
+                    if (!(ok = sv_wait(&S->v_full[st], (kt / SV_KST) & 1, S, A.err))) break;
+                    if (!sv_masked(w.q, w.t0, i)) {
+                        if (lane == 0) mbar_arrive(&S->v_ok[st]);
+                        continue;
+                    }
+                    unsigned char* V = Vs + st * SV_TILE_BYTES;
+                    uint32_t nan = 0;  // sticky: 0 * x is NaN for what is no number
+#pragma unroll 8
+                    for (int u = lane; u < SV_TILE_BYTES / 16; u += 32) {
+                        const uint4 v = *reinterpret_cast<const uint4*>(V + u * 16);
+                        nan = hfma2_u(v.x, 0, nan), nan = hfma2_u(v.y, 0, nan);
+                        nan = hfma2_u(v.z, 0, nan), nan = hfma2_u(v.w, 0, nan);
+                    }
+                    const __half2 nh = *reinterpret_cast<const __half2*>(&nan);
+                    if (__any_sync(0xffffffffu, __hisnan(nh.x) || __hisnan(nh.y))) {
+                        if (lane == 0) S->any_bad[seg & 1] = 1;
+                        for (int u = lane; u < SV_KT * CUINF_HD; u += 32) {
+                            const int r = u >> 6, d = u & 63;
+                            __half* p = reinterpret_cast<__half*>(V + r * 128 + (((d >> 3) ^ (r & 7)) << 4)) + (d & 7);
+                            const float f = __half2float(*p);
+                            if (isfinite(f)) continue;
+                            *p = __float2half_rn(0.f);
+                            atomicMin(&S->bad[seg & 1][isnan(f) ? 2 : f > 0.f ? 0 : 1][d], i * SV_KT + r);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+                    }
+                    __threadfence_block();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&S->v_ok[st]);
+                }
+                if (!ok) break;
+                if (lane == 0) mbar_arrive(&S->epi[seg & 1]);
+            }
+            __syncwarp();
+        } else if (PAGED && warp < 12) {
+            if constexpr (PAGED) sv_convert(A, w, tq, split, S, Ks, Vs, tid - 256);
+        }
+    }
+    pdl_trigger();
+    sv_fence_before();
+    __syncthreads();
+    if (warp == C::MMA_WARP) {
+        sv_fence_after();
+        if (lane == 0) sv_drain(&S->done, 0, A.err);
+        __syncwarp();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(SV_TMEM_COLS)
+                     : "memory");
+    }
+}
+
+// ---------------------------------------------------------------------------
+// joins the partial results of the items that were cut: CTA (i, j) takes a
+// quarter (64 rows) of the item that CTA i began and did not finish, whose
+// other parts are slot 0 of the CTAs behind it.  Fixed order: same bits.
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(256) k_serve_combine(const AttnArgs A, const SvWs W, const int n_ctas) {
+    pdl_wait();
+    const int i = blockIdx.x;
+    const SvPart p = W.part[i * 2 + 1];
+    if (!p.valid) return;
+    const int G = A.nh / A.nkv, TOK = 128 / G;
+    const int r = blockIdx.y * 64 + (threadIdx.x >> 2), c = (threadIdx.x & 3) * 16;  // a row, 16 of its columns
+    const int t = r >> 7, row = r & 127, tok = t * TOK + row / G;
+    if (row >= TOK * G || tok >= p.tokens) return;
+    float m = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+    for (int d = 0; d < 16; d++) o[d] = 0.f;
+    for (int k = i; k < n_ctas; k++) {
+        const size_t slot = (size_t)k * 2 + (k == i);
+        const SvPart pk = W.part[slot];
+        if (!pk.valid) continue;  // an empty share
+        const float2 ml = reinterpret_cast<const float2*>(W.ml)[slot * 256 + r];
+        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+        const float f0 = m == -INFINITY ? 0.f : sv_exp2(m - ref), f1 = ml.x == -INFINITY ? 0.f : sv_exp2(ml.x - ref);
+        // a part of NaN scores alone has no maximum: its sum carries them
+        l = l * f0 + (ml.x == -INFINITY ? ml.y : ml.y * f1);
+        m = mn;
+        const float4* src = reinterpret_cast<const float4*>(W.o + (slot * 256 + r) * 64 + c);
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+            const float4 x = src[d];
+            o[4 * d] = o[4 * d] * f0 + x.x * f1, o[4 * d + 1] = o[4 * d + 1] * f0 + x.y * f1;
+            o[4 * d + 2] = o[4 * d + 2] * f0 + x.z * f1, o[4 * d + 3] = o[4 * d + 3] * f0 + x.w * f1;
+        }
+        if (pk.last) break;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t h[8];
+#pragma unroll
+    for (int d = 0; d < 8; d++) h[d] = sv_pack_h2(o[2 * d] * inv, o[2 * d + 1] * inv);
+    uint4* dst = reinterpret_cast<uint4*>(A.out + ((size_t)(p.row0 + tok) * A.nh + p.h * G + row % G) * CUINF_HD + c);
+    dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+}
