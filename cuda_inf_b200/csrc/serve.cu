@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "serve.cuh"
+#include "serve_few.cuh"
 #include "serve_tc.cuh"
 
 #define ST(s) ((cudaStream_t)(s))
@@ -249,8 +250,20 @@ static int num_ctas(int* n) {
     return CUINF_OK;
 }
 
+static cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaStream_t st, cudaLaunchAttribute* attr) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr->val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
 template <bool PAGED>
-static int launch_tc(const AttnArgs& A, bool cuts, void* ws, cudaStream_t st) {
+static int launch_many(const AttnArgs& A, bool cuts, const SvWs& W, int ctas, cudaStream_t st) {
     CUtensorMap qm, km, vm;
     const int G = A.nh / A.nkv;
     if (int rc = rows_map(&qm, A.q, A.q_stride, A.nh, A.rows.n_rows, G, 128 / G)) return rc;
@@ -259,29 +272,30 @@ static int launch_tc(const AttnArgs& A, bool cuts, void* ws, cudaStream_t st) {
         if (int rc = rows_map(&km, A.k, A.k_stride, A.nkv, A.rows.n_rows, 1, SV_KT)) return rc;
         if (int rc = rows_map(&vm, A.v, A.v_stride, A.nkv, A.rows.n_rows, 1, SV_KT)) return rc;
     }
-    int ctas;
-    if (int rc = num_ctas(&ctas)) return rc;
-    const SvWs W = sv_ws(ws, ctas);
     CUINF_TRY(cudaFuncSetAttribute(k_serve_attn<PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)SV_SMEM_BYTES));
     k_serve_attn<PAGED><<<ctas, SvCfg<PAGED>::WARPS * 32, SV_SMEM_BYTES, st>>>(qm, km, vm, A, cuts, W);
-    if (int rc = cuinf_launch_status()) return rc;
-    if (!cuts) return CUINF_OK;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas, 4);
-    cfg.blockDim = dim3(256);
-    cfg.stream = st;
+    return cuinf_launch_status();
+}
+// `beside`: a chunks' kernel of the same call runs before (its results do not matter to this one)
+static int launch_few(const AttnArgs& A, bool cuts, const SvWs& W, int ctas, bool beside, cudaStream_t st) {
+    CUINF_TRY(cudaFuncSetAttribute(k_serve_few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FW_SMEM_BYTES));
     cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_combine, A, W, ctas));
+    cudaLaunchConfig_t cfg = pdl_config(dim3(ctas), (FW_WARPS + 1) * 32, FW_SMEM_BYTES, st, attr);
+    cfg.numAttrs = beside ? 1 : 0;
+    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_few, A, (int)cuts, W));
+    return cuinf_launch_status();
+}
+static int launch_combine(const AttnArgs& A, const SvWs& Wm, const SvWs& Wf, int ctas, bool many, bool few,
+                          cudaStream_t st) {
+    cudaLaunchAttribute attr[1];
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, (many ? 4 : 0) + (few ? 1 : 0)), 256, 0, st, attr);
+    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_combine, A, Wm, Wf, ctas, many ? 4 : 0));
     return cuinf_launch_status();
 }
 
 extern "C" size_t cuinf_attn_varlen_workspace_size(int n_seqs, int n_rows, int nh, int nkv) {
-    return sv_cuts(n_rows) ? sv_ws_bytes(SERVE_MAX_CTAS) : 0;
+    return sv_cuts(n_rows) ? sv_ws_bytes(SERVE_MAX_CTAS, 256) : 0;
 }
 extern "C" int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                                  int64_t v_stride, const int* cu_seqlens, int n_seqs, int n_rows, float scale,
@@ -304,12 +318,22 @@ extern "C" int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k,
     if (int rc = check_ws(workspace, workspace_bytes, cuinf_attn_varlen_workspace_size(n_seqs, n_rows, nh, nkv)))
         return rc;
     if (int rc = serve_err_ptr(&A.err)) return rc;
-    return launch_tc<false>(A, cuts, workspace, ST(stream));
+    int ctas;
+    if (int rc = num_ctas(&ctas)) return rc;
+    const SvWs W = sv_ws(workspace, ctas, 256);
+    if (int rc = launch_many<false>(A, cuts, W, ctas, ST(stream))) return rc;
+    return cuts ? launch_combine(A, W, W, ctas, true, false, ST(stream)) : CUINF_OK;
 }
+
+// Which of the two kernels a paged call can need.
+static bool has_many(int max_q, int nh, int nkv) { return (long long)max_q * (nh / nkv) > SERVE_FEW_ROWS; }
+static bool has_few(int nh, int nkv) { return nh / nkv <= SERVE_FEW_ROWS; }
 
 extern "C" size_t cuinf_attn_paged_workspace_size(int n_seqs, int n_rows, int max_q, int nh, int nkv,
                                                   int table_width) {
-    return sv_cuts(((long long)table_width + 1) * SERVE_PAGE) ? sv_ws_bytes(SERVE_MAX_CTAS) : 0;
+    if (nkv <= 0 || !sv_cuts(((long long)table_width + 1) * SERVE_PAGE)) return 0;
+    const bool many = has_many(max_q, nh, nkv), few = has_few(nh, nkv);
+    return (many ? sv_ws_bytes(SERVE_MAX_CTAS, 256) : 0) + (few ? sv_ws_bytes(SERVE_MAX_CTAS, 16) : 0);
 }
 extern "C" int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_seqlens, const int* kv_lens,
                                 int n_seqs, int n_rows, int max_q, const int* table, int table_width,
@@ -336,5 +360,14 @@ extern "C" int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_s
                           cuinf_attn_paged_workspace_size(n_seqs, n_rows, max_q, nh, nkv, table_width)))
         return rc;
     if (int rc = serve_err_ptr(&A.err)) return rc;
-    return launch_tc<true>(A, cuts, workspace, ST(stream));
+    int ctas;
+    if (int rc = num_ctas(&ctas)) return rc;
+    const bool many = has_many(max_q, nh, nkv), few = has_few(nh, nkv);
+    const SvWs Wm = sv_ws(workspace, ctas, 256);
+    const SvWs Wf = sv_ws((char*)workspace + (many && cuts ? sv_ws_bytes(ctas, 256) : 0), ctas, 16);
+    if (many)
+        if (int rc = launch_many<true>(A, cuts, Wm, ctas, ST(stream))) return rc;
+    if (few)
+        if (int rc = launch_few(A, cuts, Wf, ctas, many, ST(stream))) return rc;
+    return cuts ? launch_combine(A, Wm, Wf, ctas, many, few, ST(stream)) : CUINF_OK;
 }

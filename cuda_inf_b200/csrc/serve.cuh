@@ -25,7 +25,7 @@ struct PagedKV {
 
 // Paged: sequences of at most this many rows (new tokens x query heads per kv
 // head) go to the single-token kernel, longer ones to the tensor-core kernel.
-#define SERVE_FEW_ROWS 0
+#define SERVE_FEW_ROWS 16
 
 // New rows of packed sequences: sequence s holds rows cu[s]..cu[s+1]-1 of
 // n_rows.  Offsets outside [0, n_rows] or out of order are clamped (and

@@ -1,0 +1,206 @@
+// The line of work units that the serving attention kernels share out: one CTA
+// per SM, each takes an equal contiguous share of all sequences' units laid
+// end to end (key tiles of the tensor-core kernel, pages of the single-token
+// kernel), so the load is even whatever the lengths are.  An item that a
+// share's end cuts is joined from partial results by k_serve_combine.
+#pragma once
+#include "serve.cuh"
+
+// ---- waits (bounded; the first that gives up raises the CTA's abort word) ----
+#define SV_WAIT_LIMIT_NS 500000000ull
+__device__ __forceinline__ bool sv_wait(uint64_t* bar, uint32_t parity, int* abort_, unsigned* err) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = globaltimer_ns();
+    for (int k = 1;; k++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((k & 15) == 0) {
+            if (*(volatile int*)abort_) return false;
+            if (globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS) break;
+        }
+    }
+    *(volatile int*)abort_ = 1;
+    atomicOr(err, SERVE_ERR_WAIT);
+    return false;
+}
+// Before the CTA ends: a phase that copies or products in flight complete.
+__device__ __forceinline__ void sv_drain(uint64_t* bar, uint32_t parity, unsigned* err) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(bar, parity))
+        if (globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS) {
+            atomicOr(err, SERVE_ERR_WAIT);
+            return;
+        }
+}
+
+// ---- arithmetic ----
+__device__ __forceinline__ float sv_exp2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t sv_pack_h2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t sv_e4m3x2(uint32_t two) {  // low 16 bits: two codes -> two halves, exact
+    uint32_t r;
+    asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(r) : "r"(two));
+    return r;
+}
+// FP8: the weights carry the page's value scale times this.  A scale is at most
+// 65504 / 448, so with weights up to 2^3 fp16 still holds them; a usual scale
+// (0.01) keeps weights above 4e-4 in fp16's normal range.
+#define SV_VEXP 16.f
+
+// ---- sequences ----
+enum { SV_PACKED = 0, SV_MANY = 1, SV_FEW = 2 };  // packed prompts; paged, many or few rows of a sequence
+// One sequence as a kernel sees it: c new rows from row a on, the first at
+// position p0 of kv keys.
+struct SvSeq {
+    int a, c, p0, kv;
+};
+// False: nothing for this kernel (empty, out of range, or the other kernel's).
+template <int KIND>
+__device__ __forceinline__ bool sv_seq(const AttnArgs& A, int s, SvSeq& q, bool report) {
+    int b;
+    bool fine = packed_range(A.rows, s, q.a, b);
+    q.c = b - q.a;
+    if (KIND != SV_PACKED) {
+        q.kv = __ldg(A.kv_lens + s);
+        if (q.c > 0 && (q.kv < 0 || q.kv / SERVE_PAGE > A.kv.width || q.c > A.max_q)) {
+            fine = false;
+            q.c = 0;
+        }
+        const bool few = (long long)q.c * (A.nh / A.nkv) <= SERVE_FEW_ROWS;
+        if (few != (KIND == SV_FEW)) q.c = 0;
+    } else {
+        q.kv = q.c;
+    }
+    q.p0 = q.kv - q.c;
+    if (report && !fine) atomicOr(A.err, SERVE_ERR_RANGE);
+    return q.c > 0;
+}
+
+// The CTA's share [W i / N, W (i+1) / N) of the line of W units.
+struct SvShare {
+    int s;           // sequence in which it begins
+    long long rem;   // units of that sequence before it
+    long long left;  // its units (0: nothing to do)
+    long long scan[32];
+};
+// All threads call; `units` gives a sequence's units.
+template <int KIND, class F>
+__device__ __forceinline__ void sv_share(const AttnArgs& A, SvShare* S, int cta, int n_ctas, F units) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
+    long long total = 0, beg = 0, end = 0, base = 0;
+    if (tid == 0) S->left = 0;
+    for (int pass = 0; pass < 2; pass++) {
+        for (int b = 0; b < A.rows.n_seqs; b += nt) {
+            const int s = b + tid;
+            SvSeq q;
+            long long w = 0;
+            if (s < A.rows.n_seqs && sv_seq<KIND>(A, s, q, pass == 0 && cta == 0)) w = units(q);
+            long long x = w;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const long long y = __shfl_up_sync(0xffffffffu, x, o);
+                if (lane >= o) x += y;
+            }
+            __syncthreads();
+            if (lane == 31) S->scan[warp] = x;
+            __syncthreads();
+            long long before = 0, all = 0;
+            for (int i = 0; i < nw; i++) {
+                const long long y = S->scan[i];
+                if (i < warp) before += y;
+                all += y;
+            }
+            if (pass == 0) {
+                total += all;
+            } else {
+                const long long lo = base + before + x - w;
+                if (end > beg && beg >= lo && beg < lo + w) {
+                    S->s = s;
+                    S->rem = beg - lo;
+                    S->left = end - beg;
+                }
+                base += all;
+            }
+        }
+        if (pass == 0) {
+            beg = total * cta / n_ctas;
+            end = total * (cta + 1) / n_ctas;
+        }
+    }
+    __syncthreads();
+}
+
+// ---- partial results: [CTA][2] slots of `rows` rows; slot 0: the CTA's share
+// began inside the item, slot 1: it began the item and did not finish it ----
+struct SvPart {
+    int valid, last, row0, tokens, h, pad[3];  // first token row, tokens of the item, kv head
+};
+struct SvWs {
+    SvPart* part;  // [ctas][2]
+    float* ml;     // [ctas][2][rows][2]: reference (power of two) and sum
+    float* o;      // [ctas][2][rows][64], not divided by the sum
+};
+static inline size_t sv_ws_bytes(int ctas, int rows) {
+    return (size_t)ctas * 2 * (sizeof(SvPart) + (size_t)rows * (2 + CUINF_HD) * 4);
+}
+static inline SvWs sv_ws(void* p, int ctas, int rows) {
+    SvWs w;
+    w.o = (float*)p;
+    w.ml = w.o + (size_t)ctas * 2 * rows * CUINF_HD;
+    w.part = (SvPart*)(w.ml + (size_t)ctas * 2 * rows * 2);
+    return w;
+}
+
+// Joins the items that were cut: CTA (i, j) takes 64 rows of the item that CTA
+// i of the attention began and did not finish; the other parts are slot 0 of
+// the CTAs behind it.  j < many_y: the tensor-core kernel's items (256 rows),
+// else the single-token kernel's (16).  Fixed order: the same bits every time.
+__global__ void __launch_bounds__(256) k_serve_combine(const AttnArgs A, const SvWs Wm, const SvWs Wf, const int n_ctas,
+                                                       const int many_y) {
+    pdl_wait();
+    const bool few = (int)blockIdx.y >= many_y;
+    const SvWs& W = few ? Wf : Wm;
+    const int rows = few ? 16 : 256, y = few ? 0 : blockIdx.y;
+    const int i = blockIdx.x;
+    const SvPart p = W.part[i * 2 + 1];
+    if (!p.valid) return;
+    const int G = A.nh / A.nkv, TOK = 128 / G;
+    const int r = y * 64 + (threadIdx.x >> 2), c = (threadIdx.x & 3) * 16;  // a row, 16 of its columns
+    const int row = r & 127, tok = (r >> 7) * TOK + row / G;
+    if (r >= rows || row >= TOK * G || tok >= p.tokens) return;
+    float m = -INFINITY, l = 0.f, o[16];
+#pragma unroll
+    for (int d = 0; d < 16; d++) o[d] = 0.f;
+    for (int k = i; k < n_ctas; k++) {
+        const size_t slot = (size_t)k * 2 + (k == i);
+        const SvPart pk = W.part[slot];
+        if (!pk.valid) continue;  // an empty share
+        const float2 ml = reinterpret_cast<const float2*>(W.ml)[slot * rows + r];
+        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
+        const float f0 = m == -INFINITY ? 0.f : sv_exp2(m - ref), f1 = ml.x == -INFINITY ? 0.f : sv_exp2(ml.x - ref);
+        // a part of NaN scores alone has no maximum: its sum carries them
+        l = l * f0 + (ml.x == -INFINITY ? ml.y : ml.y * f1);
+        m = mn;
+        const float4* src = reinterpret_cast<const float4*>(W.o + (slot * rows + r) * CUINF_HD + c);
+#pragma unroll
+        for (int d = 0; d < 4; d++) {
+            const float4 x = src[d];
+            o[4 * d] = o[4 * d] * f0 + x.x * f1, o[4 * d + 1] = o[4 * d + 1] * f0 + x.y * f1;
+            o[4 * d + 2] = o[4 * d + 2] * f0 + x.z * f1, o[4 * d + 3] = o[4 * d + 3] * f0 + x.w * f1;
+        }
+        if (pk.last) break;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t h[8];
+#pragma unroll
+    for (int d = 0; d < 8; d++) h[d] = sv_pack_h2(o[2 * d] * inv, o[2 * d + 1] * inv);
+    uint4* dst = reinterpret_cast<uint4*>(A.out + ((size_t)(p.row0 + tok) * A.nh + p.h * G + row % G) * CUINF_HD + c);
+    dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
+    dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
+}

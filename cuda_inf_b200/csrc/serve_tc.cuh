@@ -31,7 +31,7 @@
 // key); the epilogue adds them to the rows that do attend them.
 #pragma once
 #include <cuda.h>
-#include "serve.cuh"
+#include "serve_line.cuh"
 
 #define SV_KT 128        // keys per tile
 #define SV_KST 4         // K and V stages
@@ -39,13 +39,7 @@
 #define SV_TILE_BYTES (SV_KT * CUINF_HD * 2)
 #define SV_TMEM_COLS 512
 #define SV_O_COL 384     // S/P buffers at 0, 128, 256; O of row tile t at 384 + 64 t
-#define SV_VEXP 16.f     // FP8: weights carry scale * 16 (fp16 keeps 146 * 16 * 2^THR)
 
-// One sequence as this kernel sees it: c new rows from row a on, the first at
-// position p0 of kv keys.
-struct SvSeq {
-    int a, c, p0, kv;
-};
 // A role's place on the line of key tiles.  One per warp, in shared memory: the
 // softmax warps have no registers to spare for it.
 struct SvItem {
@@ -63,59 +57,37 @@ struct SvSmem {
     float sc[SV_SC][4];  // FP8: K scale of the tile's two pages (negative: absent), V scales
     int bad[2][3][CUINF_HD];  // by segment parity: first key whose value is +inf, -inf, NaN
     int any_bad[2];
-    // start of this CTA's share
-    int s, h, qb, tile;
-    long long left;
-    long long scan[32];
+    SvShare share;
+    int h, qb, tile;  // the item in which the share begins, and its tile there
     SvItem item[16];
 };
 static constexpr size_t SV_Q_BYTES = 2 * SV_TILE_BYTES;  // both row tiles of an item
 static constexpr size_t SV_SMEM_BYTES = 1024 + 2 * SV_Q_BYTES + 2 * SV_KST * (size_t)SV_TILE_BYTES + sizeof(SvSmem);
 
-// Partial results: [CTA][2] slots of 256 rows; slot 0: the CTA's share began
-// inside the item, slot 1: it began the item and did not finish it.
-struct SvPart {
-    int valid, last, row0, tokens, h, pad[3];  // first token row, tokens of the item, kv head
-};
-struct SvWs {
-    SvPart* part;  // [ctas][2]
-    float* ml;     // [ctas][2][256][2]
-    float* o;      // [ctas][2][256][64]
-};
-static inline size_t sv_ws_bytes(int ctas) { return (size_t)ctas * 2 * (sizeof(SvPart) + 256 * 2 * 4 + 256 * 64 * 4); }
-__host__ __device__ inline SvWs sv_ws(void* p, int ctas) {
-    SvWs w;
-    w.o = (float*)p;
-    w.ml = w.o + (size_t)ctas * 2 * 256 * 64;
-    w.part = (SvPart*)(w.ml + (size_t)ctas * 2 * 256 * 2);
-    return w;
+// ---- packed fp32 pairs ----
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
+    return r;
 }
-
-// ---- waits (bounded; the first that gives up raises the abort word) ----
-#define SV_WAIT_LIMIT_NS 500000000ull
-__device__ __forceinline__ bool sv_wait(uint64_t* bar, uint32_t parity, SvSmem* S, unsigned* err) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    for (int k = 1;; k++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((k & 15) == 0) {
-            if (*(volatile int*)&S->abort_) return false;
-            if (globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS) break;
-        }
-    }
-    *(volatile int*)&S->abort_ = 1;
-    atomicOr(err, SERVE_ERR_WAIT);
-    return false;
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
+    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
 }
-__device__ __forceinline__ void sv_drain(uint64_t* bar, uint32_t parity, unsigned* err) {
-    const uint64_t t0 = globaltimer_ns();
-    while (!mbar_try_wait(bar, parity))
-        if (globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS) {
-            atomicOr(err, SERVE_ERR_WAIT);
-            return;
-        }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
-
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 // ---- tcgen05 ----
 __device__ __forceinline__ void sv_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void sv_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -182,65 +154,9 @@ __device__ __forceinline__ void sv_tma_3d(void* dst, const CUtensorMap* map, int
         : "memory");
 }
 
-// ---- packed fp32 pairs ----
-__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) {
-    asm("mov.b64 {%0, %1}, %2;\n" : "=f"(a), "=f"(b) : "l"(v));
-}
-__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t f2_mul(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ float sv_exp2(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t sv_pack_h2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
 // ---------------------------------------------------------------------------
 // the line of key tiles
 // ---------------------------------------------------------------------------
-// False: nothing for this kernel (empty, out of range, or few enough rows for
-// the single-token kernel).
-template <bool PAGED>
-__device__ __forceinline__ bool sv_seq(const AttnArgs& A, int s, SvSeq& q, bool report) {
-    int b;
-    bool fine = packed_range(A.rows, s, q.a, b);
-    q.c = b - q.a;
-    if (PAGED) {
-        q.kv = A.kv_lens[s];
-        if (q.c > 0 && (q.kv < 0 || q.kv / SERVE_PAGE > A.kv.width || q.c > A.max_q)) {
-            fine = false;
-            q.c = 0;
-        }
-        if (q.c * (A.nh / A.nkv) <= SERVE_FEW_ROWS) q.c = 0;
-    } else {
-        q.kv = q.c;
-    }
-    q.p0 = q.kv - q.c;
-    if (report && !fine) atomicOr(A.err, SERVE_ERR_RANGE);
-    return q.c > 0;
-}
 // key tiles of a block of rows that ends before row `end` (at least one: a
 // block whose rows have no key still writes its zeros)
 __device__ __forceinline__ int sv_tiles(const SvSeq& q, int end) {
@@ -271,58 +187,17 @@ __device__ __forceinline__ long long sv_head_tiles(const SvSeq& q, int tq) {
     return z + floor_sum(m - z, SV_KT, tq, (long long)q.p0 + (long long)tq * (z + 1) + SV_KT - 1) + sv_tiles(q, q.c);
 }
 
-// Finds the CTA's share [W i / N, W (i+1) / N) of the line of W tiles and its
-// first item.  All threads call; the result is in S (left = 0: nothing to do).
-template <bool PAGED>
+// The CTA's share of the line of key tiles and its first item (all threads call).
+template <int KIND>
 __device__ void sv_start(const AttnArgs& A, SvSmem* S, int tq, int n_ctas) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
-    long long total = 0, beg = 0, end = 0, base = 0;
-    if (tid == 0) S->left = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        for (int b = 0; b < A.rows.n_seqs; b += nt) {
-            const int s = b + tid;
-            SvSeq q;
-            long long w = 0;
-            if (s < A.rows.n_seqs && sv_seq<PAGED>(A, s, q, pass == 0 && blockIdx.x == 0))
-                w = sv_head_tiles(q, tq) * A.nkv;
-            long long x = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            __syncthreads();
-            if (lane == 31) S->scan[warp] = x;
-            __syncthreads();
-            long long before = 0, all = 0;
-            for (int i = 0; i < nw; i++) {
-                const long long y = S->scan[i];
-                if (i < warp) before += y;
-                all += y;
-            }
-            if (pass == 0) {
-                total += all;
-            } else {
-                const long long lo = base + before + x - w;
-                if (end > beg && beg >= lo && beg < lo + w) {
-                    S->s = s;
-                    S->left = end - beg;
-                    S->scan[31] = beg - lo;
-                }
-                base += all;
-            }
-        }
-        if (pass == 0) {
-            beg = total * blockIdx.x / n_ctas;
-            end = total * (blockIdx.x + 1) / n_ctas;
-        }
-    }
-    __syncthreads();
-    if (warp == 0 && S->left > 0) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    sv_share<KIND>(A, &S->share, blockIdx.x, n_ctas,
+                   [&](const SvSeq& q) { return sv_head_tiles(q, tq) * A.nkv; });
+    if (warp == 0 && S->share.left > 0) {
         SvSeq q;
-        sv_seq<PAGED>(A, S->s, q, false);
+        sv_seq<KIND>(A, S->share.s, q, false);
         const long long per = sv_head_tiles(q, tq);
-        long long rem = S->scan[31];
+        long long rem = S->share.rem;
         const int h = (int)(rem / per);
         rem -= h * per;
         const int nqb = (q.c + tq - 1) / tq;
@@ -356,7 +231,7 @@ __device__ __forceinline__ void sv_item(SvItem& w, int tq, int split) {
     w.n = sv_tiles(w.q, min(w.t0 + tq, w.q.c));
     w.te = split ? (int)min((long long)w.n, w.tb + w.left) : w.n;
 }
-template <bool PAGED>
+template <int KIND>
 __device__ __forceinline__ void sv_advance(const AttnArgs& A, SvItem& w, int tq, int split) {
     if (++w.qb >= w.nqb) {
         w.qb = 0;
@@ -365,7 +240,7 @@ __device__ __forceinline__ void sv_advance(const AttnArgs& A, SvItem& w, int tq,
             SvSeq q;
             int s = w.s;
             do s++;
-            while (s < A.rows.n_seqs && !sv_seq<PAGED>(A, s, q, false));
+            while (s < A.rows.n_seqs && !sv_seq<KIND>(A, s, q, false));
             if (s >= A.rows.n_seqs) {
                 w.left = 0;
                 return;
@@ -377,30 +252,30 @@ __device__ __forceinline__ void sv_advance(const AttnArgs& A, SvItem& w, int tq,
     w.tb = 0;
     sv_item(w, tq, split);
 }
-template <bool PAGED>
+template <int KIND>
 __device__ __forceinline__ void sv_first(const AttnArgs& A, const SvSmem* S, SvItem& w, int tq, int split) {
-    w.s = S->s, w.h = S->h, w.qb = S->qb, w.left = S->left, w.tb = S->tile;
+    w.s = S->share.s, w.h = S->h, w.qb = S->qb, w.left = S->share.left, w.tb = S->tile;
     if (w.left <= 0) return;
     SvSeq q;
-    sv_seq<PAGED>(A, w.s, q, false);
+    sv_seq<KIND>(A, w.s, q, false);
     w.q = q;
     w.nqb = (q.c + tq - 1) / tq;
     sv_item(w, tq, split);
     if (!split && w.tb > 0) {  // the item belongs to the share in which it begins
         w.left -= w.n - w.tb;
-        if (w.left > 0) sv_advance<PAGED>(A, w, tq, split);
+        if (w.left > 0) sv_advance<KIND>(A, w, tq, split);
     }
 }
-template <bool PAGED>
+template <int KIND>
 __device__ __forceinline__ void sv_next(const AttnArgs& A, SvItem& w, int tq, int split) {
     w.left -= w.te - w.tb;
-    if (w.left > 0) sv_advance<PAGED>(A, w, tq, split);
+    if (w.left > 0) sv_advance<KIND>(A, w, tq, split);
 }
 // the same for all lanes of a warp
-template <bool PAGED>
+template <int KIND>
 __device__ __forceinline__ void sv_next_warp(const AttnArgs& A, SvItem& w, int tq, int split) {
     __syncwarp();
-    if ((threadIdx.x & 31) == 0) sv_next<PAGED>(A, w, tq, split);
+    if ((threadIdx.x & 31) == 0) sv_next<KIND>(A, w, tq, split);
     __syncwarp();
 }
 
@@ -411,6 +286,7 @@ template <bool PAGED>
 struct SvCfg {
     // softmax warps 0-7; packed: 8 TMA, 9 MMA, 10 value check (11 idle);
     // paged: 8-11 converters, 12 Q by TMA, 13 MMA (14, 15 idle)
+    static constexpr int KIND = PAGED ? SV_MANY : SV_PACKED;
     static constexpr int WARPS = PAGED ? 16 : 12;
     static constexpr int MMA_WARP = PAGED ? 13 : 9;
     static constexpr int Q_WARP = PAGED ? 12 : 8;
@@ -426,11 +302,6 @@ __device__ __forceinline__ bool sv_masked(const SvSeq& q, int t0, int tile) {
 }
 
 // ---- paged: pages widened to fp16 tiles by four warps ----
-__device__ __forceinline__ uint32_t sv_e4m3x2(uint32_t two) {  // low 16 bits: two codes -> two halves, exact
-    uint32_t r;
-    asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(r) : "r"(two));
-    return r;
-}
 template <int N>
 __device__ __forceinline__ bool sv_not_finite(const uint32_t (&h)[N]) {  // 0 * x is NaN for what is no number
     uint32_t x = 0;
@@ -520,10 +391,10 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
         }
         return page;
     };
-    for (; ok && w.left > 0; sv_next_warp<true>(A, w, tq, split), seg++) {
+    for (; ok && w.left > 0; sv_next_warp<SV_MANY>(A, w, tq, split), seg++) {
         const int par = seg & 1;
         // this parity's notes were last read two segments ago
-        if (seg >= 2 && !(ok = sv_wait(&S->epi[par], ((seg >> 1) - 1) & 1, S, A.err))) break;
+        if (seg >= 2 && !(ok = sv_wait(&S->epi[par], ((seg >> 1) - 1) & 1, &S->abort_, A.err))) break;
         if (warp == 0) {
             for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[par][0][0])[u] = 0x7fffffff;
             if (lane == 0) S->any_bad[par] = 0;
@@ -531,7 +402,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
         __threadfence_block();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S->conv);
-        if (!(ok = sv_wait(&S->conv, seg & 1, S, A.err))) break;
+        if (!(ok = sv_wait(&S->conv, seg & 1, &S->abort_, A.err))) break;
 
         const size_t tail = ((size_t)w.s * A.nkv + w.h) * SERVE_PAGE_HEAD;
         const int rest = w.q.kv % SERVE_PAGE;
@@ -560,7 +431,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
             if (tid < 4) sn = scale(pq);
 #pragma unroll
             for (int g = 0; g < 2; g++) pn[g] = i + 2 < w.te ? sv_page(A, w.q, w.s, 2 * (i + 2) + g) : -1;
-            if (!(ok = sv_wait(&S->k_empty[st], ph, S, A.err))) break;
+            if (!(ok = sv_wait(&S->k_empty[st], ph, &S->abort_, A.err))) break;
             unsigned char* kd = Ks + st * SV_TILE_BYTES;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
@@ -576,7 +447,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
             if (lane == 0) mbar_arrive(&S->k_full[st]);
 #pragma unroll
             for (int g = 0; g < 2; g++) cv.load(A.kv.kp8, pq[g], w.h, kx[g]);
-            if (!(ok = sv_wait(&S->v_empty[st], ph, S, A.err))) break;
+            if (!(ok = sv_wait(&S->v_empty[st], ph, &S->abort_, A.err))) break;
             unsigned char* vd = Vs + st * SV_TILE_BYTES;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
@@ -616,6 +487,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
     SvSmem* S = reinterpret_cast<SvSmem*>(Vs + SV_KST * SV_TILE_BYTES);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = A.nh / A.nkv, TOK = 128 / G, tq = 2 * TOK;
+    pdl_trigger();
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -641,13 +513,13 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     if (split && tid < 2) W.part[blockIdx.x * 2 + tid].valid = 0;
-    sv_start<PAGED>(A, S, tq, gridDim.x);
+    sv_start<C::KIND>(A, S, tq, gridDim.x);
     sv_fence_before();
     __syncthreads();
     sv_fence_after();
     const uint32_t tmem = S->tmem;
     SvItem& w = S->item[warp];
-    if (lane == 0) sv_first<PAGED>(A, S, w, tq, split);
+    if (lane == 0) sv_first<C::KIND>(A, S, w, tq, split);
     __syncwarp();
 
     if (warp < 8) {
@@ -660,11 +532,11 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         uint32_t n = 0, ops = 0, tiles = 0, seg = 0;
         uint32_t sbits = 0;  // phases of s_full[t] by buffer
         bool ok = true;
-        for (; ok && w.left > 0; sv_next_warp<PAGED>(A, w, tq, split), seg++) {
+        for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
             const int nt = w.te - w.tb;
             const bool act1 = w.t0 + TOK < w.q.c;
             // all who arrive at a segment's epi barrier have seen the one before of the same parity complete
-            if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, S, A.err))) break;
+            if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_, A.err))) break;
             if (t == 1 && !act1) {
                 n += nt, tiles += nt;
                 __syncwarp();
@@ -678,7 +550,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             uint64_t l2 = 0;  // two partial sums
             for (int i = w.tb; i < w.te; i++, ops++, tiles++) {
                 const uint32_t nn = n + (act1 ? 2 * (i - w.tb) + t : i - w.tb), b = nn % 3;
-                if (!(ok = sv_wait(&S->s_full[t][b], (sbits >> b) & 1, S, A.err))) break;
+                if (!(ok = sv_wait(&S->s_full[t][b], (sbits >> b) & 1, &S->abort_, A.err))) break;
                 sbits ^= 1u << b;
                 sv_fence_after();
                 uint32_t sr[128];
@@ -737,7 +609,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     const float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
                     m = mn;
                     l2 = f2_mul(l2, f2_pack(f, f));
-                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, S, A.err))) break;
+                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
                     sv_fence_after();
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
@@ -773,14 +645,14 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 sv_fence_before();
                 // every phase of o_full is seen (a parity tells only neighbouring phases apart); the last
                 // product is long done here
-                if (i > w.tb && !(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, S, A.err))) break;
+                if (i > w.tb && !(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S->p_full[b]);
             }
             if (!ok) break;
             n += act1 ? 2 * nt : nt;
             // ---- epilogue of the item (or of the CTA's part of it) ----
-            if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, S, A.err))) break;
+            if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
             sv_fence_after();
             uint32_t o[64];
             sv_ld32(o_addr, o);
@@ -845,11 +717,11 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             // ---- Q (and, packed, K and V) by TMA ----
             uint32_t seg = 0, kt = 0, nq = 0, nk = 0, nv = 0;  // copies issued
             bool ok = true;
-            for (; ok && w.left > 0; sv_next_warp<PAGED>(A, w, tq, split), seg++) {
+            for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
                 const uint32_t qsl = seg & 1;
                 bool r = true;
                 if (lane == 0) {
-                    r = sv_wait(&S->q_empty[qsl], ((seg >> 1) & 1) ^ 1, S, A.err);
+                    r = sv_wait(&S->q_empty[qsl], ((seg >> 1) & 1) ^ 1, &S->abort_, A.err);
                     if (r) {
                         const bool act1 = w.t0 + TOK < w.q.c;
                         mbar_arrive_expect_tx(&S->q_full[qsl], (uint32_t)(TOK * G * 128) * (act1 ? 2 : 1));
@@ -864,12 +736,12 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 for (int i = w.tb; i < w.te; i++, kt++) {
                     const uint32_t st = kt % SV_KST, ph = ((kt / SV_KST) & 1) ^ 1;
                     if (lane == 0) {
-                        r = sv_wait(&S->k_empty[st], ph, S, A.err);
+                        r = sv_wait(&S->k_empty[st], ph, &S->abort_, A.err);
                         if (r) {
                             mbar_arrive_expect_tx(&S->k_full[st], SV_TILE_BYTES);
                             sv_tma_3d(Ks + st * SV_TILE_BYTES, &kmap, 0, w.h, w.q.a + i * SV_KT, &S->k_full[st]);
                             nk++;
-                            r = sv_wait(&S->v_empty[st], ph, S, A.err);
+                            r = sv_wait(&S->v_empty[st], ph, &S->abort_, A.err);
                         }
                         if (r) {
                             mbar_arrive_expect_tx(&S->v_full[st], SV_TILE_BYTES);
@@ -900,13 +772,13 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 bool ok = true;
                 auto issue_pv = [&]() -> bool {
                     const uint32_t op = pend[pv % 3], b = pv % 3, t = op & 1, st = vt % SV_KST;
-                    if ((op & 2) && segs[t] > 0 && !sv_wait(&S->o_free[t], (segs[t] - 1) & 1, S, A.err)) return false;
+                    if ((op & 2) && segs[t] > 0 && !sv_wait(&S->o_free[t], (segs[t] - 1) & 1, &S->abort_, A.err)) return false;
                     if (op & 2) segs[t]++;
                     if (op & 4) {
-                        if (!sv_wait(&S->v_full[st], (vt / SV_KST) & 1, S, A.err)) return false;
-                        if (!PAGED && !sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, S, A.err)) return false;
+                        if (!sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
+                        if (!PAGED && !sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
                     }
-                    if (!sv_wait(&S->p_full[b], (pv / 3) & 1, S, A.err)) return false;
+                    if (!sv_wait(&S->p_full[b], (pv / 3) & 1, &S->abort_, A.err)) return false;
                     sv_fence_after();
                     const uint32_t va = smem_u32(Vs + st * SV_TILE_BYTES);
 #pragma unroll
@@ -927,9 +799,9 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     if (mbar_test_wait(bar, parity)) return true;
                     while (pv < n)
                         if (!issue_pv()) return false;
-                    return sv_wait(bar, parity, S, A.err);
+                    return sv_wait(bar, parity, &S->abort_, A.err);
                 };
-                for (; ok && w.left > 0; sv_next<PAGED>(A, w, tq, split), seg++) {
+                for (; ok && w.left > 0; sv_next<C::KIND>(A, w, tq, split), seg++) {
                     const bool act1 = w.t0 + TOK < w.q.c;
                     if (!(ok = wait_input(&S->q_full[seg & 1], (seg >> 1) & 1))) break;
                     for (int i = w.tb; ok && i < w.te; i++, kt++) {
@@ -964,16 +836,16 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             // ---- values that are no numbers, in tiles with masked places ----
             uint32_t seg = 0, kt = 0;
             bool ok = true;
-            for (; ok && w.left > 0; sv_next_warp<PAGED>(A, w, tq, split), seg++) {
+            for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
                 // this parity's notes were last read two segments ago
-                if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, S, A.err))) break;
+                if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_, A.err))) break;
                 for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[seg & 1][0][0])[u] = 0x7fffffff;
                 if (lane == 0) S->any_bad[seg & 1] = 0;
                 __syncwarp();
                 for (int i = w.tb; i < w.te; i++, kt++) {
                     const uint32_t st = kt % SV_KST;
                     // every tile passes here, so that no phase of v_full goes unseen
-                    if (!(ok = sv_wait(&S->v_full[st], (kt / SV_KST) & 1, S, A.err))) break;
+                    if (!(ok = sv_wait(&S->v_full[st], (kt / SV_KST) & 1, &S->abort_, A.err))) break;
                     if (!sv_masked(w.q, w.t0, i)) {
                         if (lane == 0) mbar_arrive(&S->v_ok[st]);
                         continue;
@@ -1011,7 +883,6 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             if constexpr (PAGED) sv_convert(A, w, tq, split, S, Ks, Vs, tid - 256);
         }
     }
-    pdl_trigger();
     sv_fence_before();
     __syncthreads();
     if (warp == C::MMA_WARP) {
@@ -1021,49 +892,4 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(SV_TMEM_COLS)
                      : "memory");
     }
-}
-
-// ---------------------------------------------------------------------------
-// joins the partial results of the items that were cut: CTA (i, j) takes a
-// quarter (64 rows) of the item that CTA i began and did not finish, whose
-// other parts are slot 0 of the CTAs behind it.  Fixed order: same bits.
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) k_serve_combine(const AttnArgs A, const SvWs W, const int n_ctas) {
-    pdl_wait();
-    const int i = blockIdx.x;
-    const SvPart p = W.part[i * 2 + 1];
-    if (!p.valid) return;
-    const int G = A.nh / A.nkv, TOK = 128 / G;
-    const int r = blockIdx.y * 64 + (threadIdx.x >> 2), c = (threadIdx.x & 3) * 16;  // a row, 16 of its columns
-    const int t = r >> 7, row = r & 127, tok = t * TOK + row / G;
-    if (row >= TOK * G || tok >= p.tokens) return;
-    float m = -INFINITY, l = 0.f, o[16];
-#pragma unroll
-    for (int d = 0; d < 16; d++) o[d] = 0.f;
-    for (int k = i; k < n_ctas; k++) {
-        const size_t slot = (size_t)k * 2 + (k == i);
-        const SvPart pk = W.part[slot];
-        if (!pk.valid) continue;  // an empty share
-        const float2 ml = reinterpret_cast<const float2*>(W.ml)[slot * 256 + r];
-        const float mn = fmaxf(m, ml.x), ref = mn == -INFINITY ? 0.f : mn;
-        const float f0 = m == -INFINITY ? 0.f : sv_exp2(m - ref), f1 = ml.x == -INFINITY ? 0.f : sv_exp2(ml.x - ref);
-        // a part of NaN scores alone has no maximum: its sum carries them
-        l = l * f0 + (ml.x == -INFINITY ? ml.y : ml.y * f1);
-        m = mn;
-        const float4* src = reinterpret_cast<const float4*>(W.o + (slot * 256 + r) * 64 + c);
-#pragma unroll
-        for (int d = 0; d < 4; d++) {
-            const float4 x = src[d];
-            o[4 * d] = o[4 * d] * f0 + x.x * f1, o[4 * d + 1] = o[4 * d + 1] * f0 + x.y * f1;
-            o[4 * d + 2] = o[4 * d + 2] * f0 + x.z * f1, o[4 * d + 3] = o[4 * d + 3] * f0 + x.w * f1;
-        }
-        if (pk.last) break;
-    }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint32_t h[8];
-#pragma unroll
-    for (int d = 0; d < 8; d++) h[d] = sv_pack_h2(o[2 * d] * inv, o[2 * d + 1] * inv);
-    uint4* dst = reinterpret_cast<uint4*>(A.out + ((size_t)(p.row0 + tok) * A.nh + p.h * G + row % G) * CUINF_HD + c);
-    dst[0] = make_uint4(h[0], h[1], h[2], h[3]);
-    dst[1] = make_uint4(h[4], h[5], h[6], h[7]);
 }
