@@ -82,32 +82,34 @@ __device__ __forceinline__ bool sv_seq(const AttnArgs& A, int s, SvSeq& q, bool 
     return q.c > 0;
 }
 
-// The CTA's share [W i / N, W (i+1) / N) of the line of W units.
+// The CTA's share of the line (equal parts, to a unit).
 struct SvShare {
     int s;           // sequence in which it begins
     long long rem;   // units of that sequence before it
     long long left;  // its units (0: nothing to do)
     long long scan[32];
 };
-// All threads call; `units` gives a sequence's units.
+// All threads call; `units` gives a sequence's units.  One pass over the
+// sequences where the CTA has a thread for each, else one for the sum and one
+// for the place.
 template <int KIND, class F>
 __device__ __forceinline__ void sv_share(const AttnArgs& A, SvShare* S, int cta, int n_ctas, F units) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nt = blockDim.x, nw = nt >> 5;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nt = blockDim.x, nw = nt >> 5, n = A.rows.n_seqs;
     long long total = 0, beg = 0, end = 0, base = 0;
     if (tid == 0) S->left = 0;
-    for (int pass = 0; pass < 2; pass++) {
-        for (int b = 0; b < A.rows.n_seqs; b += nt) {
+    for (int pass = n <= nt ? 1 : 0; pass < 2; pass++) {
+        for (int b = 0; b < n; b += nt) {
             const int s = b + tid;
             SvSeq q;
             long long w = 0;
-            if (s < A.rows.n_seqs && sv_seq<KIND>(A, s, q, pass == 0 && cta == 0)) w = units(q);
+            if (s < n && sv_seq<KIND>(A, s, q, (pass == 0 || n <= nt) && cta == 0)) w = units(q);
             long long x = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long y = __shfl_up_sync(0xffffffffu, x, o);
                 if (lane >= o) x += y;
             }
-            __syncthreads();
+            if (b > 0 || pass == 1) __syncthreads();
             if (lane == 31) S->scan[warp] = x;
             __syncthreads();
             long long before = 0, all = 0;
@@ -118,19 +120,21 @@ __device__ __forceinline__ void sv_share(const AttnArgs& A, SvShare* S, int cta,
             }
             if (pass == 0) {
                 total += all;
-            } else {
-                const long long lo = base + before + x - w;
-                if (end > beg && beg >= lo && beg < lo + w) {
-                    S->s = s;
-                    S->rem = beg - lo;
-                    S->left = end - beg;
-                }
-                base += all;
+                continue;
             }
-        }
-        if (pass == 0) {
-            beg = total * cta / n_ctas;
-            end = total * (cta + 1) / n_ctas;
+            if (n <= nt) total = all;
+            if (b == 0) {
+                const long long per = total / n_ctas, more = total - per * n_ctas;
+                beg = per * cta + min((long long)cta, more);
+                end = beg + per + (cta < more);
+            }
+            const long long lo = base + before + x - w;
+            if (end > beg && beg >= lo && beg < lo + w) {
+                S->s = s;
+                S->rem = beg - lo;
+                S->left = end - beg;
+            }
+            base += all;
         }
     }
     __syncthreads();

@@ -46,7 +46,8 @@ struct SvItem {
     int s, h, qb, nqb;  // sequence, kv head, row block of nqb
     SvSeq q;
     int t0, tb, te, n;  // first token of the block; key tiles [tb, te) of n
-    long long left;     // tiles left of the CTA's share
+    int u;              // the item's units
+    long long left;     // units from its beginning to the end of the CTA's share
 };
 
 struct SvSmem {
@@ -58,7 +59,8 @@ struct SvSmem {
     int bad[2][3][CUINF_HD];  // by segment parity: first key whose value is +inf, -inf, NaN
     int any_bad[2];
     SvShare share;
-    int h, qb, tile;  // the item in which the share begins, and its tile there
+    int h, qb;  // the item in which the share begins, and its units before that
+    long long off;
     SvItem item[16];
 };
 static constexpr size_t SV_Q_BYTES = 2 * SV_TILE_BYTES;  // both row tiles of an item
@@ -97,23 +99,28 @@ __device__ __forceinline__ void sv_commit(uint64_t* bar) {
 }
 // Shared-memory descriptor, 128-byte swizzle, 8-row groups 1024 bytes apart:
 // a K-major operand (rows of 64 values), and equally V [key][64], an MN-major
-// operand whose one 64-wide atom spans the head.
-__device__ __forceinline__ uint64_t sv_desc(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
-}
-__device__ __forceinline__ void sv_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// operand whose one 64-wide atom spans the head.  Its low word moves with the
+// address (in units of 16 bytes), its high word is constant.
+__device__ __forceinline__ uint32_t sv_desc_lo(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+#define SV_DESC_HI ((1024u >> 4) | (1u << 14) | (2u << 29))
+__device__ __forceinline__ void sv_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(
-            d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(SV_DESC_HI)
         : "memory");
 }
-__device__ __forceinline__ void sv_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void sv_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(
-            d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(SV_DESC_HI)
         : "memory");
+}
+__device__ __forceinline__ bool sv_elect() {
+    uint32_t r;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+    return r != 0;
 }
 // fp16 operands, fp32 accumulate, M = 128; bit 16: B is MN-major
 #define SV_IDESC_QK ((1u << 4) | ((uint32_t)(SV_KT >> 3) << 17) | (8u << 24))
@@ -157,82 +164,67 @@ __device__ __forceinline__ void sv_tma_3d(void* dst, const CUtensorMap* map, int
 // ---------------------------------------------------------------------------
 // the line of key tiles
 // ---------------------------------------------------------------------------
-// key tiles of a block of rows that ends before row `end` (at least one: a
-// block whose rows have no key still writes its zeros)
-__device__ __forceinline__ int sv_tiles(const SvSeq& q, int end) {
-    return max(1, (q.p0 + end + SV_KT - 1) >> 7);
+// The line's unit is a key: an item (a block of tq rows of one kv head) takes
+// the keys of its last row and SV_OVH more for its beginning and end, so the
+// blocks of a sequence form an arithmetic series and a place on the line is
+// found without a table.  Cuts fall on key tiles (sv_cut).
+#define SV_OVH 256
+__device__ __forceinline__ int sv_keys(const SvSeq& q, int end) {  // rows before `end`; a row without a key still
+    return max(1, q.p0 + end);                                     // has its zeros written
 }
-// sum over i < n of floor((a i + b) / m), all non-negative
-__device__ __forceinline__ long long floor_sum(long long n, long long m, long long a, long long b) {
-    long long r = 0;
-    while (n > 0) {
-        r += (n - 1) * n / 2 * (a / m);
-        a %= m;
-        r += n * (b / m);
-        b %= m;
-        const long long y = a * n + b;
-        if (y < m) break;
-        n = y / m;
-        b = y % m;
-        const long long t = m;
-        m = a;
-        a = t;
-    }
-    return r;
+// units of the first k blocks of a head (none of them the last)
+__device__ __forceinline__ long long sv_prefix(const SvSeq& q, int tq, int k) {
+    const int z = q.p0 < 0 ? min(k, -q.p0 / tq) : 0;  // blocks without a key
+    return (long long)k * SV_OVH + z + (long long)(k - z) * q.p0 +
+           (long long)tq * (((long long)k * (k + 1) - (long long)z * (z + 1)) / 2);
 }
-// key tiles of all row blocks of one kv head of the sequence
-__device__ __forceinline__ long long sv_head_tiles(const SvSeq& q, int tq) {
-    const int m = (q.c + tq - 1) / tq - 1;  // blocks before the last
-    const int z = q.p0 < 0 ? min(m, -q.p0 / tq) : 0;  // of these, without a key
-    return z + floor_sum(m - z, SV_KT, tq, (long long)q.p0 + (long long)tq * (z + 1) + SV_KT - 1) + sv_tiles(q, q.c);
+__device__ __forceinline__ long long sv_head_units(const SvSeq& q, int tq) {
+    return sv_prefix(q, tq, (q.c + tq - 1) / tq - 1) + sv_keys(q, q.c) + SV_OVH;
+}
+// first key tile of a part that begins x units into an item of n tiles and u units
+__device__ __forceinline__ int sv_cut(long long x, int u, int n) {
+    return x >= u ? n : min(n, (int)max(0ll, x - SV_OVH + SV_KT / 2) / SV_KT);
 }
 
-// The CTA's share of the line of key tiles and its first item (all threads call).
+// The CTA's share and the item in which it begins (all threads call).
 template <int KIND>
 __device__ void sv_start(const AttnArgs& A, SvSmem* S, int tq, int n_ctas) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     sv_share<KIND>(A, &S->share, blockIdx.x, n_ctas,
-                   [&](const SvSeq& q) { return sv_head_tiles(q, tq) * A.nkv; });
-    if (warp == 0 && S->share.left > 0) {
+                   [&](const SvSeq& q) { return sv_head_units(q, tq) * A.nkv; });
+    if (threadIdx.x == 0 && S->share.left > 0) {
         SvSeq q;
         sv_seq<KIND>(A, S->share.s, q, false);
-        const long long per = sv_head_tiles(q, tq);
-        long long rem = S->share.rem;
-        const int h = (int)(rem / per);
-        rem -= h * per;
-        const int nqb = (q.c + tq - 1) / tq;
-        for (int b = 0; b < nqb; b += 32) {
-            const int qb = b + lane;
-            const int w = qb < nqb ? sv_tiles(q, min((qb + 1) * tq, q.c)) : 0;
-            int x = w;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if (lane >= o) x += y;
-            }
-            const unsigned hit = __ballot_sync(0xffffffffu, rem < x);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    S->h = h;
-                    S->qb = qb;
-                    S->tile = (int)(rem - (x - w));
-                }
-                break;
-            }
-            rem -= __shfl_sync(0xffffffffu, x, 31);
+        const long long per = sv_head_units(q, tq);
+        const int h = (int)(S->share.rem / per);
+        const long long rem = S->share.rem - h * per;
+        int lo = 0, hi = (q.c + tq - 1) / tq;  // the block: prefix(lo) <= rem < prefix(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (sv_prefix(q, tq, mid) <= rem)
+                lo = mid;
+            else
+                hi = mid;
         }
+        S->h = h;
+        S->qb = lo;
+        S->off = rem - sv_prefix(q, tq, lo);
     }
     __syncthreads();
 }
 
 // Walks the items of the CTA's share; every role runs its own (one lane calls).
-__device__ __forceinline__ void sv_item(SvItem& w, int tq, int split) {
-    w.t0 = w.qb * tq;
-    w.n = sv_tiles(w.q, min(w.t0 + tq, w.q.c));
-    w.te = split ? (int)min((long long)w.n, w.tb + w.left) : w.n;
+// left: units from the item's beginning to the share's end.
+__device__ __forceinline__ void sv_item(SvItem& w, int tq, int split, long long off) {
+    const int t0 = w.qb * tq, keys = sv_keys(w.q, min(t0 + tq, w.q.c)), n = (keys + SV_KT - 1) / SV_KT;
+    const int u = keys + SV_OVH;
+    w.t0 = t0, w.n = n, w.u = u;
+    w.tb = split ? sv_cut(off, u, n) : 0;
+    w.te = split ? sv_cut(w.left, u, n) : n;
 }
 template <int KIND>
-__device__ __forceinline__ void sv_advance(const AttnArgs& A, SvItem& w, int tq, int split) {
+__device__ __forceinline__ void sv_next(const AttnArgs& A, SvItem& w, int tq, int split) {
+    w.left -= w.u;
+    if (w.left <= 0) return;
     if (++w.qb >= w.nqb) {
         w.qb = 0;
         if (++w.h >= A.nkv) {
@@ -249,27 +241,22 @@ __device__ __forceinline__ void sv_advance(const AttnArgs& A, SvItem& w, int tq,
             w.nqb = (q.c + tq - 1) / tq;
         }
     }
-    w.tb = 0;
-    sv_item(w, tq, split);
+    sv_item(w, tq, split, 0);
+    if (w.te == 0) w.left = 0;  // the share ends before the item's first tile
 }
 template <int KIND>
 __device__ __forceinline__ void sv_first(const AttnArgs& A, const SvSmem* S, SvItem& w, int tq, int split) {
-    w.s = S->share.s, w.h = S->h, w.qb = S->qb, w.left = S->share.left, w.tb = S->tile;
+    w.s = S->share.s, w.h = S->h, w.qb = S->qb, w.left = S->share.left;
     if (w.left <= 0) return;
+    const long long off = S->off;
+    w.left += off;
     SvSeq q;
     sv_seq<KIND>(A, w.s, q, false);
     w.q = q;
     w.nqb = (q.c + tq - 1) / tq;
-    sv_item(w, tq, split);
-    if (!split && w.tb > 0) {  // the item belongs to the share in which it begins
-        w.left -= w.n - w.tb;
-        if (w.left > 0) sv_advance<KIND>(A, w, tq, split);
-    }
-}
-template <int KIND>
-__device__ __forceinline__ void sv_next(const AttnArgs& A, SvItem& w, int tq, int split) {
-    w.left -= w.te - w.tb;
-    if (w.left > 0) sv_advance<KIND>(A, w, tq, split);
+    sv_item(w, tq, split, off);
+    // nothing of this item: its last tile is before the share, or (uncut) it belongs to the share in which it begins
+    if (split ? w.tb == w.te : off > 0) sv_next<KIND>(A, w, tq, split);
 }
 // the same for all lanes of a warp
 template <int KIND>
@@ -762,75 +749,86 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             }
             __syncwarp();
         } else if (warp == C::MMA_WARP) {
-            // ---- products: S of op n, then O of op n - 2 ----
-            if (lane == 0) {
-                uint32_t n = 0, seg = 0, kt = 0, pv = 0, vt = 0;
-                uint32_t segs[2] = {0, 0};  // segments of row tile t so far
-                // ops whose PV is still to come: bit 0 t, 1 first of its segment, 2 first and 3 last op of
-                // the key tile
-                uint32_t pend[3] = {0, 0, 0};
-                bool ok = true;
-                auto issue_pv = [&]() -> bool {
-                    const uint32_t op = pend[pv % 3], b = pv % 3, t = op & 1, st = vt % SV_KST;
-                    if ((op & 2) && segs[t] > 0 && !sv_wait(&S->o_free[t], (segs[t] - 1) & 1, &S->abort_, A.err)) return false;
-                    if (op & 2) segs[t]++;
-                    if (op & 4) {
-                        if (!sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
-                        if (!PAGED && !sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
-                    }
-                    if (!sv_wait(&S->p_full[b], (pv / 3) & 1, &S->abort_, A.err)) return false;
-                    sv_fence_after();
-                    const uint32_t va = smem_u32(Vs + st * SV_TILE_BYTES);
+            // ---- products: S of op n, then O of op n - 2.  All lanes walk, one issues ----
+            const bool leader = sv_elect();
+            const uint32_t q_lo = sv_desc_lo(smem_u32(Qs)), k_lo = sv_desc_lo(smem_u32(Ks)), v_lo = sv_desc_lo(smem_u32(Vs));
+            uint32_t n = 0, pv = 0, bn = 0, bp = 0, pph = 0;  // ops; their buffers; p_full's phase
+            uint32_t seg = 0, kt = 0, vt = 0;
+            uint32_t segs0 = 0, segs1 = 0;  // segments of the row tiles so far
+            // ops whose PV is still to come, 8 bits by buffer: bit 0 t, 1 first of its segment, 2 first and 3 last
+            // op of the key tile
+            uint32_t pend = 0;
+            bool ok = true;
+            auto issue_pv = [&]() -> bool {
+                const uint32_t op = pend >> (8 * bp), t = op & 1, st = vt % SV_KST;
+                if (op & 2) {
+                    const uint32_t before = t ? segs1 : segs0;
+                    if (before > 0 && !sv_wait(&S->o_free[t], (before - 1) & 1, &S->abort_, A.err)) return false;
+                    segs0 += t ^ 1, segs1 += t;
+                }
+                if (op & 4) {
+                    if (!sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
+                    if (!PAGED && !sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
+                }
+                if (!sv_wait(&S->p_full[bp], pph, &S->abort_, A.err)) return false;
+                sv_fence_after();
+                if (leader) {
+                    const uint32_t d = tmem + SV_O_COL + t * CUINF_HD, pa = tmem + bp * 128;
+                    const uint32_t va = v_lo + st * (SV_TILE_BYTES >> 4);
+                    sv_mma_ts(d, pa, va, SV_IDESC_PV, (op & 2) == 0);
 #pragma unroll
-                    for (int k = 0; k < SV_KT / 16; k++)
-                        sv_mma_ts(tmem + SV_O_COL + t * CUINF_HD, tmem + b * 128 + 8 * k, sv_desc(va + k * 16 * 128),
-                                  SV_IDESC_PV, !((op & 2) && k == 0));
+                    for (int k = 1; k < SV_KT / 16; k++) sv_mma_ts(d, pa + 8 * k, va + k * (16 * 128 >> 4), SV_IDESC_PV, 1);
                     sv_commit(&S->o_full[t]);
-                    if (op & 8) {
-                        sv_commit(&S->v_empty[st]);
-                        vt++;
-                    }
-                    pv++;
-                    return true;
-                };
-                // What comes next may wait for what is pending (notes of values that are no numbers are reused
-                // two segments on), so nothing stays pending while an input is awaited.
-                auto wait_input = [&](uint64_t* bar, uint32_t parity) -> bool {
-                    if (mbar_test_wait(bar, parity)) return true;
+                    if (op & 8) sv_commit(&S->v_empty[st]);
+                }
+                __syncwarp();
+                if (op & 8) vt++;
+                pv++;
+                if (++bp == 3) bp = 0, pph ^= 1;
+                return true;
+            };
+            // What comes next may wait for what is pending (notes of values that are no numbers are reused two
+            // segments on), so nothing stays pending while an input is awaited.
+            auto wait_input = [&](uint64_t* bar, uint32_t parity) -> bool {
+                if (!__any_sync(0xffffffffu, mbar_test_wait(bar, parity)))
                     while (pv < n)
                         if (!issue_pv()) return false;
-                    return sv_wait(bar, parity, &S->abort_, A.err);
-                };
-                for (; ok && w.left > 0; sv_next<C::KIND>(A, w, tq, split), seg++) {
-                    const bool act1 = w.t0 + TOK < w.q.c;
-                    if (!(ok = wait_input(&S->q_full[seg & 1], (seg >> 1) & 1))) break;
-                    for (int i = w.tb; ok && i < w.te; i++, kt++) {
-                        const uint32_t st = kt % SV_KST;
-                        if (!(ok = wait_input(&S->k_full[st], (kt / SV_KST) & 1))) break;
-                        for (int t = 0; t < (act1 ? 2 : 1); t++) {
-                            const uint32_t b = n % 3;
-                            sv_fence_after();
-                            const uint32_t qa = smem_u32(Qs + (seg & 1) * SV_Q_BYTES + t * SV_TILE_BYTES);
-                            const uint32_t ka = smem_u32(Ks + st * SV_TILE_BYTES);
+                return sv_wait(bar, parity, &S->abort_, A.err);
+            };
+            for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
+                const uint32_t nt = w.t0 + TOK < w.q.c ? 2 : 1;
+                const int tb = w.tb, te = w.te;
+                if (!(ok = wait_input(&S->q_full[seg & 1], (seg >> 1) & 1))) break;
+                const uint32_t qa = q_lo + (seg & 1) * (SV_Q_BYTES >> 4);
+                for (int i = tb; ok && i < te; i++, kt++) {
+                    const uint32_t st = kt % SV_KST;
+                    if (!(ok = wait_input(&S->k_full[st], (kt / SV_KST) & 1))) break;
+                    const uint32_t ka = k_lo + st * (SV_TILE_BYTES >> 4);
+                    for (uint32_t t = 0; t < nt; t++) {
+                        sv_fence_after();
+                        const bool last_t = t + 1 == nt;
+                        if (leader) {
+                            const uint32_t d = tmem + bn * 128, qt = qa + t * (SV_TILE_BYTES >> 4);
+                            sv_mma_ss(d, qt, ka, SV_IDESC_QK, 0);
 #pragma unroll
-                            for (int k = 0; k < CUINF_HD / 16; k++)
-                                sv_mma_ss(tmem + b * 128, sv_desc(qa + 32 * k), sv_desc(ka + 32 * k), SV_IDESC_QK,
-                                          k != 0);
-                            sv_commit(&S->s_full[t][b]);
-                            const bool last_t = t == (act1 ? 1 : 0);
+                            for (int k = 1; k < CUINF_HD / 16; k++) sv_mma_ss(d, qt + 2 * k, ka + 2 * k, SV_IDESC_QK, 1);
+                            sv_commit(&S->s_full[t][bn]);
                             if (last_t) {
                                 sv_commit(&S->k_empty[st]);
-                                if (i == w.te - 1) sv_commit(&S->q_empty[seg & 1]);
+                                if (i == te - 1) sv_commit(&S->q_empty[seg & 1]);
                             }
-                            pend[b] = (uint32_t)t | (i == w.tb ? 2u : 0u) | (t == 0 ? 4u : 0u) | (last_t ? 8u : 0u);
-                            n++;
-                            if (n - pv > 2 && !(ok = issue_pv())) break;
                         }
+                        __syncwarp();
+                        const uint32_t op = t | (i == tb ? 2u : 0u) | (t == 0 ? 4u : 0u) | (last_t ? 8u : 0u);
+                        pend = (pend & ~(255u << (8 * bn))) | (op << (8 * bn));
+                        if (++bn == 3) bn = 0;
+                        n++;
+                        if (n - pv > 2 && !(ok = issue_pv())) break;
                     }
                 }
-                while (ok && pv < n) ok = issue_pv();
-                sv_commit(&S->done);
             }
+            while (ok && pv < n) ok = issue_pv();
+            if (leader) sv_commit(&S->done);
             __syncwarp();
         } else if (!PAGED && warp == 10) {
             // ---- values that are no numbers, in tiles with masked places ----
