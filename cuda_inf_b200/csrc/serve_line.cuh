@@ -9,18 +9,20 @@
 // ---- waits (bounded; the first that gives up raises the CTA's abort word) ----
 #define SV_WAIT_LIMIT_NS 500000000ull
 __device__ __forceinline__ bool sv_wait(uint64_t* bar, uint32_t parity, int* abort_, unsigned* err) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    for (int k = 1;; k++) {
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((k & 15) == 0) {
-            if (*(volatile int*)abort_) return false;
-            if (globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS) break;
+    uint64_t t0 = 0;
+    for (uint32_t k = 1; !mbar_try_wait(bar, parity); k++) {
+        if (k & 255) continue;
+        if (*(volatile int*)abort_) return false;
+        const uint64_t t = globaltimer_ns();
+        if (t0 == 0) {
+            t0 = t;
+        } else if (t - t0 > SV_WAIT_LIMIT_NS) {
+            *(volatile int*)abort_ = 1;
+            atomicOr(err, SERVE_ERR_WAIT);
+            return false;
         }
     }
-    *(volatile int*)abort_ = 1;
-    atomicOr(err, SERVE_ERR_WAIT);
-    return false;
+    return true;
 }
 // Before the CTA ends: a phase that copies or products in flight complete.
 __device__ __forceinline__ void sv_drain(uint64_t* bar, uint32_t parity, unsigned* err) {

@@ -10,15 +10,15 @@
 //   S = Q K^T        tcgen05.mma, 128 x 128 x 64, fp32 in TMEM
 //   P = exp2(c S - m) one thread per row: its 128 scores in registers, running
 //                    reference m and sum l in fp32, P rounded to fp16 (the MMA
-//                    operand) and written over S's first half in TMEM
+//                    operand) and written to TMEM
 //   O += P V         tcgen05.mma with P from TMEM, 128 x 64 x 128, fp32 in TMEM
 // The reference m follows the row's maximum only when that has grown by more
 // than 2^THR since, so O is rescaled seldom (P stays within fp16's range).
 //
-// S has three TMEM buffers in rotation: product n + 2 is issued before the
-// softmax of n is done, so the softmax warps find their next S ready and the
-// kernel runs at their pace.  With head_dim 64 that pace is the exponentials'
-// (128 x 128 of them at 16 a clock: 1024 clocks, against 512 of MMA).
+// A row tile's softmax gives its S back once the scores are in registers, so
+// the next scores come while it works and the kernel runs at the softmax's
+// pace.  With head_dim 64 that is the exponentials' (128 x 128 of them at 16 a
+// clock: 1024 clocks, against 512 of MMA).
 //
 // The row blocks' key tiles of all sequences are laid end to end, and each CTA
 // takes an equal share of that line (or, where items are short, the items that
@@ -38,7 +38,9 @@
 #define SV_SC 16         // slots of the pages' scales (more tiles than can be in flight)
 #define SV_TILE_BYTES (SV_KT * CUINF_HD * 2)
 #define SV_TMEM_COLS 512
-#define SV_O_COL 384     // S/P buffers at 0, 128, 256; O of row tile t at 384 + 64 t
+#define SV_TURN 64       // tries
+#define SV_P_COL 256     // S of row tile t at 128 t, P at 256 + 64 t, O at 384 + 64 t
+#define SV_O_COL 384
 
 // A role's place on the line of key tiles.  One per warp, in shared memory: the
 // softmax warps have no registers to spare for it.
@@ -52,7 +54,7 @@ struct SvItem {
 
 struct SvSmem {
     uint64_t q_full[2], q_empty[2], k_full[SV_KST], k_empty[SV_KST], v_full[SV_KST], v_empty[SV_KST], v_ok[SV_KST];
-    uint64_t s_full[2][3], p_full[3], o_full[2], o_free[2], epi[2], conv, done;
+    uint64_t s_full[2], s_free[2], p_full[2], o_full[2], o_free[2], epi[2], conv, done;
     uint32_t tmem;
     int abort_;
     float sc[SV_SC][4];  // FP8: K scale of the tile's two pages (negative: absent), V scales
@@ -271,8 +273,8 @@ __device__ __forceinline__ void sv_next_warp(const AttnArgs& A, SvItem& w, int t
 // ---------------------------------------------------------------------------
 template <bool PAGED>
 struct SvCfg {
-    // softmax warps 0-7; packed: 8 TMA, 9 MMA, 10 value check (11 idle);
-    // paged: 8-11 converters, 12 Q by TMA, 13 MMA (14, 15 idle)
+    // softmax warps 0-7; packed: 8 TMA, 9 and 10 MMA, 11 value check;
+    // paged: 8-11 converters, 12 Q by TMA, 13 and 14 MMA (15 idle)
     static constexpr int KIND = PAGED ? SV_MANY : SV_PACKED;
     static constexpr int WARPS = PAGED ? 16 : 12;
     static constexpr int MMA_WARP = PAGED ? 13 : 9;
@@ -478,19 +480,18 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&S->q_full[i], 1), mbar_init(&S->q_empty[i], 1);
+            mbar_init(&S->q_full[i], 1), mbar_init(&S->q_empty[i], 2);
+            mbar_init(&S->s_full[i], 1), mbar_init(&S->s_free[i], 4), mbar_init(&S->p_full[i], 4);
             mbar_init(&S->o_full[i], 1), mbar_init(&S->o_free[i], 4), mbar_init(&S->epi[i], PAGED ? 12 : 9);
             S->any_bad[i] = 0;
         }
         for (int i = 0; i < SV_KST; i++) {
-            mbar_init(&S->k_full[i], PAGED ? 4 : 1), mbar_init(&S->k_empty[i], 1);
-            mbar_init(&S->v_full[i], PAGED ? 4 : 1), mbar_init(&S->v_empty[i], 1);
+            mbar_init(&S->k_full[i], PAGED ? 4 : 1), mbar_init(&S->k_empty[i], 2);
+            mbar_init(&S->v_full[i], PAGED ? 4 : 1), mbar_init(&S->v_empty[i], 2);
             mbar_init(&S->v_ok[i], 1);
         }
-        for (int i = 0; i < 3; i++)
-            mbar_init(&S->s_full[0][i], 1), mbar_init(&S->s_full[1][i], 1), mbar_init(&S->p_full[i], 4);
         mbar_init(&S->conv, 4);
-        mbar_init(&S->done, 1);
+        mbar_init(&S->done, 2);
         S->abort_ = 0;
     }
     if (warp == C::MMA_WARP) {
@@ -516,16 +517,15 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_addr = lane_base + SV_O_COL + t * CUINF_HD;
         const float c2 = A.scale * 1.44269504088896340736f;  // scores in powers of two
-        uint32_t n = 0, ops = 0, tiles = 0, seg = 0;
-        uint32_t sbits = 0;  // phases of s_full[t] by buffer
+        const uint32_t s_addr = lane_base + t * 128, p_addr = lane_base + SV_P_COL + t * 64;
+        uint32_t ops = 0, tiles = 0, seg = 0;
         bool ok = true;
         for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
-            const int nt = w.te - w.tb;
             const bool act1 = w.t0 + TOK < w.q.c;
             // all who arrive at a segment's epi barrier have seen the one before of the same parity complete
             if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_, A.err))) break;
             if (t == 1 && !act1) {
-                n += nt, tiles += nt;
+                tiles += w.te - w.tb;
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S->epi[seg & 1]);
                 continue;
@@ -534,16 +534,15 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             const bool live_row = row < TOK * G && tok < w.q.c;
             const int pos = live_row ? w.q.p0 + tok : -1;
             float m = -INFINITY;
-            uint64_t l2 = 0;  // two partial sums
-            for (int i = w.tb; i < w.te; i++, ops++, tiles++) {
-                const uint32_t nn = n + (act1 ? 2 * (i - w.tb) + t : i - w.tb), b = nn % 3;
-                if (!(ok = sv_wait(&S->s_full[t][b], (sbits >> b) & 1, &S->abort_, A.err))) break;
-                sbits ^= 1u << b;
+            uint64_t l2[2] = {0, 0};  // four partial sums
+            const int tb = w.tb, te = w.te;
+            const int first_masked = (w.q.p0 + w.t0 + t * TOK + 1) >> 7;  // from here some row masks some key
+            for (int i = tb; i < te; i++, ops++, tiles++) {
+                if (!(ok = sv_wait(&S->s_full[t], ops & 1, &S->abort_, A.err))) break;
                 sv_fence_after();
                 uint32_t sr[128];
-                const uint32_t s_addr = lane_base + b * 128;
-#pragma unroll
-                for (int j = 0; j < 4; j++) sv_ld32(s_addr + 32 * j, sr + 32 * j);
+                float* s = reinterpret_cast<float*>(sr);
+                sv_ld32(s_addr, sr), sv_ld32(s_addr + 32, sr + 32);
                 float kc[2] = {c2, c2}, vc[2] = {1.f, 1.f};
                 bool gone[2] = {false, false};
                 if (PAGED) {
@@ -557,47 +556,51 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     }
                 }
                 sv_wait_ld();
-                float* s = reinterpret_cast<float*>(sr);
-                if (sv_masked(w.q, w.t0 + t * TOK, i)) {
-                    const int lim = pos - i * SV_KT;  // last key of the tile that the row attends
-#pragma unroll
-                    for (int j = 0; j < 128; j++) s[j] = j <= lim ? s[j] : -INFINITY;
-                    if (PAGED) {  // a page's scale that is no number reaches only rows that attend the page
-                        if (lim < 0) kc[0] = c2, vc[0] = 0.f;
-                        if (lim < 64) kc[1] = c2, vc[1] = 0.f;
-                    }
-                }
-                if (PAGED) {
-#pragma unroll
-                    for (int g = 0; g < 2; g++)
-                        if (gone[g]) {
-                            kc[g] = c2, vc[g] = 0.f;
-#pragma unroll
-                            for (int j = 0; j < 64; j++) s[64 * g + j] = -INFINITY;
-                        }
-                }
+                sv_ld32(s_addr + 64, sr + 64), sv_ld32(s_addr + 96, sr + 96);
+                const bool masked = i >= first_masked;
+                const int lim = pos - i * SV_KT;  // last key of the tile that the row attends
                 float mx[2];
 #pragma unroll
                 for (int g = 0; g < 2; g++) {
-                    float a0 = s[64 * g], a1 = s[64 * g + 1], a2 = s[64 * g + 2], a3 = s[64 * g + 3];
-#pragma unroll
-                    for (int j = 4; j < 64; j += 4) {
-                        a0 = fmaxf(a0, s[64 * g + j]), a1 = fmaxf(a1, s[64 * g + j + 1]);
-                        a2 = fmaxf(a2, s[64 * g + j + 2]), a3 = fmaxf(a3, s[64 * g + j + 3]);
+                    if (g == 1) {
+                        sv_wait_ld();
+                        sv_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&S->s_free[t]);  // the next scores may come while these are worked on
                     }
-                    mx[g] = fmaxf(fmaxf(a0, a1), fmaxf(a2, a3)) * kc[g];
+                    if (masked) {
+#pragma unroll
+                        for (int j = 64 * g; j < 64 * g + 64; j++) s[j] = j <= lim ? s[j] : -INFINITY;
+                        // a page's scale that is no number reaches only rows that attend the page
+                        if (PAGED && lim < 64 * g) kc[g] = c2, vc[g] = 0.f;
+                    }
+                    if (PAGED && gone[g]) {
+                        kc[g] = c2, vc[g] = 0.f;
+#pragma unroll
+                        for (int j = 0; j < 64; j++) s[64 * g + j] = -INFINITY;
+                    }
+                    float a[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) a[j] = s[64 * g + j];
+#pragma unroll
+                    for (int j = 8; j < 64; j++) a[j & 7] = fmaxf(a[j & 7], s[64 * g + j]);
+                    mx[g] = fmaxf(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])), fmaxf(fmaxf(a[4], a[5]), fmaxf(a[6], a[7]))) *
+                            kc[g];
                 }
                 const float x = fmaxf(mx[0], mx[1]);
-                if (i == w.tb) {
+                // the last product has read P and written O
+                if (i > tb) {
+                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
+                    sv_fence_after();
+                }
+                if (i == tb) {
                     m = x;
                 } else if (__any_sync(0xffffffffu, x > m + C::THR)) {
                     // rare: the reference follows the maximum, sum and O with it
                     const float mn = fmaxf(m, x);
                     const float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
                     m = mn;
-                    l2 = f2_mul(l2, f2_pack(f, f));
-                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
-                    sv_fence_after();
+                    l2[0] = f2_mul(l2[0], f2_pack(f, f)), l2[1] = f2_mul(l2[1], f2_pack(f, f));
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
                         uint32_t o[32];
@@ -622,22 +625,18 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                         f2_unpack(y, y0, y1);
                         y0 = sv_exp2(y0), y1 = sv_exp2(y1);
                         y = f2_pack(y0, y1);
-                        l2 = f2_add(l2, y);
+                        l2[e & 1] = f2_add(l2[e & 1], y);
                         if (PAGED) f2_unpack(f2_mul(y, vv), y0, y1);
                         pk[e] = sv_pack_h2(y0, y1);
                     }
-                    sv_st16(s_addr + 16 * j, pk);
+                    sv_st16(p_addr + 16 * j, pk);
                 }
                 sv_wait_st();
                 sv_fence_before();
-                // every phase of o_full is seen (a parity tells only neighbouring phases apart); the last
-                // product is long done here
-                if (i > w.tb && !(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&S->p_full[b]);
+                if (lane == 0) mbar_arrive(&S->p_full[t]);
             }
             if (!ok) break;
-            n += act1 ? 2 * nt : nt;
             // ---- epilogue of the item (or of the CTA's part of it) ----
             if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
             sv_fence_after();
@@ -649,7 +648,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             __syncwarp();
             if (lane == 0) mbar_arrive(&S->o_free[t]);
             float la, lb;
-            f2_unpack(l2, la, lb);
+            f2_unpack(f2_add(l2[0], l2[1]), la, lb);
             const float l = la + lb;
             float* of = reinterpret_cast<float*>(o);
             const float vs = PAGED ? 1.f / SV_VEXP : 1.f;
@@ -748,89 +747,86 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     sv_drain(&S->v_full[k % SV_KST], (k / SV_KST) & 1, A.err);
             }
             __syncwarp();
-        } else if (warp == C::MMA_WARP) {
-            // ---- products: S of op n, then O of op n - 2.  All lanes walk, one issues ----
+        } else if (warp == C::MMA_WARP || warp == C::MMA_WARP + 1) {
+            // ---- products of row tile t: S of the next key tile as soon as the scores are read, then O of this
+            // one.  A warp for each row tile (one warp's instructions for both were the kernel's pace); all lanes
+            // walk, one issues ----
+            const uint32_t t = warp - C::MMA_WARP;
             const bool leader = sv_elect();
-            const uint32_t q_lo = sv_desc_lo(smem_u32(Qs)), k_lo = sv_desc_lo(smem_u32(Ks)), v_lo = sv_desc_lo(smem_u32(Vs));
-            uint32_t n = 0, pv = 0, bn = 0, bp = 0, pph = 0;  // ops; their buffers; p_full's phase
+            const uint32_t q_lo = sv_desc_lo(smem_u32(Qs) + t * SV_TILE_BYTES), k_lo = sv_desc_lo(smem_u32(Ks));
+            const uint32_t v_lo = sv_desc_lo(smem_u32(Vs));
+            const uint32_t d_s = tmem + t * 128, d_p = tmem + SV_P_COL + t * 64, d_o = tmem + SV_O_COL + t * CUINF_HD;
             uint32_t seg = 0, kt = 0, vt = 0;
-            uint32_t segs0 = 0, segs1 = 0;  // segments of the row tiles so far
-            // ops whose PV is still to come, 8 bits by buffer: bit 0 t, 1 first of its segment, 2 first and 3 last
-            // op of the key tile
-            uint32_t pend = 0;
+            uint32_t nq = 0, np = 0, segs = 0;  // products of this row tile so far; segments in which it is active
             bool ok = true;
-            auto issue_pv = [&]() -> bool {
-                const uint32_t op = pend >> (8 * bp), t = op & 1, st = vt % SV_KST;
-                if (op & 2) {
-                    const uint32_t before = t ? segs1 : segs0;
-                    if (before > 0 && !sv_wait(&S->o_free[t], (before - 1) & 1, &S->abort_, A.err)) return false;
-                    segs0 += t ^ 1, segs1 += t;
+            uint32_t n1 = 0;  // (t = 0) products of row tile 1 in key tiles so far
+            auto scores = [&](uint32_t qa, bool turns, bool first) -> bool {
+                const uint32_t st = kt % SV_KST;
+                if (!sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_, A.err)) return false;
+                if (nq > 0 && !sv_wait(&S->s_free[t], (nq - 1) & 1, &S->abort_, A.err)) return false;
+                // The row tiles take turns: one's exponentials run beside the other's loads and maxima.  Only a
+                // matter of pace, so it is not insisted on (and a phase that has gone by unseen costs some tries).
+                if (t == 1) {
+                    for (int k = 0; k < SV_TURN && !mbar_test_wait(&S->s_free[0], kt & 1); k++) {}
+                } else if (turns) {
+                    if (!first)
+                        for (int k = 0; k < SV_TURN && !mbar_test_wait(&S->s_free[1], (n1 - 1) & 1); k++) {}
+                    n1++;
                 }
-                if (op & 4) {
-                    if (!sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
-                    if (!PAGED && !sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_, A.err)) return false;
-                }
-                if (!sv_wait(&S->p_full[bp], pph, &S->abort_, A.err)) return false;
                 sv_fence_after();
                 if (leader) {
-                    const uint32_t d = tmem + SV_O_COL + t * CUINF_HD, pa = tmem + bp * 128;
-                    const uint32_t va = v_lo + st * (SV_TILE_BYTES >> 4);
-                    sv_mma_ts(d, pa, va, SV_IDESC_PV, (op & 2) == 0);
+                    const uint32_t ka = k_lo + st * (SV_TILE_BYTES >> 4);
+                    sv_mma_ss(d_s, qa, ka, SV_IDESC_QK, 0);
 #pragma unroll
-                    for (int k = 1; k < SV_KT / 16; k++) sv_mma_ts(d, pa + 8 * k, va + k * (16 * 128 >> 4), SV_IDESC_PV, 1);
-                    sv_commit(&S->o_full[t]);
-                    if (op & 8) sv_commit(&S->v_empty[st]);
+                    for (int k = 1; k < CUINF_HD / 16; k++) sv_mma_ss(d_s, qa + 2 * k, ka + 2 * k, SV_IDESC_QK, 1);
+                    sv_commit(&S->s_full[t]);
+                    sv_commit(&S->k_empty[st]);
                 }
-                __syncwarp();
-                if (op & 8) vt++;
-                pv++;
-                if (++bp == 3) bp = 0, pph ^= 1;
+                nq++, kt++;
                 return true;
             };
-            // What comes next may wait for what is pending (notes of values that are no numbers are reused two
-            // segments on), so nothing stays pending while an input is awaited.
-            auto wait_input = [&](uint64_t* bar, uint32_t parity) -> bool {
-                if (!__any_sync(0xffffffffu, mbar_test_wait(bar, parity)))
-                    while (pv < n)
-                        if (!issue_pv()) return false;
-                return sv_wait(bar, parity, &S->abort_, A.err);
-            };
             for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
-                const uint32_t nt = w.t0 + TOK < w.q.c ? 2 : 1;
-                const int tb = w.tb, te = w.te;
-                if (!(ok = wait_input(&S->q_full[seg & 1], (seg >> 1) & 1))) break;
-                const uint32_t qa = q_lo + (seg & 1) * (SV_Q_BYTES >> 4);
-                for (int i = tb; ok && i < te; i++, kt++) {
-                    const uint32_t st = kt % SV_KST;
-                    if (!(ok = wait_input(&S->k_full[st], (kt / SV_KST) & 1))) break;
-                    const uint32_t ka = k_lo + st * (SV_TILE_BYTES >> 4);
-                    for (uint32_t t = 0; t < nt; t++) {
-                        sv_fence_after();
-                        const bool last_t = t + 1 == nt;
-                        if (leader) {
-                            const uint32_t d = tmem + bn * 128, qt = qa + t * (SV_TILE_BYTES >> 4);
-                            sv_mma_ss(d, qt, ka, SV_IDESC_QK, 0);
-#pragma unroll
-                            for (int k = 1; k < CUINF_HD / 16; k++) sv_mma_ss(d, qt + 2 * k, ka + 2 * k, SV_IDESC_QK, 1);
-                            sv_commit(&S->s_full[t][bn]);
-                            if (last_t) {
-                                sv_commit(&S->k_empty[st]);
-                                if (i == te - 1) sv_commit(&S->q_empty[seg & 1]);
-                            }
-                        }
-                        __syncwarp();
-                        const uint32_t op = t | (i == tb ? 2u : 0u) | (t == 0 ? 4u : 0u) | (last_t ? 8u : 0u);
-                        pend = (pend & ~(255u << (8 * bn))) | (op << (8 * bn));
-                        if (++bn == 3) bn = 0;
-                        n++;
-                        if (n - pv > 2 && !(ok = issue_pv())) break;
+                const int nt = w.te - w.tb;
+                if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_, A.err))) break;
+                if (t == 1 && w.t0 + TOK >= w.q.c) {  // the block has one row tile: only let the stages go
+                    for (int i = 0; ok && i < nt; i++, kt++, vt++) {
+                        const uint32_t st = kt % SV_KST;
+                        if (!(ok = sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_, A.err))) break;
+                        if (leader) mbar_arrive(&S->k_empty[st]);
+                        if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err))) break;
+                        if (leader) mbar_arrive(&S->v_empty[st]);
                     }
+                    if (leader) mbar_arrive(&S->q_empty[seg & 1]);
+                    continue;
                 }
+                const uint32_t qa = q_lo + (seg & 1) * (SV_Q_BYTES >> 4);
+                const bool turns = w.t0 + TOK < w.q.c;
+                if (!(ok = scores(qa, turns, true))) break;
+                for (int i = 0; i < nt; i++) {
+                    if (i + 1 < nt && !(ok = scores(qa, turns, false))) break;
+                    if (leader && i == max(nt - 2, 0)) sv_commit(&S->q_empty[seg & 1]);  // the last scores are under way
+                    const uint32_t st = vt % SV_KST;
+                    if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err))) break;
+                    if (!PAGED && !(ok = sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_, A.err))) break;
+                    if (i == 0 && segs > 0 && !(ok = sv_wait(&S->o_free[t], (segs - 1) & 1, &S->abort_, A.err))) break;
+                    if (!(ok = sv_wait(&S->p_full[t], np & 1, &S->abort_, A.err))) break;
+                    sv_fence_after();
+                    if (leader) {
+                        const uint32_t va = v_lo + st * (SV_TILE_BYTES >> 4);
+                        sv_mma_ts(d_o, d_p, va, SV_IDESC_PV, i > 0);
+#pragma unroll
+                        for (int k = 1; k < SV_KT / 16; k++)
+                            sv_mma_ts(d_o, d_p + 8 * k, va + k * (16 * 128 >> 4), SV_IDESC_PV, 1);
+                        sv_commit(&S->o_full[t]);
+                        sv_commit(&S->v_empty[st]);
+                    }
+                    np++, vt++;
+                }
+                segs++;
             }
-            while (ok && pv < n) ok = issue_pv();
             if (leader) sv_commit(&S->done);
             __syncwarp();
-        } else if (!PAGED && warp == 10) {
+        } else if (!PAGED && warp == 11) {
             // ---- values that are no numbers, in tiles with masked places ----
             uint32_t seg = 0, kt = 0;
             bool ok = true;
