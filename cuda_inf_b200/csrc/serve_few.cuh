@@ -31,8 +31,9 @@ struct FwSmem {
     int any_bad[3];
     int bad[3][3][CUINF_HD];  // by item, modulo 3: first key whose value is +inf, -inf, NaN
     SvShare share;
+    int left;                 // units of the share
     float ml[2][FW_WARPS][16][2];  // by item, modulo 2
-    float o[2][FW_WARPS][16][CUINF_HD];
+    alignas(16) float o[2][FW_WARPS][16][CUINF_HD];  // (read by float4)
 };
 static constexpr size_t FW_SMEM_BYTES = 128 + (size_t)FW_ST * FW_UNIT + sizeof(FwSmem);
 
@@ -40,51 +41,57 @@ static constexpr size_t FW_SMEM_BYTES = 128 + (size_t)FW_ST * FW_UNIT + sizeof(F
 __device__ __forceinline__ int fw_units(const SvSeq& q) {
     return max(1, q.kv / SERVE_PAGE + (q.kv % SERVE_PAGE + FW_TAIL - 1) / FW_TAIL);
 }
-// A place on the line: unit `rem` of sequence s's n * nkv.
+// A place on the line: unit u of the n of (sequence s, kv head h).  Kept by
+// steps: a 64-bit division per unit and lane was half of the kernel's time.
 struct FwPos {
-    int s, n;
-    long long rem;
+    int s, h, u, n;
     SvSeq q;
 };
-__device__ __forceinline__ void fw_skip(const AttnArgs& A, FwPos& p, long long by) {
-    p.rem += by;
-    while (p.s < A.rows.n_seqs && p.rem >= (long long)p.n * A.nkv) {
-        p.rem -= (long long)p.n * A.nkv;
-        do p.s++;
-        while (p.s < A.rows.n_seqs && !sv_seq<SV_FEW>(A, p.s, p.q, false));
-        if (p.s < A.rows.n_seqs) p.n = fw_units(p.q);
+__device__ __forceinline__ void fw_first(const AttnArgs& A, const SvShare& S, FwPos& p) {
+    p.s = S.s;
+    sv_seq<SV_FEW>(A, p.s, p.q, false);
+    p.n = fw_units(p.q);
+    p.h = (int)(S.rem / p.n);
+    p.u = (int)(S.rem % p.n);
+}
+__device__ __forceinline__ void fw_skip(const AttnArgs& A, FwPos& p, int by) {
+    p.u += by;
+    while (p.u >= p.n) {
+        p.u -= p.n;
+        if (++p.h < A.nkv) continue;
+        p.h = 0;
+        do {
+            if (++p.s >= A.rows.n_seqs) return;  // the line's end
+        } while (!sv_seq<SV_FEW>(A, p.s, p.q, false));
+        p.n = fw_units(p.q);
     }
 }
-// Page of unit u: an index (unchecked), or -2 for a part of the tail.
+// Page of a unit: an index (unchecked), or -2 for a part of the tail.
 __device__ __forceinline__ int fw_page(const AttnArgs& A, const FwPos& p) {
-    if (p.s >= A.rows.n_seqs) return -2;
-    const int u = (int)(p.rem % p.n);
-    return u < p.q.kv / SERVE_PAGE ? __ldg(A.kv.table + (size_t)p.s * A.kv.width + u) : -2;
+    return p.u < p.q.kv / SERVE_PAGE ? __ldg(A.kv.table + (size_t)p.s * A.kv.width + p.u) : -2;
 }
 
 __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsigned char* ring, int lane) {
     if (lane >= FW_ST) return;
-    const long long cnt = S->share.left;
+    const int cnt = S->left;
     FwPos p, np;  // the unit to copy; the one after it (FW_ST further on)
-    p.s = S->share.s, p.rem = S->share.rem;
-    sv_seq<SV_FEW>(A, p.s, p.q, false);
-    p.n = fw_units(p.q);
+    fw_first(A, S->share, p);
     fw_skip(A, p, lane);
     int page = lane < cnt ? fw_page(A, p) : -2;
     auto scales = [&](const FwPos& x, int pg, __half& k, __half& v) {
         k = v = __float2half_rn(1.f);
         if (pg < 0 || pg >= A.kv.n_pages) return;
-        const size_t blk = (size_t)pg * A.nkv + (int)(x.rem / x.n);
+        const size_t blk = (size_t)pg * A.nkv + x.h;
         k = __ldg(A.kv.kps + blk), v = __ldg(A.kv.vps + blk);
     };
     __half ks, vs;
     scales(p, page, ks, vs);
     np = p;
-    fw_skip(A, np, FW_ST);
+    if (lane + FW_ST < cnt) fw_skip(A, np, FW_ST);
     int npage = lane + FW_ST < cnt ? fw_page(A, np) : -2;
     uint32_t k = 0;      // copies of this lane so far
     bool armed = false;  // copies of the last one are in flight
-    long long j = lane;
+    int j = lane;
     uint64_t t0 = globaltimer_ns();
     for (int spin = 1;; spin++) {
         // one test per turn, so that a lane whose stage is free is not held up by the others
@@ -102,7 +109,7 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
         }
         if (!go) continue;
         unsigned char* dst = ring + (size_t)lane * FW_UNIT;
-        const int u = (int)(p.rem % p.n), h = (int)(p.rem / p.n), ng = p.q.kv / SERVE_PAGE;
+        const int u = p.u, h = p.h, ng = p.q.kv / SERVE_PAGE;
         S->sc[lane][0] = __half2float(ks), S->sc[lane][1] = __half2float(vs);
         armed = true;
         if (page == -2) {
@@ -128,12 +135,153 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
         p = np, page = npage;
         if (j + FW_ST < cnt) {
             scales(p, page, ks, vs);
-            fw_skip(A, np, FW_ST);
-            npage = j + 2 * FW_ST < cnt ? fw_page(A, np) : -2;
+            if (j + 2 * FW_ST < cnt) {
+                fw_skip(A, np, FW_ST);
+                npage = fw_page(A, np);
+            }
         }
         j += FW_ST, k++;
     }
     if (armed) sv_drain(&S->full[lane], (k - 1) & 1, A.err);  // copies land before the CTA can exit
+}
+
+// A warp's running state of 16 rows: lane 4 g + c holds rows g and g + 8.
+struct FwRows {
+    uint32_t q[4][4];  // the rows' A fragments
+    int pos[2];
+    float c2;                    // score scale, in powers of two
+    float m[2], l[2], o[8][4];   // reference, this lane's share of the sum, output columns 2 c, 2 c + 1 of 8 tiles
+};
+struct FwUnit {
+    const unsigned char* kd;
+    float ks, vs;
+    int key0, here;  // first key, keys
+};
+// One unit of 64 keys (TAIL: 32, fp16) into the state.  TWO: rows 8 to 15 are
+// in use.  MASKED: some row masks some key, or some keys are not there.
+template <bool TWO, bool MASKED, bool TAIL>
+__device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, int note, int lane) {
+    constexpr int NT = TAIL ? FW_TAIL / 8 : 8;  // score tiles of 8 keys
+    const int g = lane >> 2, c = lane & 3;
+    const unsigned char *kd = x.kd, *vd = x.kd + FW_UNIT / 2;
+    float s[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+        uint32_t w[8];
+        if (TAIL) {
+            const uint4* src = reinterpret_cast<const uint4*>(kd + (8 * t + g) * 128 + 32 * c);
+            const uint4 a = src[0], b = src[1];
+            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
+            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4*>(kd + (8 * t + g) * 64 + 16 * c);
+            w[0] = sv_e4m3x2(a.x), w[1] = sv_e4m3x2(a.x >> 16);
+            w[2] = sv_e4m3x2(a.y), w[3] = sv_e4m3x2(a.y >> 16);
+            w[4] = sv_e4m3x2(a.z), w[5] = sv_e4m3x2(a.z >> 16);
+            w[6] = sv_e4m3x2(a.w), w[7] = sv_e4m3x2(a.w >> 16);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            mma_16816(s[t], R.q[k][0], R.q[k][1], R.q[k][2], R.q[k][3], w[2 * k], w[2 * k + 1]);
+    }
+    constexpr int NR = TWO ? 2 : 1;
+    float kc[2], vc[2], top[2];
+#pragma unroll
+    for (int r = 0; r < NR; r++) {
+        kc[r] = R.c2 * x.ks, vc[r] = x.vs * SV_VEXP;
+        if (MASKED) {
+            if (kc[r] == 0.f) kc[r] = 1e-30f;  // a page of zeros: -inf * 0 is no number
+            // a page's scale that is no number reaches only rows that attend the page
+            if (R.pos[r] < x.key0) kc[r] = R.c2, vc[r] = 0.f;
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    if (x.key0 + 8 * t + 2 * c + e > R.pos[r]) s[t][2 * r + e] = -INFINITY;
+        }
+        float a[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) a[j] = s[j / 2][2 * r + (j & 1)];
+#pragma unroll
+        for (int j = 4; j < 2 * NT; j++) a[j & 3] = fmaxf(a[j & 3], s[j / 2][2 * r + (j & 1)]);
+        top[r] = fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * kc[r];
+    }
+    if (__any_sync(0xffffffffu, top[0] > R.m[0] + FW_THR || (TWO && top[NR - 1] > R.m[NR - 1] + FW_THR))) {
+#pragma unroll
+        for (int r = 0; r < NR; r++) {
+            const float mn = fmaxf(R.m[r], top[r]);
+            const float f = R.m[r] == -INFINITY ? 0.f : sv_exp2(R.m[r] - mn);
+            R.m[r] = mn, R.l[r] *= f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) R.o[i][2 * r] *= f, R.o[i][2 * r + 1] *= f;
+        }
+    }
+    uint32_t a[NT / 2][4];  // the weights' A fragments, 16 keys each
+#pragma unroll
+    for (int r = 0; r < 2; r++) {
+        if (r >= NR) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) a[t / 2][2 * (t & 1) + 1] = 0;
+            continue;
+        }
+        const float ref = R.m[r] == -INFINITY ? 0.f : R.m[r];
+        float l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float p0 = sv_exp2(fmaf(s[t][2 * r], kc[r], -ref)), p1 = sv_exp2(fmaf(s[t][2 * r + 1], kc[r], -ref));
+            l[t & 1] += p0 + p1;
+            a[t / 2][2 * (t & 1) + r] = sv_pack_h2(p0 * vc[r], p1 * vc[r]);
+        }
+        R.l[r] += l[0] + l[1];
+    }
+#pragma unroll
+    for (int q = 0; q < NT / 2; q++) {
+        // values: keys 16 q + 2 c, + 1 (z = 0) and 8 further on, dims 8 g .. 8 g + 7
+        uint32_t b[2][8];
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+            const int key = 16 * q + 8 * z + 2 * c;
+            if (TAIL) {
+                const uint4 v = *reinterpret_cast<const uint4*>(vd + key * 128 + 16 * g);
+                const uint4 y = *reinterpret_cast<const uint4*>(vd + (key + 1) * 128 + 16 * g);
+                b[z][0] = __byte_perm(v.x, y.x, 0x5410), b[z][1] = __byte_perm(v.x, y.x, 0x7632);
+                b[z][2] = __byte_perm(v.y, y.y, 0x5410), b[z][3] = __byte_perm(v.y, y.y, 0x7632);
+                b[z][4] = __byte_perm(v.z, y.z, 0x5410), b[z][5] = __byte_perm(v.z, y.z, 0x7632);
+                b[z][6] = __byte_perm(v.w, y.w, 0x5410), b[z][7] = __byte_perm(v.w, y.w, 0x7632);
+            } else {
+                const uint2 v = *reinterpret_cast<const uint2*>(vd + key * 64 + 8 * g);
+                const uint2 y = *reinterpret_cast<const uint2*>(vd + (key + 1) * 64 + 8 * g);
+                const uint32_t w0 = __byte_perm(v.x, y.x, 0x5140), w1 = __byte_perm(v.x, y.x, 0x7362);
+                const uint32_t w2 = __byte_perm(v.y, y.y, 0x5140), w3 = __byte_perm(v.y, y.y, 0x7362);
+                b[z][0] = sv_e4m3x2(w0), b[z][1] = sv_e4m3x2(w0 >> 16);
+                b[z][2] = sv_e4m3x2(w1), b[z][3] = sv_e4m3x2(w1 >> 16);
+                b[z][4] = sv_e4m3x2(w2), b[z][5] = sv_e4m3x2(w2 >> 16);
+                b[z][6] = sv_e4m3x2(w3), b[z][7] = sv_e4m3x2(w3 >> 16);
+            }
+            if (MASKED) {  // what some row masks is a number: 0 * NaN would pass a weight of zero
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const bool gone = key + e >= x.here;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const uint32_t bits = b[z][i] >> (16 * e) & 0xffffu;
+                        const bool bad = (bits & 0x7c00u) == 0x7c00u;
+                        if (bad && !gone) {
+                            atomicMin(&S->bad[note][bits & 0x3ffu ? 2 : bits & 0x8000u ? 1 : 0][8 * g + i],
+                                      x.key0 + key + e);
+                            S->any_bad[note] = 1;
+                        }
+                        if (bad || gone) b[z][i] &= e ? 0x0000ffffu : 0xffff0000u;
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) mma_16816(R.o[i], a[q][0], a[q][1], a[q][2], a[q][3], b[0][i], b[1][i]);
+    }
 }
 
 __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
@@ -152,24 +300,31 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
     for (int i = tid; i < 9 * CUINF_HD; i += blockDim.x) (&S->bad[0][0][0])[i] = 0x7fffffff;
     if (split && tid < 2) W.part[blockIdx.x * 2 + tid].valid = 0;
     sv_share<SV_FEW>(A, &S->share, blockIdx.x, gridDim.x, [&](const SvSeq& q) { return (long long)fw_units(q) * A.nkv; });
-    if (!split && tid == 0 && S->share.left > 0) {
-        // items are not cut: the share's items are those that begin in it
-        SvShare& h = S->share;
-        FwPos p;
-        p.s = h.s, p.rem = h.rem;
-        sv_seq<SV_FEW>(A, p.s, p.q, false);
-        p.n = fw_units(p.q);
-        const int skip = (int)((p.n - p.rem % p.n) % p.n);
-        const long long left = h.left;
-        fw_skip(A, p, skip);
-        h.s = p.s, h.rem = p.rem;
-        FwPos e = p;
-        fw_skip(A, e, left - skip > 0 ? left - skip : 0);
-        const int more = e.s < A.rows.n_seqs ? (int)((e.n - e.rem % e.n) % e.n) : 0;
-        h.left = left > skip ? left - skip + more : 0;
+    if (tid == 0) {
+        long long left = S->share.left;
+        if (!split && left > 0) {
+            // items are not cut: the share's items are those that begin in it
+            FwPos p;
+            fw_first(A, S->share, p);
+            const long long skip = (p.n - p.u) % p.n;
+            if (left <= skip) {
+                left = 0;
+            } else {
+                left -= skip;
+                fw_skip(A, p, (int)skip);
+                S->share.s = p.s, S->share.rem = (long long)p.h * p.n;
+                long long at = 0;  // whole items from here on
+                while (at < left && p.s < A.rows.n_seqs) {
+                    at += p.n;
+                    fw_skip(A, p, p.n);
+                }
+                left = at;
+            }
+        }
+        S->left = (int)left;
     }
     __syncthreads();
-    const long long cnt = S->share.left;
+    const int cnt = S->left;
     if (cnt > 0) {
         if (warp == FW_WARPS) {
             fw_producer(A, S, ring, lane);
@@ -178,10 +333,8 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
             const int G = A.nh / A.nkv, g = lane >> 2, c = lane & 3;
             const float c2 = A.scale * 1.44269504088896340736f;
             FwPos p;
-            p.s = S->share.s, p.rem = S->share.rem;
-            sv_seq<SV_FEW>(A, p.s, p.q, false);
-            p.n = fw_units(p.q);
-            long long j = 0;  // share's units before the item
+            fw_first(A, S->share, p);
+            int j = 0;  // share's units before the item
             uint32_t item = 0;
             bool ok = true;
             // rows g and g + 8: dims 16 c .. 16 c + 15
@@ -191,9 +344,9 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                 for (int r = 0; r < 2; r++) {
                     const int row = g + 8 * r;
                     qn[r][0] = qn[r][1] = make_uint4(0, 0, 0, 0);
-                    if (x.s < A.rows.n_seqs && row < x.q.c * G) {
+                    if (row < x.q.c * G) {
                         const uint4* src = reinterpret_cast<const uint4*>(
-                            A.q + (size_t)(x.q.a + row / G) * A.q_stride + ((int)(x.rem / x.n) * G + row % G) * CUINF_HD +
+                            A.q + (size_t)(x.q.a + row / G) * A.q_stride + (x.h * G + row % G) * CUINF_HD +
                             16 * c);
                         qn[r][0] = src[0], qn[r][1] = src[1];
                     }
@@ -201,172 +354,71 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
             };
             load_q(p);
             while (j < cnt) {
-                const int rows = p.q.c * G, h = (int)(p.rem / p.n), tb = (int)(p.rem % p.n);
-                const int te = (int)min((long long)p.n, tb + (cnt - j));
+                const int rows = p.q.c * G, h = p.h, tb = p.u;
+                const int te = min(p.n, tb + (cnt - j));
                 const int ng = p.q.kv / SERVE_PAGE;
-                uint32_t qa[4][4];
+                FwRows R;
                 {
                     const uint32_t* q0 = reinterpret_cast<const uint32_t*>(qn[0]);
                     const uint32_t* q1 = reinterpret_cast<const uint32_t*>(qn[1]);
 #pragma unroll
                     for (int t = 0; t < 4; t++)
-                        qa[t][0] = q0[2 * t], qa[t][1] = q1[2 * t], qa[t][2] = q0[2 * t + 1], qa[t][3] = q1[2 * t + 1];
+                        R.q[t][0] = q0[2 * t], R.q[t][1] = q1[2 * t], R.q[t][2] = q0[2 * t + 1], R.q[t][3] = q1[2 * t + 1];
                 }
                 FwPos nx = p;
-                fw_skip(A, nx, te - tb);
-                if (j + te - tb < cnt) load_q(nx);  // the next item's, while this one runs
-                const int pos0 = p.q.p0 + g / G, pos1 = p.q.p0 + (g + 8) / G;  // positions of rows g, g + 8
-                const bool two = rows > 8;
-                float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f, o[8][4];
+                if (j + te - tb < cnt) {  // the next item's rows, while this one runs
+                    fw_skip(A, nx, te - tb);
+                    load_q(nx);
+                }
+                R.c2 = c2;
 #pragma unroll
-                for (int i = 0; i < 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-                int(*bad)[CUINF_HD] = S->bad[item % 3];
+                for (int r = 0; r < 2; r++) {
+                    R.pos[r] = p.q.p0 + (g + 8 * r) / G;
+                    R.m[r] = -INFINITY, R.l[r] = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; i++) R.o[i][0] = R.o[i][1] = R.o[i][2] = R.o[i][3] = 0.f;
+                const int(*bad)[CUINF_HD] = S->bad[item % 3];
 
-                const long long u0 = j + ((warp - j) % FW_WARPS + FW_WARPS) % FW_WARPS;
-                for (long long u = u0; u < j + te - tb; u += FW_WARPS) {
-                    const int st = (int)(u % FW_ST), unit = tb + (int)(u - j);
+                for (int u = j + ((warp - j) & (FW_WARPS - 1)); u < j + te - tb; u += FW_WARPS) {
+                    const int st = u % FW_ST, unit = tb + u - j;
                     if (!(ok = sv_wait(&S->full[st], (u / FW_ST) & 1, &S->abort_, A.err))) break;
-                    const unsigned char* kd = ring + (size_t)st * FW_UNIT;
-                    const unsigned char* vd = kd + FW_UNIT / 2;
-                    const float ks = S->sc[st][0], vs = S->sc[st][1];
+                    FwUnit x;
+                    x.kd = ring + (size_t)st * FW_UNIT;
+                    x.ks = S->sc[st][0], x.vs = S->sc[st][1];
                     const bool tail = unit >= ng;
-                    const int key0 = tail ? ng * SERVE_PAGE + (unit - ng) * FW_TAIL : unit * SERVE_PAGE;
-                    if (ks >= 0.f || ks != ks) {  // not absent
-                        const int here = tail ? min(FW_TAIL, p.q.kv - key0) : SERVE_PAGE;
-                        const bool masked = key0 + SERVE_PAGE > p.q.p0 + 1;
-                        float s[8][4];
-#pragma unroll
-                        for (int t = 0; t < 8; t++) {
-                            s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-                            uint32_t w[8];
-                            if (tail) {
-                                if (t >= FW_TAIL / 8) continue;
-                                const uint4* src = reinterpret_cast<const uint4*>(kd + (8 * t + g) * 128 + 32 * c);
-                                const uint4 a = src[0], b = src[1];
-                                w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-                                w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-                            } else {
-                                const uint4 a = *reinterpret_cast<const uint4*>(kd + (8 * t + g) * 64 + 16 * c);
-                                w[0] = sv_e4m3x2(a.x), w[1] = sv_e4m3x2(a.x >> 16);
-                                w[2] = sv_e4m3x2(a.y), w[3] = sv_e4m3x2(a.y >> 16);
-                                w[4] = sv_e4m3x2(a.z), w[5] = sv_e4m3x2(a.z >> 16);
-                                w[6] = sv_e4m3x2(a.w), w[7] = sv_e4m3x2(a.w >> 16);
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; k++)
-                                mma_16816(s[t], qa[k][0], qa[k][1], qa[k][2], qa[k][3], w[2 * k], w[2 * k + 1]);
-                        }
-                        const float kc = c2 * ks;
-                        float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-                        for (int t = 0; t < 8; t++)
-#pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                s[t][e] *= kc, s[t][2 + e] *= kc;
-                                if (masked) {
-                                    const int key = key0 + 8 * t + 2 * c + e;
-                                    if (key > pos0 || 8 * t >= here) s[t][e] = -INFINITY;
-                                    if (key > pos1 || 8 * t >= here) s[t][2 + e] = -INFINITY;
-                                }
-                                x0 = fmaxf(x0, s[t][e]), x1 = fmaxf(x1, s[t][2 + e]);
-                            }
-                        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-                        x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-                        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-                        x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-                        if (__any_sync(0xffffffffu, x0 > m0 + FW_THR || x1 > m1 + FW_THR)) {
-                            const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
-                            const float f0 = m0 == -INFINITY ? 0.f : sv_exp2(m0 - n0);
-                            const float f1 = m1 == -INFINITY ? 0.f : sv_exp2(m1 - n1);
-                            m0 = n0, m1 = n1, l0 *= f0, l1 *= f1;
-#pragma unroll
-                            for (int i = 0; i < 8; i++) o[i][0] *= f0, o[i][1] *= f0, o[i][2] *= f1, o[i][3] *= f1;
-                        }
-                        const float r0 = m0 == -INFINITY ? 0.f : m0, r1 = m1 == -INFINITY ? 0.f : m1;
-                        const float vc = vs * SV_VEXP;
-                        // a page's scale that is no number reaches only rows that attend the page
-                        const float vc0 = pos0 < key0 ? 0.f : vc, vc1 = pos1 < key0 ? 0.f : vc;
-#pragma unroll
-                        for (int q = 0; q < 4; q++) {  // 16 keys: score tiles 2 q, 2 q + 1
-                            if (tail && q >= FW_TAIL / 16) continue;
-                            uint32_t a[4] = {0, 0, 0, 0};
-#pragma unroll
-                            for (int z = 0; z < 2; z++) {
-                                const float p0 = sv_exp2(s[2 * q + z][0] - r0), p1 = sv_exp2(s[2 * q + z][1] - r0);
-                                l0 += p0 + p1;
-                                a[2 * z] = sv_pack_h2(p0 * vc0, p1 * vc0);
-                                if (two) {
-                                    const float p2 = sv_exp2(s[2 * q + z][2] - r1), p3 = sv_exp2(s[2 * q + z][3] - r1);
-                                    l1 += p2 + p3;
-                                    a[2 * z + 1] = sv_pack_h2(p2 * vc1, p3 * vc1);
-                                }
-                            }
-                            // values: keys 16 q + 2 c, + 1 (z = 0) and 8 further on, dims 8 g .. 8 g + 7
-                            uint32_t b[2][8];
-#pragma unroll
-                            for (int z = 0; z < 2; z++) {
-                                const int key = 16 * q + 8 * z + 2 * c;
-                                if (tail) {
-                                    const uint4 x = *reinterpret_cast<const uint4*>(vd + key * 128 + 16 * g);
-                                    const uint4 y = *reinterpret_cast<const uint4*>(vd + (key + 1) * 128 + 16 * g);
-                                    b[z][0] = __byte_perm(x.x, y.x, 0x5410), b[z][1] = __byte_perm(x.x, y.x, 0x7632);
-                                    b[z][2] = __byte_perm(x.y, y.y, 0x5410), b[z][3] = __byte_perm(x.y, y.y, 0x7632);
-                                    b[z][4] = __byte_perm(x.z, y.z, 0x5410), b[z][5] = __byte_perm(x.z, y.z, 0x7632);
-                                    b[z][6] = __byte_perm(x.w, y.w, 0x5410), b[z][7] = __byte_perm(x.w, y.w, 0x7632);
-                                } else {
-                                    const uint2 x = *reinterpret_cast<const uint2*>(vd + key * 64 + 8 * g);
-                                    const uint2 y = *reinterpret_cast<const uint2*>(vd + (key + 1) * 64 + 8 * g);
-                                    const uint32_t w0 = __byte_perm(x.x, y.x, 0x5140), w1 = __byte_perm(x.x, y.x, 0x7362);
-                                    const uint32_t w2 = __byte_perm(x.y, y.y, 0x5140), w3 = __byte_perm(x.y, y.y, 0x7362);
-                                    b[z][0] = sv_e4m3x2(w0), b[z][1] = sv_e4m3x2(w0 >> 16);
-                                    b[z][2] = sv_e4m3x2(w1), b[z][3] = sv_e4m3x2(w1 >> 16);
-                                    b[z][4] = sv_e4m3x2(w2), b[z][5] = sv_e4m3x2(w2 >> 16);
-                                    b[z][6] = sv_e4m3x2(w3), b[z][7] = sv_e4m3x2(w3 >> 16);
-                                }
-                                if (masked) {  // what some row masks is a number: 0 * NaN would pass a weight of zero
-#pragma unroll
-                                    for (int i = 0; i < 8; i++)
-#pragma unroll
-                                        for (int e = 0; e < 2; e++) {
-                                            const uint32_t bits = b[z][i] >> (16 * e) & 0xffffu;
-                                            const bool gone = key + e >= here;
-                                            if (gone || (bits & 0x7c00u) == 0x7c00u) {
-                                                if (!gone) {
-                                                    atomicMin(&bad[bits & 0x3ffu ? 2 : bits & 0x8000u ? 1 : 0][8 * g + i],
-                                                              key0 + key + e);
-                                                    S->any_bad[item % 3] = 1;
-                                                }
-                                                b[z][i] &= e ? 0x0000ffffu : 0xffff0000u;
-                                            }
-                                        }
-                                }
-                            }
-#pragma unroll
-                            for (int i = 0; i < 8; i++) mma_16816(o[i], a[0], a[1], a[2], a[3], b[0][i], b[1][i]);
-                        }
+                    x.key0 = tail ? ng * SERVE_PAGE + (unit - ng) * FW_TAIL : unit * SERVE_PAGE;
+                    x.here = tail ? min(FW_TAIL, p.q.kv - x.key0) : SERVE_PAGE;
+                    // one straight path each: with these as branches inside, the loop's loads and products could not
+                    // be interleaved
+                    if (x.ks >= 0.f || x.ks != x.ks) {  // (negative: absent)
+                        if (tail)
+                            fw_unit<true, true, true>(x, R, S, item % 3, lane);
+                        else if (x.key0 + SERVE_PAGE > p.q.p0 + 1)
+                            fw_unit<true, true, false>(x, R, S, item % 3, lane);
+                        else if (rows > 8)
+                            fw_unit<true, false, false>(x, R, S, item % 3, lane);
+                        else
+                            fw_unit<false, false, false>(x, R, S, item % 3, lane);
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&S->empty[st]);
                 }
                 // ---- the item's end: join the warps ----
-                l0 += __shfl_xor_sync(0xffffffffu, l0, 1), l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-                l1 += __shfl_xor_sync(0xffffffffu, l1, 1), l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
                 const int par = item & 1;
-                if (c == 0) {
-                    S->ml[par][warp][g][0] = m0, S->ml[par][warp][g][1] = l0;
-                    S->ml[par][warp][g + 8][0] = m1, S->ml[par][warp][g + 8][1] = l1;
-                }
 #pragma unroll
-                for (int e = 0; e < 2; e++) {  // columns 2 c + e of tile i: dims 8 (2 c + e) + i
-                    if (g < rows) {
-                        float4* d = reinterpret_cast<float4*>(&S->o[par][warp][g][16 * c + 8 * e]);
-                        d[0] = make_float4(o[0][e], o[1][e], o[2][e], o[3][e]);
-                        d[1] = make_float4(o[4][e], o[5][e], o[6][e], o[7][e]);
-                    }
-                    if (g + 8 < rows) {
-                        float4* d = reinterpret_cast<float4*>(&S->o[par][warp][g + 8][16 * c + 8 * e]);
-                        d[0] = make_float4(o[0][2 + e], o[1][2 + e], o[2][2 + e], o[3][2 + e]);
-                        d[1] = make_float4(o[4][2 + e], o[5][2 + e], o[6][2 + e], o[7][2 + e]);
+                for (int r = 0; r < 2; r++) {
+                    R.l[r] += __shfl_xor_sync(0xffffffffu, R.l[r], 1);
+                    R.l[r] += __shfl_xor_sync(0xffffffffu, R.l[r], 2);
+                    const int row = g + 8 * r;
+                    if (c == 0) S->ml[par][warp][row][0] = R.m[r], S->ml[par][warp][row][1] = R.l[r];
+                    if (row >= rows) continue;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {  // columns 2 c + e of tile i: dims 8 (2 c + e) + i
+                        const int z = 2 * r + e;
+                        float4* d = reinterpret_cast<float4*>(&S->o[par][warp][row][16 * c + 8 * e]);
+                        d[0] = make_float4(R.o[0][z], R.o[1][z], R.o[2][z], R.o[3][z]);
+                        d[1] = make_float4(R.o[4][z], R.o[5][z], R.o[6][z], R.o[7][z]);
                     }
                 }
                 // notes of the next item: last read two items ago, written only after this barrier

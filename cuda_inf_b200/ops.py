@@ -8,6 +8,7 @@ strided token rows, and run on their tensors' device); fp16 activations, u8 pack
 GEMV outputs.  Errors raise CuinfError; nothing falls back to the CPU.
 """
 import ctypes
+import functools
 
 import torch
 
@@ -254,78 +255,95 @@ def quantize_int4(w):
 # --------------------------------------------------------------------------
 # serving attention: packed prompts, and a paged FP8 cache
 # --------------------------------------------------------------------------
-def _heads(t, name, dev=None):
+# These checks run before kernels of a few microseconds, so each looks at a tensor's properties once.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _heads(t, name, index=None):
     """(pointer, elements between tokens, heads) of fp16 rows [T, heads, 64]; the
     tokens may be apart (a part of a wider row), a token's heads not."""
-    _dt(t, torch.float16, name)
-    if not t.is_cuda:
+    if t.dtype is not torch.float16:
+        raise TypeError(f"{name} must be {torch.float16}, got {t.dtype}")
+    at = t.get_device()
+    if at < 0:
         raise ValueError(f"{name}: expected a CUDA tensor")
-    if dev is not None and t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    if t.dim() != 3 or t.shape[2] != 64 or t.shape[1] == 0:
-        raise ValueError(f"{name} must be [tokens, heads, 64], got {tuple(t.shape)}")
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != 64):
+    if index is not None and at != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or shape[2] != 64 or shape[1] == 0:
+        raise ValueError(f"{name} must be [tokens, heads, 64], got {tuple(shape)}")
+    if stride[2] != 1 or (shape[1] > 1 and stride[1] != 64):
         raise ValueError(f"{name}: a token's heads must be contiguous")
-    stride = t.stride(0) if t.shape[0] > 1 else t.shape[1] * 64
-    return ctypes.c_void_p(t.data_ptr()), stride, t.shape[1]
+    return t.data_ptr(), stride[0] if shape[0] > 1 else shape[1] * 64, shape[1]
 
 
-def _ints(t, shape, name, dev):
-    _dt(t, torch.int32, name)
-    if t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-    return _p(t)
+def _whole(t, dtype, shape, name, index):
+    """Pointer of a contiguous tensor of this type and shape on this device."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {tuple(shape)}, got {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name}: expected a contiguous tensor")
+    return t.data_ptr()
 
 
-def _cache(dev, n, table, kp8, vp8, kps, vps, ktail, vtail):
+def _paged(index, n, table, kp8, vp8, kps, vps, ktail, vtail):
     """Checked pointers of a paged cache, in the order of the C ABI, and its sizes."""
     if table.dim() != 2 or table.shape[1] == 0:
         raise ValueError("table must be [sequences, pages]")
-    if kp8.dim() != 4 or tuple(kp8.shape[2:]) != (64, 64) or kp8.shape[0] == 0 or kp8.shape[1] == 0:
-        raise ValueError(f"kp8 must be [pages, kv heads, 64, 64], got {tuple(kp8.shape)}")
-    n_pages, nkv = kp8.shape[:2]
-    ptrs = [_ints(table, (n, table.shape[1]), "table", dev)]
-    for t, dtype, shape, name in ((kp8, torch.uint8, (n_pages, nkv, 64, 64), "kp8"),
-                                  (vp8, torch.uint8, (n_pages, nkv, 64, 64), "vp8"),
-                                  (kps, torch.float16, (n_pages, nkv), "kps"),
-                                  (vps, torch.float16, (n_pages, nkv), "vps"),
-                                  (ktail, torch.float16, (n, nkv, 64, 64), "ktail"),
-                                  (vtail, torch.float16, (n, nkv, 64, 64), "vtail")):
-        _dt(t, dtype, name)
-        if t.device != dev:
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
-        if tuple(t.shape) != shape:
-            raise ValueError(f"{name} must be {shape}, got {tuple(t.shape)}")
-        ptrs.append(_p(t))
-    return ptrs, n_pages, nkv
+    pool = kp8.shape
+    if len(pool) != 4 or pool[2] != 64 or pool[3] != 64 or pool[0] == 0 or pool[1] == 0:
+        raise ValueError(f"kp8 must be [pages, kv heads, 64, 64], got {tuple(pool)}")
+    n_pages, nkv = pool[0], pool[1]
+    width = table.shape[1]
+    u8, f16, tail = torch.uint8, torch.float16, (n, nkv, 64, 64)
+    return (_whole(table, torch.int32, (n, width), "table", index), width,
+            _whole(kp8, u8, pool, "kp8", index), _whole(vp8, u8, pool, "vp8", index),
+            _whole(kps, f16, (n_pages, nkv), "kps", index), _whole(vps, f16, (n_pages, nkv), "vps", index), n_pages,
+            _whole(ktail, f16, tail, "ktail", index), _whole(vtail, f16, tail, "vtail", index)), nkv
 
 
-def _cu(cu_seqlens, dev):
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1:
+def _cu(cu_seqlens, index):
+    shape = cu_seqlens.shape
+    if len(shape) != 1 or shape[0] < 1:
         raise ValueError("cu_seqlens must be [sequences + 1]")
-    return _ints(cu_seqlens, (cu_seqlens.numel(),), "cu_seqlens", dev), cu_seqlens.numel() - 1
+    return _whole(cu_seqlens, torch.int32, shape, "cu_seqlens", index), shape[0] - 1
 
 
-def _out(out, q):
+def _out(out, q, index):
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _dt(out, torch.float16, "out")
-    if out.shape != q.shape or out.device != q.device:
-        raise ValueError(f"out must be {tuple(q.shape)} on {q.device}")
-    return out
+        out = torch.empty_like(q)
+    return out, _whole(out, torch.float16, q.shape, "out", index)
 
 
-def _scratch(workspace, size, dev):
-    """The workspace's pointer and bytes; without one, scratch of this call (from
+@functools.lru_cache(maxsize=256)
+def _scratch_bytes(fn, *args):
+    return getattr(lib(), fn)(*args)
+
+
+def _scratch(workspace, size, like, index):
+    """(workspace, its pointer and bytes); without one, scratch of this call (from
     torch's allocator, so it follows the stream's order and a capture's pool)."""
     if workspace is None:
-        workspace = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    elif workspace.device != dev:
-        raise ValueError(f"workspace is on {workspace.device}, expected {dev}")
-    nbytes = workspace.numel() * workspace.element_size() if workspace is not None else 0
-    return workspace, nbytes
+        if size == 0:
+            return None, None, 0
+        workspace = like.new_empty(size, dtype=torch.uint8)
+    elif workspace.get_device() != index or not workspace.is_contiguous():
+        raise ValueError(f"workspace: expected a contiguous tensor on cuda:{index}")
+    return workspace, workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _call(fn, index, *args):
+    """A C entry on the device `index` and torch's current stream there."""
+    if torch.cuda.current_device() == index:
+        check(fn(*args, _raw_stream(index)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, _raw_stream(index)))
 
 
 def attn_varlen(q, k, v, cu_seqlens, scale=0.125, out=None, workspace=None):
@@ -337,21 +355,19 @@ def attn_varlen(q, k, v, cu_seqlens, scale=0.125, out=None, workspace=None):
     query head h reads kv head h // (nh // nkv).  Rows outside all sequences are
     left as they were (undefined in a new `out`).  Nothing synchronizes."""
     qp, qs, nh = _heads(q, "q")
-    dev = q.device
-    kp, ks, nkv = _heads(k, "k", dev)
-    vp, vs, nv = _heads(v, "v", dev)
-    if k.shape[0] != q.shape[0] or v.shape[0] != q.shape[0] or nv != nkv:
-        raise ValueError("q, k and v must have the same tokens, k and v the same heads")
-    cu, n = _cu(cu_seqlens, dev)
-    out = _out(out, q)
+    index = q.get_device()
+    kp, ks, nkv = _heads(k, "k", index)
+    vp, vs, nv = _heads(v, "v", index)
     T = q.shape[0]
+    if k.shape[0] != T or v.shape[0] != T or nv != nkv:
+        raise ValueError("q, k and v must have the same tokens, k and v the same heads")
+    cu, n = _cu(cu_seqlens, index)
+    out, op = _out(out, q, index)
     if T == 0 or n == 0:
         return out
-    L = lib()
-    with torch.cuda.device(dev):
-        ws, nbytes = _scratch(workspace, L.cuinf_attn_varlen_workspace_size(n, T, nh, nkv), dev)
-        check(L.cuinf_attn_varlen(qp, qs, kp, ks, vp, vs, cu, n, T, scale, _p(out), nh, nkv, _p(ws), nbytes,
-                                  _stream()))
+    workspace, ws, nbytes = _scratch(workspace, _scratch_bytes("cuinf_attn_varlen_workspace_size", n, T, nh, nkv), q,
+                                     index)
+    _call(lib().cuinf_attn_varlen, index, qp, qs, kp, ks, vp, vs, cu, n, T, scale, op, nh, nkv, ws, nbytes)
     return out
 
 
@@ -366,20 +382,19 @@ def kv_paged_append(k, v, cu_seqlens, ctx_lens, table, kp8, vp8, kps, vps, ktail
     ktail/vtail fp16 [n,nkv,64,64].  Page indices outside the pool and lengths
     outside their ranges are skipped and reported by paged_error()."""
     kp, ks, nkv = _heads(k, "k")
-    dev = k.device
-    vp, vs, nv = _heads(v, "v", dev)
-    if v.shape[0] != k.shape[0] or nv != nkv:
+    index = k.get_device()
+    vp, vs, nv = _heads(v, "v", index)
+    T = k.shape[0]
+    if v.shape[0] != T or nv != nkv:
         raise ValueError("k and v must have the same shape")
-    cu, n = _cu(cu_seqlens, dev)
-    ctx = _ints(ctx_lens, (n,), "ctx_lens", dev)
-    (tb, *cache), n_pages, cache_kv = _cache(dev, n, table, kp8, vp8, kps, vps, ktail, vtail)
+    cu, n = _cu(cu_seqlens, index)
+    ctx = _whole(ctx_lens, torch.int32, (n,), "ctx_lens", index)
+    cache, cache_kv = _paged(index, n, table, kp8, vp8, kps, vps, ktail, vtail)
     if cache_kv != nkv:
         raise ValueError(f"the cache has {cache_kv} kv heads, k {nkv}")
-    if k.shape[0] == 0 or n == 0:
+    if T == 0 or n == 0:
         return
-    with torch.cuda.device(dev):
-        check(lib().cuinf_kv_paged_append(kp, ks, vp, vs, cu, ctx, n, k.shape[0], tb, table.shape[1], *cache[:4],
-                                          n_pages, *cache[4:], nkv, _stream()))
+    _call(lib().cuinf_kv_paged_append, index, kp, ks, vp, vs, cu, ctx, n, T, *cache, nkv)
 
 
 def attn_paged(q, cu_seqlens, kv_lens, table, kp8, vp8, kps, vps, ktail, vtail, scale=0.125, max_q=None, out=None,
@@ -395,20 +410,19 @@ def attn_paged(q, cu_seqlens, kv_lens, table, kp8, vp8, kps, vps, ktail, vtail, 
     bound lets a pure decode step skip the chunks' kernel.  Nothing
     synchronizes; what the device finds wrong is reported by paged_error()."""
     qp, qs, nh = _heads(q, "q")
-    dev = q.device
-    cu, n = _cu(cu_seqlens, dev)
-    kvl = _ints(kv_lens, (n,), "kv_lens", dev)
-    (tb, *cache), n_pages, nkv = _cache(dev, n, table, kp8, vp8, kps, vps, ktail, vtail)
-    out = _out(out, q)
+    index = q.get_device()
+    cu, n = _cu(cu_seqlens, index)
+    kvl = _whole(kv_lens, torch.int32, (n,), "kv_lens", index)
+    cache, nkv = _paged(index, n, table, kp8, vp8, kps, vps, ktail, vtail)
+    out, op = _out(out, q, index)
     T = q.shape[0]
     if T == 0 or n == 0:
         return out
-    max_q = T if max_q is None else max_q
-    L = lib()
-    with torch.cuda.device(dev):
-        ws, nbytes = _scratch(workspace, L.cuinf_attn_paged_workspace_size(n, T, max_q, nh, nkv, table.shape[1]), dev)
-        check(L.cuinf_attn_paged(qp, qs, cu, kvl, n, T, max_q, tb, table.shape[1], *cache[:4], n_pages, *cache[4:],
-                                 scale, _p(out), nh, nkv, _p(ws), nbytes, _stream()))
+    if max_q is None:
+        max_q = T
+    size = _scratch_bytes("cuinf_attn_paged_workspace_size", n, T, max_q, nh, nkv, cache[1])
+    workspace, ws, nbytes = _scratch(workspace, size, q, index)
+    _call(lib().cuinf_attn_paged, index, qp, qs, cu, kvl, n, T, max_q, *cache, scale, op, nh, nkv, ws, nbytes)
     return out
 
 
