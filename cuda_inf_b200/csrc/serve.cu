@@ -289,8 +289,8 @@ static int launch_few(const AttnArgs& A, bool cuts, const SvWs& W, int ctas, boo
 static int launch_combine(const AttnArgs& A, const SvWs& Wm, const SvWs& Wf, int ctas, bool many, bool few,
                           cudaStream_t st) {
     cudaLaunchAttribute attr[1];
-    const cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, (many ? 4 : 0) + (few ? 1 : 0)), 256, 0, st, attr);
-    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_combine, A, Wm, Wf, ctas, many ? 4 : 0));
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, (many ? SV_JOIN_Y : 0) + (few ? 1 : 0)), 256, 0, st, attr);
+    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_combine, A, Wm, Wf, ctas, (int)many));
     return cuinf_launch_status();
 }
 

@@ -18,22 +18,22 @@
 #pragma once
 #include "serve_line.cuh"
 
-#define FW_WARPS 8
-#define FW_ST 16           // stages; a multiple of FW_WARPS: a stage's phases are all seen by one warp
+#define FW_WARPS 11        // and one that copies: 3 a scheduler, at up to 168 registers a thread
+#define FW_ST 22           // stages; a multiple of FW_WARPS: a stage's phases are all seen by one warp
 #define FW_UNIT 8192       // bytes of a unit: 4096 of keys, 4096 of values
 #define FW_TAIL 32         // tail tokens of a unit
 #define FW_THR 3.f         // the reference follows the maximum when it has grown by 2^THR
 
 struct FwSmem {
-    uint64_t full[FW_ST], empty[FW_ST], merge;
+    uint64_t full[FW_ST], empty[FW_ST], merge, merged;
     int abort_;
     float sc[FW_ST][2];       // key scale (negative: absent), value scale
     int any_bad[3];
     int bad[3][3][CUINF_HD];  // by item, modulo 3: first key whose value is +inf, -inf, NaN
     SvShare share;
     int left;                 // units of the share
-    float ml[2][FW_WARPS][16][2];  // by item, modulo 2
-    alignas(16) float o[2][FW_WARPS][16][CUINF_HD];  // (read by float4)
+    float ml[FW_WARPS][16][2];
+    alignas(16) float o[FW_WARPS][16][CUINF_HD];  // (read by float4)
 };
 static constexpr size_t FW_SMEM_BYTES = 128 + (size_t)FW_ST * FW_UNIT + sizeof(FwSmem);
 
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
     pdl_trigger();
     if (tid == 0) {
         for (int i = 0; i < FW_ST; i++) mbar_init(&S->full[i], 1), mbar_init(&S->empty[i], 1);
-        mbar_init(&S->merge, FW_WARPS);
+        mbar_init(&S->merge, FW_WARPS), mbar_init(&S->merged, FW_WARPS);
         S->abort_ = 0;
         for (int i = 0; i < 3; i++) S->any_bad[i] = 0;
     }
@@ -380,7 +380,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                 for (int i = 0; i < 8; i++) R.o[i][0] = R.o[i][1] = R.o[i][2] = R.o[i][3] = 0.f;
                 const int(*bad)[CUINF_HD] = S->bad[item % 3];
 
-                for (int u = j + ((warp - j) & (FW_WARPS - 1)); u < j + te - tb; u += FW_WARPS) {
+                for (int u = j + (warp + FW_WARPS - j % FW_WARPS) % FW_WARPS; u < j + te - tb; u += FW_WARPS) {
                     const int st = u % FW_ST, unit = tb + u - j;
                     if (!(ok = sv_wait(&S->full[st], (u / FW_ST) & 1, &S->abort_, A.err))) break;
                     FwUnit x;
@@ -405,18 +405,19 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                     if (lane == 0) mbar_arrive(&S->empty[st]);
                 }
                 // ---- the item's end: join the warps ----
-                const int par = item & 1;
+                // what the last item left there has been read
+                if (!ok || (item > 0 && !(ok = sv_wait(&S->merged, (item - 1) & 1, &S->abort_, A.err)))) break;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     R.l[r] += __shfl_xor_sync(0xffffffffu, R.l[r], 1);
                     R.l[r] += __shfl_xor_sync(0xffffffffu, R.l[r], 2);
                     const int row = g + 8 * r;
-                    if (c == 0) S->ml[par][warp][row][0] = R.m[r], S->ml[par][warp][row][1] = R.l[r];
+                    if (c == 0) S->ml[warp][row][0] = R.m[r], S->ml[warp][row][1] = R.l[r];
                     if (row >= rows) continue;
 #pragma unroll
                     for (int e = 0; e < 2; e++) {  // columns 2 c + e of tile i: dims 8 (2 c + e) + i
                         const int z = 2 * r + e;
-                        float4* d = reinterpret_cast<float4*>(&S->o[par][warp][row][16 * c + 8 * e]);
+                        float4* d = reinterpret_cast<float4*>(&S->o[warp][row][16 * c + 8 * e]);
                         d[0] = make_float4(R.o[0][z], R.o[1][z], R.o[2][z], R.o[3][z]);
                         d[1] = make_float4(R.o[4][z], R.o[5][z], R.o[6][z], R.o[7][z]);
                     }
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                 __threadfence_block();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S->merge);
-                if (!ok || !(ok = sv_wait(&S->merge, item & 1, &S->abort_, A.err))) break;
+                if (!(ok = sv_wait(&S->merge, item & 1, &S->abort_, A.err))) break;
                 const bool whole = tb == 0 && te == p.n;
                 const size_t slot = (size_t)blockIdx.x * 2 + (tb == 0);
                 for (int i = tid; i < rows * 16; i += FW_WARPS * 32) {
@@ -436,14 +437,14 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                     float m = -INFINITY, l = 0.f;
                     float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                    for (int w = 0; w < FW_WARPS; w++) m = fmaxf(m, S->ml[par][w][row][0]);
+                    for (int w = 0; w < FW_WARPS; w++) m = fmaxf(m, S->ml[w][row][0]);
                     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
                     for (int w = 0; w < FW_WARPS; w++) {
-                        const float mw = S->ml[par][w][row][0], lw = S->ml[par][w][row][1];
+                        const float mw = S->ml[w][row][0], lw = S->ml[w][row][1];
                         const float f = mw == -INFINITY ? 0.f : sv_exp2(mw - ref);
                         l += mw == -INFINITY ? lw : lw * f;  // (NaN scores alone have no maximum)
-                        const float4 y = *reinterpret_cast<const float4*>(&S->o[par][w][row][d]);
+                        const float4 y = *reinterpret_cast<const float4*>(&S->o[w][row][d]);
                         x.x += y.x * f, x.y += y.y * f, x.z += y.z * f, x.w += y.w * f;
                     }
                     float* xf = reinterpret_cast<float*>(&x);
@@ -474,6 +475,8 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                     t.valid = 1, t.last = te == p.n, t.row0 = p.q.a, t.tokens = p.q.c, t.h = h;
                     W.part[slot] = t;
                 }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&S->merged);
                 j += te - tb;
                 p = nx;
                 item++;
