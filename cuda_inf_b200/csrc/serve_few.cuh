@@ -22,6 +22,7 @@
 #define FW_ST 22           // stages; a multiple of FW_WARPS: a stage's phases are all seen by one warp
 #define FW_UNIT 8192       // bytes of a unit: 4096 of keys, 4096 of values
 #define FW_TAIL 32         // tail tokens of a unit
+#define FW_IDLE (1u << 24) // turns (of 50 clocks and more) without a free stage that end the kernel
 #define FW_THR 3.f         // the reference follows the maximum when it has grown by 2^THR
 
 struct FwSmem {
@@ -92,20 +93,17 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
     uint32_t k = 0;      // copies of this lane so far
     bool armed = false;  // copies of the last one are in flight
     int j = lane;
-    uint64_t t0 = globaltimer_ns();
-    for (int spin = 1;; spin++) {
+    uint32_t idle = 0;
+#pragma unroll 1
+    for (;;) {
         // one test per turn, so that a lane whose stage is free is not held up by the others
         const bool go = j < cnt && mbar_test_wait(&S->empty[lane], (k & 1) ^ 1);
         if (!__ballot_sync((1u << FW_ST) - 1, j < cnt)) break;
         if (__ballot_sync((1u << FW_ST) - 1, go)) {
-            t0 = globaltimer_ns();
-        } else if ((spin & 63) == 0) {
-            const bool late = globaltimer_ns() - t0 > SV_WAIT_LIMIT_NS;
-            if (__ballot_sync((1u << FW_ST) - 1, late || *(volatile int*)&S->abort_)) {
-                if (late) atomicOr(A.err, SERVE_ERR_WAIT);
-                *(volatile int*)&S->abort_ = 1;
-                break;
-            }
+            idle = 0;
+        } else if (++idle >= FW_IDLE || *(volatile int*)&S->abort_) {
+            *(volatile int*)&S->abort_ = 1;
+            break;
         }
         if (!go) continue;
         unsigned char* dst = ring + (size_t)lane * FW_UNIT;
@@ -142,7 +140,7 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
         }
         j += FW_ST, k++;
     }
-    if (armed) sv_drain(&S->full[lane], (k - 1) & 1, A.err);  // copies land before the CTA can exit
+    if (armed) sv_drain(&S->full[lane], (k - 1) & 1);  // copies land before the CTA can exit
 }
 
 // A warp's running state of 16 rows: lane 4 g + c holds rows g and g + 8.
@@ -382,7 +380,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
 
                 for (int u = j + (warp + FW_WARPS - j % FW_WARPS) % FW_WARPS; u < j + te - tb; u += FW_WARPS) {
                     const int st = u % FW_ST, unit = tb + u - j;
-                    if (!(ok = sv_wait(&S->full[st], (u / FW_ST) & 1, &S->abort_, A.err))) break;
+                    if (!(ok = sv_wait(&S->full[st], (u / FW_ST) & 1, &S->abort_))) break;
                     FwUnit x;
                     x.kd = ring + (size_t)st * FW_UNIT;
                     x.ks = S->sc[st][0], x.vs = S->sc[st][1];
@@ -406,7 +404,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                 }
                 // ---- the item's end: join the warps ----
                 // what the last item left there has been read
-                if (!ok || (item > 0 && !(ok = sv_wait(&S->merged, (item - 1) & 1, &S->abort_, A.err)))) break;
+                if (!ok || (item > 0 && !(ok = sv_wait(&S->merged, (item - 1) & 1, &S->abort_)))) break;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     R.l[r] += __shfl_xor_sync(0xffffffffu, R.l[r], 1);
@@ -429,7 +427,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                 __threadfence_block();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S->merge);
-                if (!(ok = sv_wait(&S->merge, item & 1, &S->abort_, A.err))) break;
+                if (!(ok = sv_wait(&S->merge, item & 1, &S->abort_))) break;
                 const bool whole = tb == 0 && te == p.n;
                 const size_t slot = (size_t)blockIdx.x * 2 + (tb == 0);
                 for (int i = tid; i < rows * 16; i += FW_WARPS * 32) {
@@ -484,5 +482,6 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
         }
     }
     __syncthreads();
+    if (tid == 0 && S->abort_) atomicOr(A.err, SERVE_ERR_WAIT);
     pdl_wait();  // launched beside the chunks' kernel: what follows this kernel follows that one too
 }

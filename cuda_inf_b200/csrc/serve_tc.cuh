@@ -42,8 +42,7 @@
 #define SV_P_COL 256     // S of row tile t at 128 t, P at 256 + 64 t, O at 384 + 64 t
 #define SV_O_COL 384
 
-// A role's place on the line of key tiles.  One per warp, in shared memory: the
-// softmax warps have no registers to spare for it.
+// An item, or the part of it that falls to this CTA.
 struct SvItem {
     int s, h, qb, nqb;  // sequence, kv head, row block of nqb
     SvSeq q;
@@ -63,7 +62,7 @@ struct SvSmem {
     SvShare share;
     int h, qb;  // the item in which the share begins, and its units before that
     long long off;
-    SvItem item[16];
+    SvItem item[4];  // of segment seg, modulo 4 (published by q_full; n = 0: no more)
 };
 static constexpr size_t SV_Q_BYTES = 2 * SV_TILE_BYTES;  // both row tiles of an item
 static constexpr size_t SV_SMEM_BYTES = 1024 + 2 * SV_Q_BYTES + 2 * SV_KST * (size_t)SV_TILE_BYTES + sizeof(SvSmem);
@@ -139,12 +138,11 @@ __device__ __forceinline__ void sv_ld32(uint32_t t, uint32_t* r) {
         : SV_R8(r, 0), SV_R8(r, 8), SV_R8(r, 16), SV_R8(r, 24)
         : "r"(t));
 }
-__device__ __forceinline__ void sv_st32(uint32_t t, const uint32_t* r) {
+__device__ __forceinline__ void sv_ld16(uint32_t t, uint32_t* r) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};\n" ::SV_I8(r, 0),
-        SV_I8(r, 8), SV_I8(r, 16), SV_I8(r, 24), "r"(t)
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+        : SV_R8(r, 0), SV_R8(r, 8)
+        : "r"(t));
 }
 __device__ __forceinline__ void sv_st16(uint32_t t, const uint32_t* r) {
     asm volatile(
@@ -214,7 +212,8 @@ __device__ void sv_start(const AttnArgs& A, SvSmem* S, int tq, int n_ctas) {
     __syncthreads();
 }
 
-// Walks the items of the CTA's share; every role runs its own (one lane calls).
+// Walks the items of the CTA's share (the lane that copies Q; the other roles
+// read the items from a ring).
 // left: units from the item's beginning to the share's end.
 __device__ __forceinline__ void sv_item(SvItem& w, int tq, int split, long long off) {
     const int t0 = w.qb * tq, keys = sv_keys(w.q, min(t0 + tq, w.q.c)), n = (keys + SV_KT - 1) / SV_KT;
@@ -259,13 +258,6 @@ __device__ __forceinline__ void sv_first(const AttnArgs& A, const SvSmem* S, SvI
     sv_item(w, tq, split, off);
     // nothing of this item: its last tile is before the share, or (uncut) it belongs to the share in which it begins
     if (split ? w.tb == w.te : off > 0) sv_next<KIND>(A, w, tq, split);
-}
-// the same for all lanes of a warp
-template <int KIND>
-__device__ __forceinline__ void sv_next_warp(const AttnArgs& A, SvItem& w, int tq, int split) {
-    __syncwarp();
-    if ((threadIdx.x & 31) == 0) sv_next<KIND>(A, w, tq, split);
-    __syncwarp();
 }
 
 // ---------------------------------------------------------------------------
@@ -366,24 +358,27 @@ __device__ __forceinline__ int sv_page(const AttnArgs& A, const SvSeq& q, int s,
     if (g >= ng) return g == ng && q.kv % SERVE_PAGE ? -2 : -1;
     return __ldg(A.kv.table + (size_t)s * A.kv.width + g);
 }
-__device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq, int split, SvSmem* S,
-                                           unsigned char* Ks, unsigned char* Vs, int tid) {
+__device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigned char* Ks, unsigned char* Vs, int tid) {
     const int lane = tid & 31, warp = tid >> 5;
     const SvConv cv = {A, S, tid};
     uint32_t seg = 0, kt = 0;
     bool ok = true;
     // an index outside the pool: reported once per use, then absent
-    auto valid = [&](int page, int g) -> int {
+    auto valid = [&](const SvItem& w, int page, int g) -> int {
         if (g < w.q.kv / SERVE_PAGE && (page < 0 || page >= A.kv.n_pages)) {
             if (tid == 0) atomicOr(A.err, SERVE_ERR_PAGE);
             return -3;
         }
         return page;
     };
-    for (; ok && w.left > 0; sv_next_warp<SV_MANY>(A, w, tq, split), seg++) {
+    for (; ok; seg++) {
         const int par = seg & 1;
+        if (!(ok = sv_wait(&S->q_full[par], (seg >> 1) & 1, &S->abort_))) break;
+        const SvItem& w = S->item[seg & 3];
+        if (w.n == 0) break;
+        if (lane == 0) mbar_arrive(&S->q_empty[par]);
         // this parity's notes were last read two segments ago
-        if (seg >= 2 && !(ok = sv_wait(&S->epi[par], ((seg >> 1) - 1) & 1, &S->abort_, A.err))) break;
+        if (seg >= 2 && !(ok = sv_wait(&S->epi[par], ((seg >> 1) - 1) & 1, &S->abort_))) break;
         if (warp == 0) {
             for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[par][0][0])[u] = 0x7fffffff;
             if (lane == 0) S->any_bad[par] = 0;
@@ -391,7 +386,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
         __threadfence_block();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S->conv);
-        if (!(ok = sv_wait(&S->conv, seg & 1, &S->abort_, A.err))) break;
+        if (!(ok = sv_wait(&S->conv, seg & 1, &S->abort_))) break;
 
         const size_t tail = ((size_t)w.s * A.nkv + w.h) * SERVE_PAGE_HEAD;
         const int rest = w.q.kv % SERVE_PAGE;
@@ -405,7 +400,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
             return __half2float((tid & 2 ? A.kv.vps : A.kv.kps)[(size_t)page * A.nkv + w.h]);
         };
 #pragma unroll
-        for (int g = 0; g < 2; g++) pg[g] = valid(sv_page(A, w.q, w.s, 2 * w.tb + g), 2 * w.tb + g);
+        for (int g = 0; g < 2; g++) pg[g] = valid(w, sv_page(A, w.q, w.s, 2 * w.tb + g), 2 * w.tb + g);
 #pragma unroll
         for (int g = 0; g < 2; g++) cv.load(A.kv.kp8, pg[g], w.h, kx[g]), cv.load(A.kv.vp8, pg[g], w.h, vx[g]);
         if (tid < 4) sc = scale(pg);
@@ -416,11 +411,11 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
             const bool masked = sv_masked(w.q, w.t0, i);
             int pq[2];  // the next tile's pages, checked
 #pragma unroll
-            for (int g = 0; g < 2; g++) pq[g] = i + 1 < w.te ? valid(pn[g], 2 * (i + 1) + g) : -1;
+            for (int g = 0; g < 2; g++) pq[g] = i + 1 < w.te ? valid(w, pn[g], 2 * (i + 1) + g) : -1;
             if (tid < 4) sn = scale(pq);
 #pragma unroll
             for (int g = 0; g < 2; g++) pn[g] = i + 2 < w.te ? sv_page(A, w.q, w.s, 2 * (i + 2) + g) : -1;
-            if (!(ok = sv_wait(&S->k_empty[st], ph, &S->abort_, A.err))) break;
+            if (!(ok = sv_wait(&S->k_empty[st], ph, &S->abort_))) break;
             unsigned char* kd = Ks + st * SV_TILE_BYTES;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
@@ -436,7 +431,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvItem& w, int tq,
             if (lane == 0) mbar_arrive(&S->k_full[st]);
 #pragma unroll
             for (int g = 0; g < 2; g++) cv.load(A.kv.kp8, pq[g], w.h, kx[g]);
-            if (!(ok = sv_wait(&S->v_empty[st], ph, &S->abort_, A.err))) break;
+            if (!(ok = sv_wait(&S->v_empty[st], ph, &S->abort_))) break;
             unsigned char* vd = Vs + st * SV_TILE_BYTES;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
@@ -480,7 +475,10 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&S->q_full[i], 1), mbar_init(&S->q_empty[i], 2);
+            mbar_init(&S->q_full[i], 1);
+            // the last scores of both row tiles, and every role's warps once they have seen the item (so that no
+            // phase of q_full goes by unseen)
+            mbar_init(&S->q_empty[i], 2 + 8 + (PAGED ? 4 : 1));
             mbar_init(&S->s_full[i], 1), mbar_init(&S->s_free[i], 4), mbar_init(&S->p_full[i], 4);
             mbar_init(&S->o_full[i], 1), mbar_init(&S->o_free[i], 4), mbar_init(&S->epi[i], PAGED ? 12 : 9);
             S->any_bad[i] = 0;
@@ -506,9 +504,6 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
     __syncthreads();
     sv_fence_after();
     const uint32_t tmem = S->tmem;
-    SvItem& w = S->item[warp];
-    if (lane == 0) sv_first<C::KIND>(A, S, w, tq, split);
-    __syncwarp();
 
     if (warp < 8) {
         // ---- softmax and epilogue: one thread per row of row tile t ----
@@ -520,10 +515,14 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         const uint32_t s_addr = lane_base + t * 128, p_addr = lane_base + SV_P_COL + t * 64;
         uint32_t ops = 0, tiles = 0, seg = 0;
         bool ok = true;
-        for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
+        for (; ok; seg++) {
+            if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
+            const SvItem& w = S->item[seg & 3];
+            if (w.n == 0) break;
+            if (lane == 0) mbar_arrive(&S->q_empty[seg & 1]);
             const bool act1 = w.t0 + TOK < w.q.c;
             // all who arrive at a segment's epi barrier have seen the one before of the same parity complete
-            if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_, A.err))) break;
+            if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_))) break;
             if (t == 1 && !act1) {
                 tiles += w.te - w.tb;
                 __syncwarp();
@@ -538,7 +537,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             const int tb = w.tb, te = w.te;
             const int first_masked = (w.q.p0 + w.t0 + t * TOK + 1) >> 7;  // from here some row masks some key
             for (int i = tb; i < te; i++, ops++, tiles++) {
-                if (!(ok = sv_wait(&S->s_full[t], ops & 1, &S->abort_, A.err))) break;
+                if (!(ok = sv_wait(&S->s_full[t], ops & 1, &S->abort_))) break;
                 sv_fence_after();
                 uint32_t sr[128];
                 float* s = reinterpret_cast<float*>(sr);
@@ -590,7 +589,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 const float x = fmaxf(mx[0], mx[1]);
                 // the last product has read P and written O
                 if (i > tb) {
-                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
+                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_))) break;
                     sv_fence_after();
                 }
                 if (i == tb) {
@@ -601,14 +600,14 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     const float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
                     m = mn;
                     l2[0] = f2_mul(l2[0], f2_pack(f, f)), l2[1] = f2_mul(l2[1], f2_pack(f, f));
-#pragma unroll
-                    for (int j = 0; j < 2; j++) {
-                        uint32_t o[32];
-                        sv_ld32(o_addr + 32 * j, o);
+#pragma unroll 1
+                    for (uint32_t j = 0; j < CUINF_HD; j += 16) {
+                        uint32_t o[16];
+                        sv_ld16(o_addr + j, o);
                         sv_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                        sv_st32(o_addr + 32 * j, o);
+                        for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                        sv_st16(o_addr + j, o);
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
@@ -638,55 +637,51 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             }
             if (!ok) break;
             // ---- epilogue of the item (or of the CTA's part of it) ----
-            if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_, A.err))) break;
+            if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_))) break;
             sv_fence_after();
-            uint32_t o[64];
-            sv_ld32(o_addr, o);
-            sv_ld32(o_addr + 32, o + 32);
-            sv_wait_ld();
-            sv_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&S->o_free[t]);
             float la, lb;
             f2_unpack(f2_add(l2[0], l2[1]), la, lb);
             const float l = la + lb;
-            float* of = reinterpret_cast<float*>(o);
             const float vs = PAGED ? 1.f / SV_VEXP : 1.f;
-            if (S->any_bad[seg & 1]) {
-                const int(*bad)[CUINF_HD] = S->bad[seg & 1];
+            const bool whole = w.tb == 0 && w.te == w.n, any_bad = S->any_bad[seg & 1] != 0;
+            const size_t slot = (size_t)blockIdx.x * 2 + (w.tb == 0);
+            const float inv = whole ? (l == 0.f ? 0.f : vs / l) : vs;
+            __half* dst = A.out + ((size_t)(w.q.a + tok) * A.nh + w.h * G + row % G) * CUINF_HD;
+            float* part = W.o + (slot * 256 + t * 128 + row) * CUINF_HD;
+#pragma unroll 1
+            for (int d0 = 0; d0 < CUINF_HD; d0 += 16) {
+                uint32_t o[16];
+                sv_ld16(o_addr + d0, o);
+                sv_wait_ld();
+                float* of = reinterpret_cast<float*>(o);
+                if (any_bad) {
+                    const int(*bad)[CUINF_HD] = S->bad[seg & 1];
 #pragma unroll
-                for (int d = 0; d < 64; d++) {
-                    if (bad[0][d] <= pos) of[d] += INFINITY;
-                    if (bad[1][d] <= pos) of[d] -= INFINITY;
-                    if (bad[2][d] <= pos) of[d] = NAN;
-                }
-            }
-            const bool whole = w.tb == 0 && w.te == w.n;
-            if (whole) {
-                if (live_row) {
-                    const float inv = l == 0.f ? 0.f : vs / l;
-                    uint4* dst = reinterpret_cast<uint4*>(A.out + ((size_t)(w.q.a + tok) * A.nh + w.h * G + row % G) *
-                                                                      CUINF_HD);
-#pragma unroll
-                    for (int d = 0; d < 64; d += 8) {
-                        uint4 r;
-                        r.x = sv_pack_h2(of[d] * inv, of[d + 1] * inv);
-                        r.y = sv_pack_h2(of[d + 2] * inv, of[d + 3] * inv);
-                        r.z = sv_pack_h2(of[d + 4] * inv, of[d + 5] * inv);
-                        r.w = sv_pack_h2(of[d + 6] * inv, of[d + 7] * inv);
-                        dst[d / 8] = r;
+                    for (int d = 0; d < 16; d++) {
+                        if (bad[0][d0 + d] <= pos) of[d] += INFINITY;
+                        if (bad[1][d0 + d] <= pos) of[d] -= INFINITY;
+                        if (bad[2][d0 + d] <= pos) of[d] = NAN;
                     }
                 }
-            } else {
-                const size_t slot = (size_t)blockIdx.x * 2 + (w.tb == 0);
-                if (live_row) {
-                    const size_t r = slot * 256 + t * 128 + row;
-                    reinterpret_cast<float2*>(W.ml)[r] = make_float2(m, l);
-                    float4* dst = reinterpret_cast<float4*>(W.o + r * 64);
+                if (!live_row) continue;
+                if (whole) {
 #pragma unroll
-                    for (int d = 0; d < 64; d += 4)
-                        dst[d / 4] = make_float4(of[d] * vs, of[d + 1] * vs, of[d + 2] * vs, of[d + 3] * vs);
+                    for (int d = 0; d < 16; d += 8)
+                        *reinterpret_cast<uint4*>(dst + d0 + d) =
+                            make_uint4(sv_pack_h2(of[d] * inv, of[d + 1] * inv), sv_pack_h2(of[d + 2] * inv, of[d + 3] * inv),
+                                       sv_pack_h2(of[d + 4] * inv, of[d + 5] * inv), sv_pack_h2(of[d + 6] * inv, of[d + 7] * inv));
+                } else {
+#pragma unroll
+                    for (int d = 0; d < 16; d += 4)
+                        *reinterpret_cast<float4*>(part + d0 + d) =
+                            make_float4(of[d] * inv, of[d + 1] * inv, of[d + 2] * inv, of[d + 3] * inv);
                 }
+            }
+            sv_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&S->o_free[t]);
+            if (!whole) {
+                if (live_row) reinterpret_cast<float2*>(W.ml)[slot * 256 + t * 128 + row] = make_float2(m, l);
                 if (t == 0 && row == 0) {
                     SvPart p;
                     p.valid = 1, p.last = w.te == w.n, p.row0 = w.q.a + w.t0, p.tokens = min(tq, w.q.c - w.t0);
@@ -700,51 +695,52 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(C::REG_LO));
         if (warp == C::Q_WARP) {
-            // ---- Q (and, packed, K and V) by TMA ----
-            uint32_t seg = 0, kt = 0, nq = 0, nk = 0, nv = 0;  // copies issued
-            bool ok = true;
-            for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
-                const uint32_t qsl = seg & 1;
-                bool r = true;
-                if (lane == 0) {
-                    r = sv_wait(&S->q_empty[qsl], ((seg >> 1) & 1) ^ 1, &S->abort_, A.err);
-                    if (r) {
-                        const bool act1 = w.t0 + TOK < w.q.c;
-                        mbar_arrive_expect_tx(&S->q_full[qsl], (uint32_t)(TOK * G * 128) * (act1 ? 2 : 1));
-                        for (int t = 0; t < (act1 ? 2 : 1); t++)
-                            sv_tma_3d(Qs + qsl * SV_Q_BYTES + t * SV_TILE_BYTES, &qmap, 0, w.h * G,
-                                      w.q.a + w.t0 + t * TOK, &S->q_full[qsl]);
-                        nq++;
+            // ---- the walk; Q (and, packed, K and V) by TMA ----
+            if (lane == 0) {
+                SvItem w;
+                uint32_t seg = 0, kt = 0, nq = 0, nk = 0, nv = 0;  // copies issued
+                sv_first<C::KIND>(A, S, w, tq, split);
+                for (;; seg++) {
+                    const uint32_t qsl = seg & 1;
+                    if (!sv_wait(&S->q_empty[qsl], ((seg >> 1) & 1) ^ 1, &S->abort_)) break;
+                    if (w.left <= 0) {
+                        S->item[seg & 3].n = 0;
+                        mbar_arrive(&S->q_full[qsl]);
+                        break;
                     }
-                }
-                if (!(ok = __shfl_sync(0xffffffffu, (int)r, 0) != 0)) break;
-                if (PAGED) continue;
-                for (int i = w.tb; i < w.te; i++, kt++) {
-                    const uint32_t st = kt % SV_KST, ph = ((kt / SV_KST) & 1) ^ 1;
-                    if (lane == 0) {
-                        r = sv_wait(&S->k_empty[st], ph, &S->abort_, A.err);
-                        if (r) {
+                    S->item[seg & 3] = w;
+                    const int nt = w.t0 + TOK < w.q.c ? 2 : 1;
+                    mbar_arrive_expect_tx(&S->q_full[qsl], (uint32_t)(TOK * G * 128) * nt);
+                    for (int t = 0; t < nt; t++)
+                        sv_tma_3d(Qs + qsl * SV_Q_BYTES + t * SV_TILE_BYTES, &qmap, 0, w.h * G, w.q.a + w.t0 + t * TOK,
+                                  &S->q_full[qsl]);
+                    nq = seg + 1;
+                    bool ok = true;
+                    if (!PAGED) {
+                        for (int i = w.tb; i < w.te; i++, kt++) {
+                            const uint32_t st = kt % SV_KST, ph = ((kt / SV_KST) & 1) ^ 1;
+                            if (!(ok = sv_wait(&S->k_empty[st], ph, &S->abort_))) break;
                             mbar_arrive_expect_tx(&S->k_full[st], SV_TILE_BYTES);
                             sv_tma_3d(Ks + st * SV_TILE_BYTES, &kmap, 0, w.h, w.q.a + i * SV_KT, &S->k_full[st]);
                             nk++;
-                            r = sv_wait(&S->v_empty[st], ph, &S->abort_, A.err);
-                        }
-                        if (r) {
+                            if (!(ok = sv_wait(&S->v_empty[st], ph, &S->abort_))) break;
                             mbar_arrive_expect_tx(&S->v_full[st], SV_TILE_BYTES);
                             sv_tma_3d(Vs + st * SV_TILE_BYTES, &vmap, 0, w.h, w.q.a + i * SV_KT, &S->v_full[st]);
                             nv++;
                         }
                     }
-                    if (!(ok = __shfl_sync(0xffffffffu, (int)r, 0) != 0)) break;
+                    if (!ok) break;
+                    sv_next<C::KIND>(A, w, tq, split);
                 }
-            }
-            // what is in flight lands before the CTA can exit
-            if (lane == 0) {
-                for (uint32_t k = nq < 2 ? 0 : nq - 2; k < nq; k++) sv_drain(&S->q_full[k & 1], (k >> 1) & 1, A.err);
-                for (uint32_t k = nk < SV_KST ? 0 : nk - SV_KST; k < nk; k++)
-                    sv_drain(&S->k_full[k % SV_KST], (k / SV_KST) & 1, A.err);
-                for (uint32_t k = nv < SV_KST ? 0 : nv - SV_KST; k < nv; k++)
-                    sv_drain(&S->v_full[k % SV_KST], (k / SV_KST) & 1, A.err);
+                // every copy is waited for by those who use it; after an abort, what is in flight has to land before
+                // the CTA can exit
+                if (*(volatile int*)&S->abort_) {
+                    for (uint32_t k = nq < 2 ? 0 : nq - 2; k < nq; k++) sv_drain(&S->q_full[k & 1], (k >> 1) & 1);
+                    for (uint32_t k = nk < SV_KST ? 0 : nk - SV_KST; k < nk; k++)
+                        sv_drain(&S->k_full[k % SV_KST], (k / SV_KST) & 1);
+                    for (uint32_t k = nv < SV_KST ? 0 : nv - SV_KST; k < nv; k++)
+                        sv_drain(&S->v_full[k % SV_KST], (k / SV_KST) & 1);
+                }
             }
             __syncwarp();
         } else if (warp == C::MMA_WARP || warp == C::MMA_WARP + 1) {
@@ -762,8 +758,8 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             uint32_t n1 = 0;  // (t = 0) products of row tile 1 in key tiles so far
             auto scores = [&](uint32_t qa, bool turns, bool first) -> bool {
                 const uint32_t st = kt % SV_KST;
-                if (!sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_, A.err)) return false;
-                if (nq > 0 && !sv_wait(&S->s_free[t], (nq - 1) & 1, &S->abort_, A.err)) return false;
+                if (!sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_)) return false;
+                if (nq > 0 && !sv_wait(&S->s_free[t], (nq - 1) & 1, &S->abort_)) return false;
                 // The row tiles take turns: one's exponentials run beside the other's loads and maxima.  Only a
                 // matter of pace, so it is not insisted on (and a phase that has gone by unseen costs some tries).
                 if (t == 1) {
@@ -785,15 +781,17 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 nq++, kt++;
                 return true;
             };
-            for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
+            for (; ok; seg++) {
+                if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
+                const SvItem& w = S->item[seg & 3];
+                if (w.n == 0) break;
                 const int nt = w.te - w.tb;
-                if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_, A.err))) break;
                 if (t == 1 && w.t0 + TOK >= w.q.c) {  // the block has one row tile: only let the stages go
                     for (int i = 0; ok && i < nt; i++, kt++, vt++) {
                         const uint32_t st = kt % SV_KST;
-                        if (!(ok = sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_, A.err))) break;
+                        if (!(ok = sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_))) break;
                         if (leader) mbar_arrive(&S->k_empty[st]);
-                        if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err))) break;
+                        if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_))) break;
                         if (leader) mbar_arrive(&S->v_empty[st]);
                     }
                     if (leader) mbar_arrive(&S->q_empty[seg & 1]);
@@ -806,10 +804,10 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     if (i + 1 < nt && !(ok = scores(qa, turns, false))) break;
                     if (leader && i == max(nt - 2, 0)) sv_commit(&S->q_empty[seg & 1]);  // the last scores are under way
                     const uint32_t st = vt % SV_KST;
-                    if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_, A.err))) break;
-                    if (!PAGED && !(ok = sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_, A.err))) break;
-                    if (i == 0 && segs > 0 && !(ok = sv_wait(&S->o_free[t], (segs - 1) & 1, &S->abort_, A.err))) break;
-                    if (!(ok = sv_wait(&S->p_full[t], np & 1, &S->abort_, A.err))) break;
+                    if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_))) break;
+                    if (!PAGED && !(ok = sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_))) break;
+                    if (i == 0 && segs > 0 && !(ok = sv_wait(&S->o_free[t], (segs - 1) & 1, &S->abort_))) break;
+                    if (!(ok = sv_wait(&S->p_full[t], np & 1, &S->abort_))) break;
                     sv_fence_after();
                     if (leader) {
                         const uint32_t va = v_lo + st * (SV_TILE_BYTES >> 4);
@@ -830,16 +828,20 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             // ---- values that are no numbers, in tiles with masked places ----
             uint32_t seg = 0, kt = 0;
             bool ok = true;
-            for (; ok && w.left > 0; sv_next_warp<C::KIND>(A, w, tq, split), seg++) {
+            for (; ok; seg++) {
+                if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
+                const SvItem& w = S->item[seg & 3];
+                if (w.n == 0) break;
+                if (lane == 0) mbar_arrive(&S->q_empty[seg & 1]);
                 // this parity's notes were last read two segments ago
-                if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_, A.err))) break;
+                if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_))) break;
                 for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[seg & 1][0][0])[u] = 0x7fffffff;
                 if (lane == 0) S->any_bad[seg & 1] = 0;
                 __syncwarp();
                 for (int i = w.tb; i < w.te; i++, kt++) {
                     const uint32_t st = kt % SV_KST;
                     // every tile passes here, so that no phase of v_full goes unseen
-                    if (!(ok = sv_wait(&S->v_full[st], (kt / SV_KST) & 1, &S->abort_, A.err))) break;
+                    if (!(ok = sv_wait(&S->v_full[st], (kt / SV_KST) & 1, &S->abort_))) break;
                     if (!sv_masked(w.q, w.t0, i)) {
                         if (lane == 0) mbar_arrive(&S->v_ok[st]);
                         continue;
@@ -874,14 +876,17 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             }
             __syncwarp();
         } else if (PAGED && warp < 12) {
-            if constexpr (PAGED) sv_convert(A, w, tq, split, S, Ks, Vs, tid - 256);
+            if constexpr (PAGED) sv_convert(A, S, Ks, Vs, tid - 256);
         }
     }
     sv_fence_before();
     __syncthreads();
     if (warp == C::MMA_WARP) {
         sv_fence_after();
-        if (lane == 0) sv_drain(&S->done, 0, A.err);
+        if (lane == 0) {
+            sv_drain(&S->done, 0);
+            if (S->abort_) atomicOr(A.err, SERVE_ERR_WAIT);
+        }
         __syncwarp();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(SV_TMEM_COLS)
                      : "memory");
