@@ -155,6 +155,51 @@ struct FwUnit {
     float ks, vs;
     int key0, here;  // first key, keys
 };
+// Values that some row masks become numbers, since 0 * NaN would pass a weight
+// of zero: those that are none are noted by (column, first key) and become
+// zero, keys behind the last are zero.  The stage is the warp's own.
+template <bool TAIL>
+__device__ __forceinline__ void fw_clean(const FwUnit& x, FwSmem* S, int note, int lane) {
+    unsigned char* vd = const_cast<unsigned char*>(x.kd) + FW_UNIT / 2;
+    bool touched = false;
+#pragma unroll 1
+    for (int u = lane; u < FW_UNIT / 2 / 16; u += 32) {
+        uint4* p = reinterpret_cast<uint4*>(vd + 16 * u);
+        const int row = TAIL ? u >> 3 : u >> 2, d0 = TAIL ? 8 * (u & 7) : 16 * (u & 3);
+        if (row >= x.here) {
+            *p = make_uint4(0, 0, 0, 0);
+            touched = true;
+            continue;
+        }
+        uint32_t any = 0;
+        const uint4 v = *p;
+        if (TAIL)  // exponent all ones
+            any = ((v.x & 0x7fff7fffu) + 0x04000400u | (v.y & 0x7fff7fffu) + 0x04000400u | (v.z & 0x7fff7fffu) + 0x04000400u |
+                   (v.w & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;
+        else  // E4M3's NaN: all ones but the sign
+            any = ((v.x & 0x7f7f7f7fu) + 0x01010101u | (v.y & 0x7f7f7f7fu) + 0x01010101u | (v.z & 0x7f7f7f7fu) + 0x01010101u |
+                   (v.w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        if (!any) continue;
+        touched = true;
+#pragma unroll 1
+        for (int e = 0; e < (TAIL ? 8 : 16); e++) {
+            int kind = 2;
+            if (TAIL) {
+                const uint16_t bits = reinterpret_cast<const uint16_t*>(p)[e];
+                if ((bits & 0x7c00) != 0x7c00) continue;
+                kind = bits & 0x3ff ? 2 : bits >> 15;
+                reinterpret_cast<uint16_t*>(p)[e] = 0;
+            } else {
+                if ((reinterpret_cast<const uint8_t*>(p)[e] & 0x7f) != 0x7f) continue;
+                reinterpret_cast<uint8_t*>(p)[e] = 0;
+            }
+            atomicMin(&S->bad[note][kind][d0 + e], x.key0 + row);
+            S->any_bad[note] = 1;
+        }
+    }
+    if (touched) asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");  // before the next copy into the stage
+    __syncwarp();
+}
 // One unit of 64 keys (TAIL: 32, fp16) into the state.  TWO: rows 8 to 15 are
 // in use.  MASKED: some row masks some key, or some keys are not there.
 template <bool TWO, bool MASKED, bool TAIL>
@@ -162,6 +207,7 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
     constexpr int NT = TAIL ? FW_TAIL / 8 : 8;  // score tiles of 8 keys
     const int g = lane >> 2, c = lane & 3;
     const unsigned char *kd = x.kd, *vd = x.kd + FW_UNIT / 2;
+    if (MASKED) fw_clean<TAIL>(x, S, note, lane);
     float s[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
@@ -258,23 +304,6 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
                 b[z][2] = sv_e4m3x2(w1), b[z][3] = sv_e4m3x2(w1 >> 16);
                 b[z][4] = sv_e4m3x2(w2), b[z][5] = sv_e4m3x2(w2 >> 16);
                 b[z][6] = sv_e4m3x2(w3), b[z][7] = sv_e4m3x2(w3 >> 16);
-            }
-            if (MASKED) {  // what some row masks is a number: 0 * NaN would pass a weight of zero
-#pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    const bool gone = key + e >= x.here;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const uint32_t bits = b[z][i] >> (16 * e) & 0xffffu;
-                        const bool bad = (bits & 0x7c00u) == 0x7c00u;
-                        if (bad && !gone) {
-                            atomicMin(&S->bad[note][bits & 0x3ffu ? 2 : bits & 0x8000u ? 1 : 0][8 * g + i],
-                                      x.key0 + key + e);
-                            S->any_bad[note] = 1;
-                        }
-                        if (bad || gone) b[z][i] &= e ? 0x0000ffffu : 0xffff0000u;
-                    }
-                }
             }
         }
 #pragma unroll

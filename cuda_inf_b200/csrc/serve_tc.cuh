@@ -283,26 +283,22 @@ __device__ __forceinline__ bool sv_masked(const SvSeq& q, int t0, int tile) {
 }
 
 // ---- paged: pages widened to fp16 tiles by four warps ----
-template <int N>
-__device__ __forceinline__ bool sv_not_finite(const uint32_t (&h)[N]) {  // 0 * x is NaN for what is no number
-    uint32_t x = 0;
-#pragma unroll
-    for (int i = 0; i < N; i++) x = hfma2_u(h[i], 0, x);
+// Value `half` of key `key`, column d, of an item (notes `par`): if it is no number it is noted and becomes zero.
+__device__ __forceinline__ void sv_note(SvSmem* S, int par, __half* p, int key, int d) {
+    const float f = __half2float(*p);
+    if (isfinite(f)) return;
+    *p = __float2half_rn(0.f);
+    atomicMin(&S->bad[par][isnan(f) ? 2 : f > 0.f ? 0 : 1][d], key);
+    S->any_bad[par] = 1;
+}
+// place of column d of row r in a 128-byte-swizzled tile of 64-value rows
+__device__ __forceinline__ __half* sv_at(unsigned char* tile, int r, int d) {
+    return reinterpret_cast<__half*>(tile + r * 128 + (((d >> 3) ^ (r & 7)) << 4)) + (d & 7);
+}
+__device__ __forceinline__ uint32_t sv_sticky(uint32_t x, uint32_t h) { return hfma2_u(h, 0, x); }  // 0 * x is NaN
+__device__ __forceinline__ bool sv_stuck(uint32_t x) {                                                // or 0
     const __half2 y = *reinterpret_cast<const __half2*>(&x);
     return __hisnan(y.x) || __hisnan(y.y);
-}
-// Values that are no numbers, of key `key`, columns d0..: noted and set to zero (rare).
-template <int N>
-__device__ __forceinline__ void sv_note_bad(SvSmem* S, int par, int key, int d0, uint32_t (&h)[N]) {
-#pragma unroll
-    for (int i = 0; i < 2 * N; i++) {
-        const uint32_t bits = h[i >> 1] >> (16 * (i & 1)) & 0xffffu;
-        if ((bits & 0x7c00u) == 0x7c00u) {
-            atomicMin(&S->bad[par][(bits & 0x3ffu) ? 2 : bits & 0x8000u ? 1 : 0][d0 + i], key);
-            S->any_bad[par] = 1;
-            h[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
-        }
-    }
 }
 struct SvConv {
     const AttnArgs& A;
@@ -318,8 +314,9 @@ struct SvConv {
         x[0] = __ldg(src);
         x[1] = __ldg(src + 128);
     }
-    template <bool CHECK>
-    __device__ __forceinline__ void store(unsigned char* dst, int g, const uint4* x, int par, int key0) const {
+    // widens group g of the tile; returns whether some value is no number
+    __device__ __forceinline__ bool store(unsigned char* dst, int g, const uint4* x) const {
+        uint32_t bad = 0;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int u = tid + 128 * i, r = 64 * g + (u >> 2), c = 2 * (u & 3);
@@ -327,28 +324,35 @@ struct SvConv {
             uint32_t h[8];
 #pragma unroll
             for (int j = 0; j < 4; j++) h[2 * j] = sv_e4m3x2(w[j]), h[2 * j + 1] = sv_e4m3x2(w[j] >> 16);
-            if (CHECK && sv_not_finite(h)) sv_note_bad(S, par, key0 + r, 8 * c, h);
+#pragma unroll
+            for (int j = 0; j < 8; j++) bad = sv_sticky(bad, h[j]);
             unsigned char* row = dst + r * 128;
             *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
+        return sv_stuck(bad);
     }
-    // the fp16 tail (rows behind `rest` are zero)
-    template <bool CHECK>
-    __device__ __forceinline__ void tail(unsigned char* dst, int g, const __half* src, int rest, int par, int key0) const {
-#pragma unroll
+    // the fp16 tail (rows behind `rest` are zero): chunk u = tid + 128 i of 512, row u / 8, 8 values
+    __device__ __forceinline__ bool tail(unsigned char* dst, int g, const __half* src, int rest) const {
+        uint32_t bad = 0;
+#pragma unroll 1
         for (int i = 0; i < 4; i++) {
             const int u = tid + 128 * i, r = u >> 3, c = u & 7, rr = 64 * g + r;
             uint4 x = make_uint4(0, 0, 0, 0);
             if (r < rest) x = *reinterpret_cast<const uint4*>(src + r * CUINF_HD + c * 8);
-            if (CHECK) {
-                uint32_t h[4] = {x.x, x.y, x.z, x.w};
-                if (sv_not_finite(h)) {
-                    sv_note_bad(S, par, key0 + rr, 8 * c, h);
-                    x = make_uint4(h[0], h[1], h[2], h[3]);
-                }
-            }
+            bad = sv_sticky(sv_sticky(sv_sticky(sv_sticky(bad, x.x), x.y), x.z), x.w);
             *reinterpret_cast<uint4*>(dst + rr * 128 + ((c ^ (rr & 7)) << 4)) = x;
+        }
+        return sv_stuck(bad);
+    }
+    // this thread's 32 values of group g once more, one by one (rare)
+    __device__ __forceinline__ void note(unsigned char* dst, int g, bool is_tail, int par, int key0) const {
+#pragma unroll 1
+        for (int k = 0; k < 32; k++) {
+            const int u = tid + 128 * (is_tail ? k >> 3 : k >> 4);
+            const int r = 64 * g + (is_tail ? u >> 3 : u >> 2);
+            const int d = is_tail ? 8 * (u & 7) + (k & 7) : 16 * (u & 3) + (k & 15);
+            sv_note(S, par, sv_at(dst, r, d), key0 + r, d);
         }
     }
 };
@@ -420,9 +424,9 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigne
 #pragma unroll
             for (int g = 0; g < 2; g++) {
                 if (pg[g] == -2)
-                    cv.tail<false>(kd, g, A.kv.ktail + tail, rest, 0, 0);
+                    cv.tail(kd, g, A.kv.ktail + tail, rest);
                 else
-                    cv.store<false>(kd, g, kx[g], 0, 0);
+                    cv.store(kd, g, kx[g]);
             }
             if (tid < 4) S->sc[kt % SV_SC][tid] = sc;
             sc = sn;
@@ -435,16 +439,8 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigne
             unsigned char* vd = Vs + st * SV_TILE_BYTES;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-                if (masked) {
-                    if (pg[g] == -2)
-                        cv.tail<true>(vd, g, A.kv.vtail + tail, rest, par, i * SV_KT);
-                    else
-                        cv.store<true>(vd, g, vx[g], par, i * SV_KT);
-                } else if (pg[g] == -2) {
-                    cv.tail<false>(vd, g, A.kv.vtail + tail, rest, 0, 0);
-                } else {
-                    cv.store<false>(vd, g, vx[g], 0, 0);
-                }
+                const bool bad = pg[g] == -2 ? cv.tail(vd, g, A.kv.vtail + tail, rest) : cv.store(vd, g, vx[g]);
+                if (masked && bad) cv.note(vd, g, pg[g] == -2, par, i * SV_KT);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __threadfence_block();
@@ -847,24 +843,16 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                         continue;
                     }
                     unsigned char* V = Vs + st * SV_TILE_BYTES;
-                    uint32_t nan = 0;  // sticky: 0 * x is NaN for what is no number
+                    uint32_t nan = 0;
 #pragma unroll 8
                     for (int u = lane; u < SV_TILE_BYTES / 16; u += 32) {
                         const uint4 v = *reinterpret_cast<const uint4*>(V + u * 16);
-                        nan = hfma2_u(v.x, 0, nan), nan = hfma2_u(v.y, 0, nan);
-                        nan = hfma2_u(v.z, 0, nan), nan = hfma2_u(v.w, 0, nan);
+                        nan = sv_sticky(sv_sticky(sv_sticky(sv_sticky(nan, v.x), v.y), v.z), v.w);
                     }
-                    const __half2 nh = *reinterpret_cast<const __half2*>(&nan);
-                    if (__any_sync(0xffffffffu, __hisnan(nh.x) || __hisnan(nh.y))) {
-                        if (lane == 0) S->any_bad[seg & 1] = 1;
-                        for (int u = lane; u < SV_KT * CUINF_HD; u += 32) {
-                            const int r = u >> 6, d = u & 63;
-                            __half* p = reinterpret_cast<__half*>(V + r * 128 + (((d >> 3) ^ (r & 7)) << 4)) + (d & 7);
-                            const float f = __half2float(*p);
-                            if (isfinite(f)) continue;
-                            *p = __float2half_rn(0.f);
-                            atomicMin(&S->bad[seg & 1][isnan(f) ? 2 : f > 0.f ? 0 : 1][d], i * SV_KT + r);
-                        }
+                    if (__any_sync(0xffffffffu, sv_stuck(nan))) {
+#pragma unroll 1
+                        for (int u = lane; u < SV_KT * CUINF_HD; u += 32)
+                            sv_note(S, seg & 1, sv_at(V, u >> 6, u & 63), i * SV_KT + (u >> 6), u & 63);
                         asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
                     }
                     __threadfence_block();
