@@ -36,14 +36,18 @@ extern "C" int cuinf_paged_error(unsigned* flags) {
 // append: new rows of packed sequences into pages and tails
 //
 // A sequence with `ctx` cached tokens and L new ones touches the 64-token
-// groups ctx/64 .. (ctx+L-1)/64.  One CTA takes one (group, kv head), keys and
-// values; a group that the call completes is read once (its first rows from
-// the old tail, the rest from the new rows), its maximum reduced over the CTA
-// and its bytes written once: 16 values of one row per thread, so a head's
-// page block is one run of 256 16-byte stores.  The rows of the unfinished
-// last group go to the tail; that copy is made by the CTA of the sequence's
-// first group, after it has read the old tail, so that no other CTA reads what
-// it overwrites.
+// groups ctx/64 .. (ctx+L-1)/64.  One warp takes one (group, kv head) of the
+// keys or of the values: 8 KB, all asked for at once into the warp's own part
+// of shared memory, so a CTA's 8 warps need no barrier, an SM has 192 KB in
+// flight, and the loops over it stay small (held in registers the rows made
+// 28 KB of straight code, which a CTA's one pass spent its time fetching).  The
+// maximum is reduced over the warp and the codes written once, a head's page
+// block being one run of 4096 bytes.  Bound by HBM: 256 bytes in and 128 out
+// per token and head.
+//
+// The rows of the unfinished last group go to the tail.  The warp of the
+// sequence's first group copies them, after it has read the old tail, so nobody
+// reads what it overwrites.
 //
 // CTA -> (sequence, group) without a plan: sequence s owns the slots from
 // (cu[s] + 62 s) / 64 + s on, which are at least the groups L new rows can
@@ -59,13 +63,15 @@ struct AppendArgs {
 };
 __host__ __device__ __forceinline__ long long append_slot(long long row, int s) { return (row + 62ll * s) / 64 + s; }
 
-__device__ __forceinline__ uint8_t serve_e4m3(float x) {
-    return (uint8_t)__nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint32_t serve_e4m3x2(float lo, float hi) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;\n" : "=h"(r) : "f"(hi), "f"(lo));
+    return r;
 }
-
-__global__ void __launch_bounds__(256) k_paged_append(const AppendArgs A) {
-    __shared__ float red[2][8];
-    const int h = blockIdx.y, tid = threadIdx.x;
+#define APPEND_SMEM (8 * SERVE_PAGE_HEAD * 2)
+__global__ void __launch_bounds__(256, 3) k_paged_append(const AppendArgs A) {
+    extern __shared__ __align__(16) unsigned char append_raw[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int s = -1;
     for (int b = 0; b < A.rows.n_seqs; b += 256) {
         const int i = b + tid;
@@ -81,74 +87,85 @@ __global__ void __launch_bounds__(256) k_paged_append(const AppendArgs A) {
         if (tid == 0) atomicOr(A.err, SERVE_ERR_RANGE);
         return;
     }
-    const int L = b - a, total = ctx + L, g0 = ctx / SERVE_PAGE;
+    const int L = b - a, total = ctx + L, g0 = ctx / SERVE_PAGE, nkv = A.kv.nkv;
     const long long gl = (long long)blockIdx.x - append_slot(a, s);
-    if (L == 0 || gl > (total - 1) / SERVE_PAGE - g0) return;
-    const int g = g0 + (int)gl, nkv = A.kv.nkv;
-    const int r = tid >> 2, c = (tid & 3) * 16;  // this thread: 16 values of row r
-    const int pos = g * SERVE_PAGE + r;
-    const size_t tail = ((size_t)s * nkv + h) * SERVE_PAGE_HEAD;
-    const bool whole = g < total / SERVE_PAGE;
-
-    uint4 x[2][2];
-    if (whole) {
-        const __half *ks, *vs;
-        if (pos < ctx) {
-            ks = A.kv.ktail + tail + r * CUINF_HD + c;
-            vs = A.kv.vtail + tail + r * CUINF_HD + c;
-        } else {
-            const size_t row = (size_t)a + (pos - ctx);
-            ks = A.k + row * A.k_stride + h * CUINF_HD + c;
-            vs = A.v + row * A.v_stride + h * CUINF_HD + c;
-        }
-        x[0][0] = *reinterpret_cast<const uint4*>(ks);
-        x[0][1] = *reinterpret_cast<const uint4*>(ks + 8);
-        x[1][0] = *reinterpret_cast<const uint4*>(vs);
-        x[1][1] = *reinterpret_cast<const uint4*>(vs + 8);
-        float mx[2];
-#pragma unroll
-        for (int p = 0; p < 2; p++) {
-            const __half* e = reinterpret_cast<const __half*>(x[p]);
-            mx[p] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; i++) mx[p] = fmaxf(mx[p], fabsf(__half2float(e[i])));
-            mx[p] = warp_max(mx[p]);
-            if ((tid & 31) == 0) red[p][tid >> 5] = mx[p];
-        }
-        __syncthreads();  // also: the old tail has been read before it is overwritten below
+    const int h = blockIdx.y * 4 + (warp >> 1);
+    if (L == 0 || gl > (total - 1) / SERVE_PAGE - g0 || h >= nkv) return;
+    const bool val = warp & 1;  // keys or values
+    const int g = g0 + (int)gl, r0 = lane >> 3, c = (lane & 7) * 8;  // this lane: 8 values of rows r0 + 4 i
+    __half* tail = (val ? A.kv.vtail : A.kv.ktail) + ((size_t)s * nkv + h) * SERVE_PAGE_HEAD + c;
+    const long long stride = val ? A.v_stride : A.k_stride;
+    const __half* src = (val ? A.v : A.k) + (size_t)a * stride + h * CUINF_HD + c;  // token ctx
+    if (g < total / SERVE_PAGE) {
         const int page = g < A.kv.width ? A.kv.table[(size_t)s * A.kv.width + g] : -1;
+        // a lane reads back what it has copied itself
+        uint4* mine = reinterpret_cast<uint4*>(append_raw + warp * SERVE_PAGE_HEAD * 2) + lane;
+#pragma unroll 4
+        for (int i = 0; i < 16; i++) {
+            const int r = r0 + 4 * i, pos = g * SERVE_PAGE + r;
+            const __half* from = pos < ctx ? tail + r * CUINF_HD : src + (long long)(pos - ctx) * stride;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(mine + 32 * i)), "l"(from) : "memory");
+        }
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+        __half2 mx = __float2half2_rn(0.f);  // (a maximum passes NaN by)
+#pragma unroll 4
+        for (int i = 0; i < 16; i++) {
+            const uint4 x = mine[32 * i];
+            const __half2* e = reinterpret_cast<const __half2*>(&x);
+#pragma unroll
+            for (int j = 0; j < 4; j++) mx = __hmax2(mx, __habs2(e[j]));
+        }
+        const float amax = warp_max(fmaxf(__low2float(mx), __high2float(mx)));
+        // kv_commit_group's rule: fp32 scale for the codes, fp16 in the cache
+        const float sc = amax / 448.0f + 1e-12f;
+        // x / sc rounded to nearest (the codes have to be those of the division) by two products with the rounded
+        // reciprocal: q = x y, q + (x - q sc) y (Markstein, IBM J. Res. Dev. 34, 1990; no step of it underflows for
+        // fp16 x).  A row that is infinite makes every quotient 0 or NaN.
+        const bool finite = sc < INFINITY;
+        const float y = 1.f / sc, y2 = finite ? y : 0.f, nsc = finite ? -sc : 0.f;
         if (page >= 0 && page < A.kv.n_pages) {
+            const size_t blk = (size_t)page * nkv + h;
+            uint8_t* dst = (val ? A.kv.vp8 : A.kv.kp8) + blk * SERVE_PAGE_HEAD + c;
+#pragma unroll 2
+            for (int i = 0; i < 16; i++) {
+                const uint4 x = mine[32 * i];
+                const __half2* e = reinterpret_cast<const __half2*>(&x);
+                float q[8];
 #pragma unroll
-            for (int p = 0; p < 2; p++) {
-                float amax = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) amax = fmaxf(amax, red[p][i]);
-                // kv_commit_group's rule: fp32 scale for the codes, fp16 in the cache
-                const float sc = amax / 448.0f + 1e-12f;
-                const __half* e = reinterpret_cast<const __half*>(x[p]);
-                uint8_t q[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) q[i] = serve_e4m3(__half2float(e[i]) / sc);
-                const size_t blk = (size_t)page * nkv + h;
-                *reinterpret_cast<uint4*>((p ? A.kv.vp8 : A.kv.kp8) + blk * SERVE_PAGE_HEAD + r * CUINF_HD + c) =
-                    *reinterpret_cast<const uint4*>(q);
-                if (tid == 0) (p ? A.kv.vps : A.kv.kps)[blk] = __float2half_rn(sc);
+                for (int j = 0; j < 4; j++) {
+                    const float2 f = __half22float2(e[j]);
+                    q[2 * j] = f.x * y, q[2 * j + 1] = f.y * y;
+                    q[2 * j] = fmaf(fmaf(q[2 * j], nsc, f.x), y2, q[2 * j]);
+                    q[2 * j + 1] = fmaf(fmaf(q[2 * j + 1], nsc, f.y), y2, q[2 * j + 1]);
+                }
+                *reinterpret_cast<uint2*>(dst + (r0 + 4 * i) * CUINF_HD) =
+                    make_uint2(serve_e4m3x2(q[0], q[1]) | serve_e4m3x2(q[2], q[3]) << 16,
+                               serve_e4m3x2(q[4], q[5]) | serve_e4m3x2(q[6], q[7]) << 16);
             }
-        } else if (tid == 0) {
+            if (lane == 0) (val ? A.kv.vps : A.kv.kps)[blk] = __float2half_rn(sc);
+        } else if (lane == 0) {
             atomicOr(A.err, SERVE_ERR_PAGE);
         }
     }
     if (g != g0) return;
-    const int last = total / SERVE_PAGE;  // the unfinished group: its new rows go to the tail
-    const int tp = last * SERVE_PAGE + r;
-    if (tp < total && tp >= ctx) {
-        const size_t row = (size_t)a + (tp - ctx);
-        const uint4* ks = reinterpret_cast<const uint4*>(A.k + row * A.k_stride + h * CUINF_HD + c);
-        const uint4* vs = reinterpret_cast<const uint4*>(A.v + row * A.v_stride + h * CUINF_HD + c);
-        uint4* kd = reinterpret_cast<uint4*>(A.kv.ktail + tail + r * CUINF_HD + c);
-        uint4* vd = reinterpret_cast<uint4*>(A.kv.vtail + tail + r * CUINF_HD + c);
-        const uint4 k0 = ks[0], k1 = ks[1], v0 = vs[0], v1 = vs[1];
-        kd[0] = k0, kd[1] = k1, vd[0] = v0, vd[1] = v1;
+    __syncwarp();  // the old tail has been read
+    // the unfinished group: its new rows go to the tail, asked for at once too
+    const int last = total / SERVE_PAGE * SERVE_PAGE;
+    if (last == total) return;
+    uint4* mine = reinterpret_cast<uint4*>(append_raw + warp * SERVE_PAGE_HEAD * 2) + lane;
+#pragma unroll 4
+    for (int i = 0; i < 16; i++) {
+        const int pos = last + r0 + 4 * i;
+        if (pos < total && pos >= ctx)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(smem_u32(mine + 32 * i)),
+                         "l"(src + (long long)(pos - ctx) * stride)
+                         : "memory");
+    }
+    asm volatile("cp.async.wait_all;\n" ::: "memory");
+#pragma unroll 4
+    for (int i = 0; i < 16; i++) {
+        const int pos = last + r0 + 4 * i;
+        if (pos < total && pos >= ctx) *reinterpret_cast<uint4*>(tail + (r0 + 4 * i) * CUINF_HD) = mine[32 * i];
     }
 }
 
@@ -199,7 +216,8 @@ extern "C" int cuinf_kv_paged_append(const void* k, int64_t k_stride, const void
     if (int rc = serve_err_ptr(&A.err)) return rc;
     const long long slots = append_slot(n_rows, n_seqs);
     REQUIRE(slots < (1ll << 31), "too many rows");
-    k_paged_append<<<dim3((unsigned)slots, nkv), 256, 0, ST(stream)>>>(A);
+    CUINF_TRY(cudaFuncSetAttribute(k_paged_append, cudaFuncAttributeMaxDynamicSharedMemorySize, APPEND_SMEM));
+    k_paged_append<<<dim3((unsigned)slots, (nkv + 3) / 4), 256, APPEND_SMEM, ST(stream)>>>(A);
     return cuinf_launch_status();
 }
 

@@ -288,6 +288,21 @@ def test_append_zero_and_extreme_rows(cuda):
     assert torch.equal(c.kp8[page], c.vp8[page])
 
 
+def test_append_infinities_and_nan_as_the_commit(cuda):
+    """Pages with an infinite value, a NaN, both: codes and scales of kv_commit_group, bit for bit."""
+    c = Cache(1, 4, 64, cuda)
+    k = rnd((64, 4, 64), 3, cuda)
+    k[5, 0, 7], k[6, 1, 8], k[7, 2, 9], k[8, 2, 3] = INF, NAN, -INF, NAN
+    c.append(k, k.flip(1).contiguous(), [64])
+    k8, v8 = (torch.empty((64, 4, 64), dtype=torch.uint8, device=cuda) for _ in range(2))
+    ks, vs = (torch.empty((1, 4), dtype=torch.float16, device=cuda) for _ in range(2))
+    ops.kv_commit_group(k, k.flip(1).contiguous(), k8, v8, ks, vs, 0, 0)
+    page = int(c.table[0, 0])
+    assert torch.equal(c.kp8[page], k8.transpose(0, 1)) and torch.equal(c.vp8[page], v8.transpose(0, 1))
+    assert torch.equal(c.kps[page].view(torch.int16), ks[0].view(torch.int16))
+    assert torch.equal(c.vps[page].view(torch.int16), vs[0].view(torch.int16))
+
+
 def test_append_bad_page_and_lengths_are_reported(cuda):
     c = Cache(3, 2, 128, cuda)
     fill(c, [60, 60, 60], 5)
