@@ -409,7 +409,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
 
                 for (int u = j + (warp + FW_WARPS - j % FW_WARPS) % FW_WARPS; u < j + te - tb; u += FW_WARPS) {
                     const int st = u % FW_ST, unit = tb + u - j;
-                    if (!(ok = sv_wait(&S->full[st], (u / FW_ST) & 1, &S->abort_))) break;
+                    if (!(ok = sv_wait_all(&S->full[st], (u / FW_ST) & 1, &S->abort_))) break;
                     FwUnit x;
                     x.kd = ring + (size_t)st * FW_UNIT;
                     x.ks = S->sc[st][0], x.vs = S->sc[st][1];
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                 }
                 // ---- the item's end: join the warps ----
                 // what the last item left there has been read
-                if (!ok || (item > 0 && !(ok = sv_wait(&S->merged, (item - 1) & 1, &S->abort_)))) break;
+                if (!ok || (item > 0 && !(ok = sv_wait_all(&S->merged, (item - 1) & 1, &S->abort_)))) break;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     R.l[r] += __shfl_xor_sync(0xffffffffu, R.l[r], 1);
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                 __threadfence_block();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S->merge);
-                if (!(ok = sv_wait(&S->merge, item & 1, &S->abort_))) break;
+                if (!(ok = sv_wait_all(&S->merge, item & 1, &S->abort_))) break;
                 const bool whole = tb == 0 && te == p.n;
                 const size_t slot = (size_t)blockIdx.x * 2 + (tb == 0);
                 for (int i = tid; i < rows * 16; i += FW_WARPS * 32) {

@@ -21,6 +21,11 @@ __device__ __forceinline__ bool sv_wait(uint64_t* bar, uint32_t parity, int* abo
     *(volatile int*)abort_ = 1;
     return false;
 }
+// The same by all lanes of a warp, with one answer (lanes that part after an
+// abort would wait for each other in the warp's next vote or TMEM access).
+__device__ __forceinline__ bool sv_wait_all(uint64_t* bar, uint32_t parity, int* abort_) {
+    return __all_sync(0xffffffffu, sv_wait(bar, parity, abort_));
+}
 // Before the CTA ends: a phase that copies or products in flight complete.
 __device__ __forceinline__ void sv_drain(uint64_t* bar, uint32_t parity) {
 #pragma unroll 1

@@ -34,7 +34,8 @@
 #include "serve_line.cuh"
 
 #define SV_KT 128        // keys per tile
-#define SV_KST 4         // K and V stages
+#define SV_FST 4         // paged: stages of FP8 tiles (two pages' keys and values)
+#define SV_F_BYTES (4 * SERVE_PAGE_HEAD)
 #define SV_SC 16         // slots of the pages' scales (more tiles than can be in flight)
 #define SV_TILE_BYTES (SV_KT * CUINF_HD * 2)
 #define SV_TMEM_COLS 512
@@ -52,11 +53,12 @@ struct SvItem {
 };
 
 struct SvSmem {
-    uint64_t q_full[2], q_empty[2], k_full[SV_KST], k_empty[SV_KST], v_full[SV_KST], v_empty[SV_KST], v_ok[SV_KST];
+    uint64_t q_full[2], q_empty[2], k_full[4], k_empty[4], v_full[4], v_empty[4], v_ok[4], f_full[SV_FST], f_empty[SV_FST];
     uint64_t s_full[2], s_free[2], p_full[2], o_full[2], o_free[2], epi[2], conv, done;
     uint32_t tmem;
     int abort_;
     float sc[SV_SC][4];  // FP8: K scale of the tile's two pages (negative: absent), V scales
+    int kind[SV_FST][2];  // FP8: what the tile's two groups are (SV_PAGE ...)
     int bad[2][3][CUINF_HD];  // by segment parity: first key whose value is +inf, -inf, NaN
     int any_bad[2];
     SvShare share;
@@ -65,7 +67,10 @@ struct SvSmem {
     SvItem item[4];  // of segment seg, modulo 4 (published by q_full; n = 0: no more)
 };
 static constexpr size_t SV_Q_BYTES = 2 * SV_TILE_BYTES;  // both row tiles of an item
-static constexpr size_t SV_SMEM_BYTES = 1024 + 2 * SV_Q_BYTES + 2 * SV_KST * (size_t)SV_TILE_BYTES + sizeof(SvSmem);
+enum { SV_PAGE = 0, SV_TAIL = 1, SV_NONE = 2 };  // a page, the fp16 tail, no keys
+// (packed: 4 stages of K and V; paged: 2 of each, and 4 of FP8 tiles, which are asked for ahead)
+static constexpr size_t SV_SMEM_BYTES = 1024 + 2 * SV_Q_BYTES + 8 * (size_t)SV_TILE_BYTES + sizeof(SvSmem);
+static_assert(SV_FST * SV_F_BYTES == 4 * SV_TILE_BYTES, "the same shared memory for both kernels");
 
 // ---- packed fp32 pairs ----
 __device__ __forceinline__ uint64_t f2_pack(float a, float b) {
@@ -263,6 +268,11 @@ __device__ __forceinline__ void sv_first(const AttnArgs& A, const SvSmem* S, SvI
 // ---------------------------------------------------------------------------
 // roles
 // ---------------------------------------------------------------------------
+// Does some row of the block mask some key of the tile?
+__device__ __forceinline__ bool sv_masked(const SvSeq& q, int t0, int tile) {
+    return (tile + 1) * SV_KT > q.p0 + t0 + 1;
+}
+
 template <bool PAGED>
 struct SvCfg {
     // softmax warps 0-7; packed: 8 TMA, 9 and 10 MMA, 11 value check;
@@ -271,16 +281,12 @@ struct SvCfg {
     static constexpr int WARPS = PAGED ? 16 : 12;
     static constexpr int MMA_WARP = PAGED ? 13 : 9;
     static constexpr int Q_WARP = PAGED ? 12 : 8;
-    // registers: 512 x 128 = 256 x 184 + 256 x 72; 384 x 168 = 256 x 208 + 128 x 88
-    static constexpr int REG_HI = PAGED ? 184 : 208;
-    static constexpr int REG_LO = PAGED ? 72 : 88;
+    static constexpr int KST = PAGED ? 2 : 4;  // K and V stages
+    // registers: 512 x 128 = 256 x 200 + 256 x 56; 384 x 168 = 256 x 208 + 128 x 88
+    static constexpr int REG_HI = PAGED ? 200 : 208;
+    static constexpr int REG_LO = PAGED ? 56 : 88;
     static constexpr float THR = PAGED ? 3.f : 8.f;
 };
-
-// Does some row of the block mask some key of the tile?
-__device__ __forceinline__ bool sv_masked(const SvSeq& q, int t0, int tile) {
-    return (tile + 1) * SV_KT > q.p0 + t0 + 1;
-}
 
 // ---- paged: pages widened to fp16 tiles by four warps ----
 // Value `half` of key `key`, column d, of an item (notes `par`): if it is no number it is noted and becomes zero.
@@ -301,88 +307,69 @@ __device__ __forceinline__ bool sv_stuck(uint32_t x) {                          
     return __hisnan(y.x) || __hisnan(y.y);
 }
 struct SvConv {
-    const AttnArgs& A;
     SvSmem* S;
     int tid;
-    // chunk u = tid + 128 i of a group's 256: row u / 4, 16 values from 16 (u % 4)
-    __device__ __forceinline__ void load(const uint8_t* pool, int page, int h, uint4* x) const {
-        if (page < 0) {
-            x[0] = x[1] = make_uint4(0, 0, 0, 0);
-            return;
-        }
-        const uint4* src = reinterpret_cast<const uint4*>(pool + ((size_t)page * A.nkv + h) * SERVE_PAGE_HEAD) + tid;
-        x[0] = __ldg(src);
-        x[1] = __ldg(src + 128);
-    }
-    // widens group g of the tile; returns whether some value is no number
-    __device__ __forceinline__ bool store(unsigned char* dst, int g, const uint4* x) const {
-        uint32_t bad = 0;
+    // Widens a page's block (chunk u = tid + 128 i of its 256: row u / 4, 16 values from 16 (u % 4)) to rows 64 g..
+    // of the tile.
+    __device__ __forceinline__ void page(unsigned char* dst, int g, const unsigned char* src) const {
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int u = tid + 128 * i, r = 64 * g + (u >> 2), c = 2 * (u & 3);
-            const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-            uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 4; j++) h[2 * j] = sv_e4m3x2(w[j]), h[2 * j + 1] = sv_e4m3x2(w[j] >> 16);
-#pragma unroll
-            for (int j = 0; j < 8; j++) bad = sv_sticky(bad, h[j]);
+            const uint4 x = *reinterpret_cast<const uint4*>(src + 16 * u);
             unsigned char* row = dst + r * 128;
-            *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+            *reinterpret_cast<uint4*>(row + ((c ^ (r & 7)) << 4)) =
+                make_uint4(sv_e4m3x2(x.x), sv_e4m3x2(x.x >> 16), sv_e4m3x2(x.y), sv_e4m3x2(x.y >> 16));
+            *reinterpret_cast<uint4*>(row + (((c + 1) ^ (r & 7)) << 4)) =
+                make_uint4(sv_e4m3x2(x.z), sv_e4m3x2(x.z >> 16), sv_e4m3x2(x.w), sv_e4m3x2(x.w >> 16));
         }
-        return sv_stuck(bad);
     }
-    // the fp16 tail (rows behind `rest` are zero): chunk u = tid + 128 i of 512, row u / 8, 8 values
-    __device__ __forceinline__ bool tail(unsigned char* dst, int g, const __half* src, int rest) const {
-        uint32_t bad = 0;
-#pragma unroll 1
+    // The fp16 tail's first `rest` rows (chunk u = tid + 128 i of 512: row u / 8, 8 values), zeros behind them.
+    __device__ __forceinline__ void tail(unsigned char* dst, int g, const __half* src, int rest) const {
+#pragma unroll
         for (int i = 0; i < 4; i++) {
             const int u = tid + 128 * i, r = u >> 3, c = u & 7, rr = 64 * g + r;
             uint4 x = make_uint4(0, 0, 0, 0);
             if (r < rest) x = *reinterpret_cast<const uint4*>(src + r * CUINF_HD + c * 8);
-            bad = sv_sticky(sv_sticky(sv_sticky(sv_sticky(bad, x.x), x.y), x.z), x.w);
             *reinterpret_cast<uint4*>(dst + rr * 128 + ((c ^ (rr & 7)) << 4)) = x;
         }
-        return sv_stuck(bad);
     }
-    // this thread's 32 values of group g once more, one by one (rare)
-    __device__ __forceinline__ void note(unsigned char* dst, int g, bool is_tail, int par, int key0) const {
+    __device__ __forceinline__ void group(unsigned char* dst, int g, int kind, const unsigned char* src, const __half* tl,
+                                          int rest) const {
+        if (kind == SV_PAGE)
+            page(dst, g, src);
+        else
+            tail(dst, g, tl, kind == SV_TAIL ? rest : 0);
+    }
+    // In tiles with masked places, this thread's 32 values of the group once more: is one no number?
+    __device__ __forceinline__ void note(unsigned char* dst, int g, int kind, int par, int key0) const {
+        const bool pg = kind == SV_PAGE;
 #pragma unroll 1
-        for (int k = 0; k < 32; k++) {
-            const int u = tid + 128 * (is_tail ? k >> 3 : k >> 4);
-            const int r = 64 * g + (is_tail ? u >> 3 : u >> 2);
-            const int d = is_tail ? 8 * (u & 7) + (k & 7) : 16 * (u & 3) + (k & 15);
-            sv_note(S, par, sv_at(dst, r, d), key0 + r, d);
+        for (int i = 0; i < 4; i++) {  // its four 16-byte chunks of the tile
+            const int u = tid + 128 * (pg ? i >> 1 : i), r = 64 * g + (pg ? u >> 2 : u >> 3);
+            const int c = pg ? 2 * (u & 3) + (i & 1) : u & 7;
+            const uint4 x = *reinterpret_cast<const uint4*>(dst + r * 128 + ((c ^ (r & 7)) << 4));
+            if (!sv_stuck(sv_sticky(sv_sticky(sv_sticky(sv_sticky(0, x.x), x.y), x.z), x.w))) continue;
+#pragma unroll 1
+            for (int e = 0; e < 8; e++) sv_note(S, par, sv_at(dst, r, 8 * c + e), key0 + r, 8 * c + e);
         }
     }
 };
-// page of group g: -1 absent, -2 the tail
-__device__ __forceinline__ int sv_page(const AttnArgs& A, const SvSeq& q, int s, int g) {
-    const int ng = q.kv / SERVE_PAGE;
-    if (g >= ng) return g == ng && q.kv % SERVE_PAGE ? -2 : -1;
-    return __ldg(A.kv.table + (size_t)s * A.kv.width + g);
-}
-__device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigned char* Ks, unsigned char* Vs, int tid) {
+// Four warps widen the FP8 tiles that the copying warp asks for.
+__device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigned char* Ks, unsigned char* Vs,
+                                           const unsigned char* Fs, int tid) {
+    constexpr int KST = SvCfg<true>::KST;
     const int lane = tid & 31, warp = tid >> 5;
-    const SvConv cv = {A, S, tid};
+    const SvConv cv = {S, tid};
     uint32_t seg = 0, kt = 0;
     bool ok = true;
-    // an index outside the pool: reported once per use, then absent
-    auto valid = [&](const SvItem& w, int page, int g) -> int {
-        if (g < w.q.kv / SERVE_PAGE && (page < 0 || page >= A.kv.n_pages)) {
-            if (tid == 0) atomicOr(A.err, SERVE_ERR_PAGE);
-            return -3;
-        }
-        return page;
-    };
     for (; ok; seg++) {
         const int par = seg & 1;
-        if (!(ok = sv_wait(&S->q_full[par], (seg >> 1) & 1, &S->abort_))) break;
+        if (!(ok = sv_wait_all(&S->q_full[par], (seg >> 1) & 1, &S->abort_))) break;
         const SvItem& w = S->item[seg & 3];
         if (w.n == 0) break;
         if (lane == 0) mbar_arrive(&S->q_empty[par]);
         // this parity's notes were last read two segments ago
-        if (seg >= 2 && !(ok = sv_wait(&S->epi[par], ((seg >> 1) - 1) & 1, &S->abort_))) break;
+        if (seg >= 2 && !(ok = sv_wait_all(&S->epi[par], ((seg >> 1) - 1) & 1, &S->abort_))) break;
         if (warp == 0) {
             for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[par][0][0])[u] = 0x7fffffff;
             if (lane == 0) S->any_bad[par] = 0;
@@ -390,68 +377,82 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigne
         __threadfence_block();
         __syncwarp();
         if (lane == 0) mbar_arrive(&S->conv);
-        if (!(ok = sv_wait(&S->conv, seg & 1, &S->abort_))) break;
+        if (!(ok = sv_wait_all(&S->conv, seg & 1, &S->abort_))) break;
 
         const size_t tail = ((size_t)w.s * A.nkv + w.h) * SERVE_PAGE_HEAD;
-        const int rest = w.q.kv % SERVE_PAGE;
-        int pg[2], pn[2];  // pages of this tile and (as read) of the next
-        uint4 kx[2][2], vx[2][2];
-        float sc = 0.f, sn = 0.f;  // threads 0..3: (K, V) x (group 0, 1)
-        auto scale = [&](const int* p) -> float {
-            const int page = p[tid & 1];
-            if (page == -3) return -1.f;
-            if (page < 0) return 1.f;
-            return __half2float((tid & 2 ? A.kv.vps : A.kv.kps)[(size_t)page * A.nkv + w.h]);
-        };
+        const int tb = w.tb, te = w.te, rest = w.q.kv % SERVE_PAGE, first_masked = (w.q.p0 + w.t0 + 1) >> 7;
+        for (int i = tb; i < te; i++, kt++) {
+            const uint32_t st = kt % KST, ph = ((kt / KST) & 1) ^ 1, fs = kt % SV_FST;
+            const unsigned char* f = Fs + fs * SV_F_BYTES;  // keys of both groups, then values
+            unsigned char *kd = Ks + st * SV_TILE_BYTES, *vd = Vs + st * SV_TILE_BYTES;
+            if (!(ok = sv_wait_all(&S->f_full[fs], (kt / SV_FST) & 1, &S->abort_))) break;
+            const int kind[2] = {S->kind[fs][0], S->kind[fs][1]};
+            if (!(ok = sv_wait_all(&S->k_empty[st], ph, &S->abort_))) break;
 #pragma unroll
-        for (int g = 0; g < 2; g++) pg[g] = valid(w, sv_page(A, w.q, w.s, 2 * w.tb + g), 2 * w.tb + g);
-#pragma unroll
-        for (int g = 0; g < 2; g++) cv.load(A.kv.kp8, pg[g], w.h, kx[g]), cv.load(A.kv.vp8, pg[g], w.h, vx[g]);
-        if (tid < 4) sc = scale(pg);
-#pragma unroll
-        for (int g = 0; g < 2; g++) pn[g] = w.tb + 1 < w.te ? sv_page(A, w.q, w.s, 2 * (w.tb + 1) + g) : -1;
-        for (int i = w.tb; i < w.te; i++, kt++) {
-            const uint32_t st = kt % SV_KST, ph = ((kt / SV_KST) & 1) ^ 1;
-            const bool masked = sv_masked(w.q, w.t0, i);
-            int pq[2];  // the next tile's pages, checked
-#pragma unroll
-            for (int g = 0; g < 2; g++) pq[g] = i + 1 < w.te ? valid(w, pn[g], 2 * (i + 1) + g) : -1;
-            if (tid < 4) sn = scale(pq);
-#pragma unroll
-            for (int g = 0; g < 2; g++) pn[g] = i + 2 < w.te ? sv_page(A, w.q, w.s, 2 * (i + 2) + g) : -1;
-            if (!(ok = sv_wait(&S->k_empty[st], ph, &S->abort_))) break;
-            unsigned char* kd = Ks + st * SV_TILE_BYTES;
-#pragma unroll
-            for (int g = 0; g < 2; g++) {
-                if (pg[g] == -2)
-                    cv.tail(kd, g, A.kv.ktail + tail, rest);
-                else
-                    cv.store(kd, g, kx[g]);
-            }
-            if (tid < 4) S->sc[kt % SV_SC][tid] = sc;
-            sc = sn;
+            for (int g = 0; g < 2; g++) cv.group(kd, g, kind[g], f + g * SERVE_PAGE_HEAD, A.kv.ktail + tail, rest);
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&S->k_full[st]);
-#pragma unroll
-            for (int g = 0; g < 2; g++) cv.load(A.kv.kp8, pq[g], w.h, kx[g]);
-            if (!(ok = sv_wait(&S->v_empty[st], ph, &S->abort_))) break;
-            unsigned char* vd = Vs + st * SV_TILE_BYTES;
+            if (!(ok = sv_wait_all(&S->v_empty[st], ph, &S->abort_))) break;
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-                const bool bad = pg[g] == -2 ? cv.tail(vd, g, A.kv.vtail + tail, rest) : cv.store(vd, g, vx[g]);
-                if (masked && bad) cv.note(vd, g, pg[g] == -2, par, i * SV_KT);
+                cv.group(vd, g, kind[g], f + (2 + g) * SERVE_PAGE_HEAD, A.kv.vtail + tail, rest);
+                if (i >= first_masked) cv.note(vd, g, kind[g], par, i * SV_KT);
             }
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __threadfence_block();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&S->v_full[st]);
-#pragma unroll
-            for (int g = 0; g < 2; g++) cv.load(A.kv.vp8, pq[g], w.h, vx[g]), pg[g] = pq[g];
+            if (lane == 0) mbar_arrive(&S->v_full[st]), mbar_arrive(&S->f_empty[fs]);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&S->epi[par]);
     }
+}
+// The tiles of an item, two pages each, by the copying warp; kt: tiles so far.  Lane l has the page index and the
+// scales of group l of 16 tiles.
+__device__ __forceinline__ bool sv_pages(const AttnArgs& A, SvSmem* S, const SvItem& w, unsigned char* Fs, uint32_t& kt,
+                                         int lane) {
+    const int ng = w.q.kv / SERVE_PAGE, te = w.te;
+    for (int c = w.tb; c < te; c += 16) {
+        const int g = 2 * c + lane;
+        int kind = g < ng ? SV_PAGE : g == ng && w.q.kv % SERVE_PAGE ? SV_TAIL : SV_NONE;
+        size_t blk = 0;
+        float ks = 1.f, vs = 1.f;
+        if (kind == SV_PAGE && g < 2 * te) {
+            const int page = __ldg(A.kv.table + (size_t)w.s * A.kv.width + g);
+            if (page >= 0 && page < A.kv.n_pages) {
+                blk = (size_t)page * A.nkv + w.h;
+                ks = __half2float(__ldg(A.kv.kps + blk)), vs = __half2float(__ldg(A.kv.vps + blk));
+            } else {
+                atomicOr(A.err, SERVE_ERR_PAGE);
+                kind = SV_NONE, ks = -1.f;
+            }
+        }
+        const int n = min(16, te - c);
+        for (int i = 0; i < n; i++, kt++) {
+            const uint32_t fs = kt % SV_FST;
+            if (!sv_wait_all(&S->f_empty[fs], ((kt / SV_FST) & 1) ^ 1, &S->abort_)) return false;
+            const bool mine = lane >> 1 == i;
+            if (mine) {
+                S->sc[kt % SV_SC][lane & 1] = ks, S->sc[kt % SV_SC][2 + (lane & 1)] = vs;
+                S->kind[fs][lane & 1] = kind;
+            }
+            const uint32_t pages = __popc(__ballot_sync(0xffffffffu, mine && kind == SV_PAGE));
+            if (lane == 0) {
+                if (pages)
+                    mbar_arrive_expect_tx(&S->f_full[fs], pages * 2 * SERVE_PAGE_HEAD);
+                else
+                    mbar_arrive(&S->f_full[fs]);
+            }
+            __syncwarp();
+            if (mine && kind == SV_PAGE) {
+                unsigned char* dst = Fs + fs * SV_F_BYTES + (lane & 1) * SERVE_PAGE_HEAD;
+                tma_load_1d(dst, A.kv.kp8 + blk * SERVE_PAGE_HEAD, SERVE_PAGE_HEAD, &S->f_full[fs]);
+                tma_load_1d(dst + 2 * SERVE_PAGE_HEAD, A.kv.vp8 + blk * SERVE_PAGE_HEAD, SERVE_PAGE_HEAD, &S->f_full[fs]);
+            }
+        }
+    }
+    return true;
 }
 
 template <bool PAGED>
@@ -463,8 +464,10 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
     unsigned char* sm = sv_raw + ((1024 - (smem_u32(sv_raw) & 1023)) & 1023);
     unsigned char* Qs = sm;
     unsigned char* Ks = Qs + 2 * SV_Q_BYTES;
-    unsigned char* Vs = Ks + SV_KST * SV_TILE_BYTES;
-    SvSmem* S = reinterpret_cast<SvSmem*>(Vs + SV_KST * SV_TILE_BYTES);
+    constexpr int KST = C::KST;
+    unsigned char* Vs = Ks + KST * SV_TILE_BYTES;
+    unsigned char* Fs = Vs + KST * SV_TILE_BYTES;  // (paged)
+    SvSmem* S = reinterpret_cast<SvSmem*>(Ks + 8 * SV_TILE_BYTES);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = A.nh / A.nkv, TOK = 128 / G, tq = 2 * TOK;
     pdl_trigger();
@@ -479,7 +482,8 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             mbar_init(&S->o_full[i], 1), mbar_init(&S->o_free[i], 4), mbar_init(&S->epi[i], PAGED ? 12 : 9);
             S->any_bad[i] = 0;
         }
-        for (int i = 0; i < SV_KST; i++) {
+        for (int i = 0; i < SV_FST; i++) mbar_init(&S->f_full[i], 1), mbar_init(&S->f_empty[i], 4);
+        for (int i = 0; i < KST; i++) {
             mbar_init(&S->k_full[i], PAGED ? 4 : 1), mbar_init(&S->k_empty[i], 2);
             mbar_init(&S->v_full[i], PAGED ? 4 : 1), mbar_init(&S->v_empty[i], 2);
             mbar_init(&S->v_ok[i], 1);
@@ -512,13 +516,13 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         uint32_t ops = 0, tiles = 0, seg = 0;
         bool ok = true;
         for (; ok; seg++) {
-            if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
+            if (!(ok = sv_wait_all(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
             const SvItem& w = S->item[seg & 3];
             if (w.n == 0) break;
             if (lane == 0) mbar_arrive(&S->q_empty[seg & 1]);
             const bool act1 = w.t0 + TOK < w.q.c;
             // all who arrive at a segment's epi barrier have seen the one before of the same parity complete
-            if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_))) break;
+            if (seg >= 2 && !(ok = sv_wait_all(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_))) break;
             if (t == 1 && !act1) {
                 tiles += w.te - w.tb;
                 __syncwarp();
@@ -533,7 +537,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             const int tb = w.tb, te = w.te;
             const int first_masked = (w.q.p0 + w.t0 + t * TOK + 1) >> 7;  // from here some row masks some key
             for (int i = tb; i < te; i++, ops++, tiles++) {
-                if (!(ok = sv_wait(&S->s_full[t], ops & 1, &S->abort_))) break;
+                if (!(ok = sv_wait_all(&S->s_full[t], ops & 1, &S->abort_))) break;
                 sv_fence_after();
                 uint32_t sr[128];
                 float* s = reinterpret_cast<float*>(sr);
@@ -585,7 +589,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 const float x = fmaxf(mx[0], mx[1]);
                 // the last product has read P and written O
                 if (i > tb) {
-                    if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_))) break;
+                    if (!(ok = sv_wait_all(&S->o_full[t], (ops - 1) & 1, &S->abort_))) break;
                     sv_fence_after();
                 }
                 if (i == tb) {
@@ -633,7 +637,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             }
             if (!ok) break;
             // ---- epilogue of the item (or of the CTA's part of it) ----
-            if (!(ok = sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_))) break;
+            if (!(ok = sv_wait_all(&S->o_full[t], (ops - 1) & 1, &S->abort_))) break;
             sv_fence_after();
             float la, lb;
             f2_unpack(f2_add(l2[0], l2[1]), la, lb);
@@ -692,51 +696,58 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(C::REG_LO));
         if (warp == C::Q_WARP) {
             // ---- the walk; Q (and, packed, K and V) by TMA ----
-            if (lane == 0) {
-                SvItem w;
-                uint32_t seg = 0, kt = 0, nq = 0, nk = 0, nv = 0;  // copies issued
-                sv_first<C::KIND>(A, S, w, tq, split);
-                for (;; seg++) {
-                    const uint32_t qsl = seg & 1;
-                    if (!sv_wait(&S->q_empty[qsl], ((seg >> 1) & 1) ^ 1, &S->abort_)) break;
-                    if (w.left <= 0) {
+            SvItem w;  // (lane 0's)
+            uint32_t seg = 0, kt = 0, nq = 0, nk = 0, nv = 0;  // copies issued
+            if (lane == 0) sv_first<C::KIND>(A, S, w, tq, split);
+            bool ok = true;
+            for (; ok; seg++) {
+                const uint32_t qsl = seg & 1;
+                bool more = false;
+                if (lane == 0) {
+                    ok = sv_wait(&S->q_empty[qsl], ((seg >> 1) & 1) ^ 1, &S->abort_);
+                    more = ok && w.left > 0;
+                    if (more) {
+                        S->item[seg & 3] = w;
+                        const int nt = w.t0 + TOK < w.q.c ? 2 : 1;
+                        mbar_arrive_expect_tx(&S->q_full[qsl], (uint32_t)(TOK * G * 128) * nt);
+                        for (int t = 0; t < nt; t++)
+                            sv_tma_3d(Qs + qsl * SV_Q_BYTES + t * SV_TILE_BYTES, &qmap, 0, w.h * G,
+                                      w.q.a + w.t0 + t * TOK, &S->q_full[qsl]);
+                        nq = seg + 1;
+                    } else if (ok) {
                         S->item[seg & 3].n = 0;
                         mbar_arrive(&S->q_full[qsl]);
-                        break;
                     }
-                    S->item[seg & 3] = w;
-                    const int nt = w.t0 + TOK < w.q.c ? 2 : 1;
-                    mbar_arrive_expect_tx(&S->q_full[qsl], (uint32_t)(TOK * G * 128) * nt);
-                    for (int t = 0; t < nt; t++)
-                        sv_tma_3d(Qs + qsl * SV_Q_BYTES + t * SV_TILE_BYTES, &qmap, 0, w.h * G, w.q.a + w.t0 + t * TOK,
-                                  &S->q_full[qsl]);
-                    nq = seg + 1;
-                    bool ok = true;
-                    if (!PAGED) {
-                        for (int i = w.tb; i < w.te; i++, kt++) {
-                            const uint32_t st = kt % SV_KST, ph = ((kt / SV_KST) & 1) ^ 1;
-                            if (!(ok = sv_wait(&S->k_empty[st], ph, &S->abort_))) break;
-                            mbar_arrive_expect_tx(&S->k_full[st], SV_TILE_BYTES);
-                            sv_tma_3d(Ks + st * SV_TILE_BYTES, &kmap, 0, w.h, w.q.a + i * SV_KT, &S->k_full[st]);
-                            nk++;
-                            if (!(ok = sv_wait(&S->v_empty[st], ph, &S->abort_))) break;
-                            mbar_arrive_expect_tx(&S->v_full[st], SV_TILE_BYTES);
-                            sv_tma_3d(Vs + st * SV_TILE_BYTES, &vmap, 0, w.h, w.q.a + i * SV_KT, &S->v_full[st]);
-                            nv++;
-                        }
+                }
+                if constexpr (PAGED) {
+                    if (!__shfl_sync(0xffffffffu, (int)more, 0)) break;
+                    __syncwarp();
+                    ok = sv_pages(A, S, S->item[seg & 3], Fs, kt, lane);
+                } else {
+                    if (!more) break;  // (lane 0 alone goes on)
+                    for (int i = w.tb; i < w.te; i++, kt++) {
+                        const uint32_t st = kt % KST, ph = ((kt / KST) & 1) ^ 1;
+                        if (!(ok = sv_wait(&S->k_empty[st], ph, &S->abort_))) break;
+                        mbar_arrive_expect_tx(&S->k_full[st], SV_TILE_BYTES);
+                        sv_tma_3d(Ks + st * SV_TILE_BYTES, &kmap, 0, w.h, w.q.a + i * SV_KT, &S->k_full[st]);
+                        nk++;
+                        if (!(ok = sv_wait(&S->v_empty[st], ph, &S->abort_))) break;
+                        mbar_arrive_expect_tx(&S->v_full[st], SV_TILE_BYTES);
+                        sv_tma_3d(Vs + st * SV_TILE_BYTES, &vmap, 0, w.h, w.q.a + i * SV_KT, &S->v_full[st]);
+                        nv++;
                     }
-                    if (!ok) break;
-                    sv_next<C::KIND>(A, w, tq, split);
                 }
-                // every copy is waited for by those who use it; after an abort, what is in flight has to land before
-                // the CTA can exit
-                if (*(volatile int*)&S->abort_) {
-                    for (uint32_t k = nq < 2 ? 0 : nq - 2; k < nq; k++) sv_drain(&S->q_full[k & 1], (k >> 1) & 1);
-                    for (uint32_t k = nk < SV_KST ? 0 : nk - SV_KST; k < nk; k++)
-                        sv_drain(&S->k_full[k % SV_KST], (k / SV_KST) & 1);
-                    for (uint32_t k = nv < SV_KST ? 0 : nv - SV_KST; k < nv; k++)
-                        sv_drain(&S->v_full[k % SV_KST], (k / SV_KST) & 1);
-                }
+                if (lane == 0) sv_next<C::KIND>(A, w, tq, split);
+            }
+            // every copy is waited for by those who use it; after an abort, what is in flight has to land before the
+            // CTA can exit
+            if (lane == 0 && *(volatile int*)&S->abort_) {
+                for (uint32_t k = nq < 2 ? 0 : nq - 2; k < nq; k++) sv_drain(&S->q_full[k & 1], (k >> 1) & 1);
+                for (uint32_t k = nk < KST ? 0 : nk - KST; k < nk; k++) sv_drain(&S->k_full[k % KST], (k / KST) & 1);
+                for (uint32_t k = nv < KST ? 0 : nv - KST; k < nv; k++) sv_drain(&S->v_full[k % KST], (k / KST) & 1);
+                if (PAGED)
+                    for (uint32_t k = kt < SV_FST ? 0 : kt - SV_FST; k < kt; k++)
+                        sv_drain(&S->f_full[k % SV_FST], (k / SV_FST) & 1);
             }
             __syncwarp();
         } else if (warp == C::MMA_WARP || warp == C::MMA_WARP + 1) {
@@ -753,9 +764,9 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             bool ok = true;
             uint32_t n1 = 0;  // (t = 0) products of row tile 1 in key tiles so far
             auto scores = [&](uint32_t qa, bool turns, bool first) -> bool {
-                const uint32_t st = kt % SV_KST;
-                if (!sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_)) return false;
-                if (nq > 0 && !sv_wait(&S->s_free[t], (nq - 1) & 1, &S->abort_)) return false;
+                const uint32_t st = kt % KST;
+                if (!sv_wait_all(&S->k_full[st], (kt / KST) & 1, &S->abort_)) return false;
+                if (nq > 0 && !sv_wait_all(&S->s_free[t], (nq - 1) & 1, &S->abort_)) return false;
                 // The row tiles take turns: one's exponentials run beside the other's loads and maxima.  Only a
                 // matter of pace, so it is not insisted on (and a phase that has gone by unseen costs some tries).
                 if (t == 1) {
@@ -778,16 +789,16 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 return true;
             };
             for (; ok; seg++) {
-                if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
+                if (!(ok = sv_wait_all(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
                 const SvItem& w = S->item[seg & 3];
                 if (w.n == 0) break;
                 const int nt = w.te - w.tb;
                 if (t == 1 && w.t0 + TOK >= w.q.c) {  // the block has one row tile: only let the stages go
                     for (int i = 0; ok && i < nt; i++, kt++, vt++) {
-                        const uint32_t st = kt % SV_KST;
-                        if (!(ok = sv_wait(&S->k_full[st], (kt / SV_KST) & 1, &S->abort_))) break;
+                        const uint32_t st = kt % KST;
+                        if (!(ok = sv_wait_all(&S->k_full[st], (kt / KST) & 1, &S->abort_))) break;
                         if (leader) mbar_arrive(&S->k_empty[st]);
-                        if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_))) break;
+                        if (!(ok = sv_wait_all(&S->v_full[st], (vt / KST) & 1, &S->abort_))) break;
                         if (leader) mbar_arrive(&S->v_empty[st]);
                     }
                     if (leader) mbar_arrive(&S->q_empty[seg & 1]);
@@ -799,11 +810,11 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 for (int i = 0; i < nt; i++) {
                     if (i + 1 < nt && !(ok = scores(qa, turns, false))) break;
                     if (leader && i == max(nt - 2, 0)) sv_commit(&S->q_empty[seg & 1]);  // the last scores are under way
-                    const uint32_t st = vt % SV_KST;
-                    if (!(ok = sv_wait(&S->v_full[st], (vt / SV_KST) & 1, &S->abort_))) break;
-                    if (!PAGED && !(ok = sv_wait(&S->v_ok[st], (vt / SV_KST) & 1, &S->abort_))) break;
-                    if (i == 0 && segs > 0 && !(ok = sv_wait(&S->o_free[t], (segs - 1) & 1, &S->abort_))) break;
-                    if (!(ok = sv_wait(&S->p_full[t], np & 1, &S->abort_))) break;
+                    const uint32_t st = vt % KST;
+                    if (!(ok = sv_wait_all(&S->v_full[st], (vt / KST) & 1, &S->abort_))) break;
+                    if (!PAGED && !(ok = sv_wait_all(&S->v_ok[st], (vt / KST) & 1, &S->abort_))) break;
+                    if (i == 0 && segs > 0 && !(ok = sv_wait_all(&S->o_free[t], (segs - 1) & 1, &S->abort_))) break;
+                    if (!(ok = sv_wait_all(&S->p_full[t], np & 1, &S->abort_))) break;
                     sv_fence_after();
                     if (leader) {
                         const uint32_t va = v_lo + st * (SV_TILE_BYTES >> 4);
@@ -825,19 +836,19 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             uint32_t seg = 0, kt = 0;
             bool ok = true;
             for (; ok; seg++) {
-                if (!(ok = sv_wait(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
+                if (!(ok = sv_wait_all(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
                 const SvItem& w = S->item[seg & 3];
                 if (w.n == 0) break;
                 if (lane == 0) mbar_arrive(&S->q_empty[seg & 1]);
                 // this parity's notes were last read two segments ago
-                if (seg >= 2 && !(ok = sv_wait(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_))) break;
+                if (seg >= 2 && !(ok = sv_wait_all(&S->epi[seg & 1], ((seg >> 1) - 1) & 1, &S->abort_))) break;
                 for (int u = lane; u < 3 * CUINF_HD; u += 32) (&S->bad[seg & 1][0][0])[u] = 0x7fffffff;
                 if (lane == 0) S->any_bad[seg & 1] = 0;
                 __syncwarp();
                 for (int i = w.tb; i < w.te; i++, kt++) {
-                    const uint32_t st = kt % SV_KST;
+                    const uint32_t st = kt % KST;
                     // every tile passes here, so that no phase of v_full goes unseen
-                    if (!(ok = sv_wait(&S->v_full[st], (kt / SV_KST) & 1, &S->abort_))) break;
+                    if (!(ok = sv_wait_all(&S->v_full[st], (kt / KST) & 1, &S->abort_))) break;
                     if (!sv_masked(w.q, w.t0, i)) {
                         if (lane == 0) mbar_arrive(&S->v_ok[st]);
                         continue;
@@ -864,7 +875,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             }
             __syncwarp();
         } else if (PAGED && warp < 12) {
-            if constexpr (PAGED) sv_convert(A, S, Ks, Vs, tid - 256);
+            if constexpr (PAGED) sv_convert(A, S, Ks, Vs, Fs, tid - 256);
         }
     }
     sv_fence_before();
