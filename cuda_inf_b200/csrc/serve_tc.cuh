@@ -537,7 +537,8 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             const int tb = w.tb, te = w.te;
             const int first_masked = (w.q.p0 + w.t0 + t * TOK + 1) >> 7;  // from here some row masks some key
             for (int i = tb; i < te; i++, ops++, tiles++) {
-                if (!(ok = sv_wait_all(&S->s_full[t], ops & 1, &S->abort_))) break;
+                // (a wait that gave up ends the loop after the tile, for all lanes alike)
+                ok = sv_wait(&S->s_full[t], ops & 1, &S->abort_);
                 sv_fence_after();
                 uint32_t sr[128];
                 float* s = reinterpret_cast<float*>(sr);
@@ -589,7 +590,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 const float x = fmaxf(mx[0], mx[1]);
                 // the last product has read P and written O
                 if (i > tb) {
-                    if (!(ok = sv_wait_all(&S->o_full[t], (ops - 1) & 1, &S->abort_))) break;
+                    ok &= sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_);
                     sv_fence_after();
                 }
                 if (i == tb) {
@@ -634,6 +635,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 sv_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S->p_full[t]);
+                if (!(ok = __all_sync(0xffffffffu, ok))) break;
             }
             if (!ok) break;
             // ---- epilogue of the item (or of the CTA's part of it) ----
@@ -765,8 +767,8 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             uint32_t n1 = 0;  // (t = 0) products of row tile 1 in key tiles so far
             auto scores = [&](uint32_t qa, bool turns, bool first) -> bool {
                 const uint32_t st = kt % KST;
-                if (!sv_wait_all(&S->k_full[st], (kt / KST) & 1, &S->abort_)) return false;
-                if (nq > 0 && !sv_wait_all(&S->s_free[t], (nq - 1) & 1, &S->abort_)) return false;
+                bool fine = sv_wait(&S->k_full[st], (kt / KST) & 1, &S->abort_);
+                if (nq > 0) fine &= sv_wait(&S->s_free[t], (nq - 1) & 1, &S->abort_);
                 // The row tiles take turns: one's exponentials run beside the other's loads and maxima.  Only a
                 // matter of pace, so it is not insisted on (and a phase that has gone by unseen costs some tries).
                 if (t == 1) {
@@ -786,7 +788,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     sv_commit(&S->k_empty[st]);
                 }
                 nq++, kt++;
-                return true;
+                return fine;
             };
             for (; ok; seg++) {
                 if (!(ok = sv_wait_all(&S->q_full[seg & 1], (seg >> 1) & 1, &S->abort_))) break;
@@ -806,15 +808,15 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 }
                 const uint32_t qa = q_lo + (seg & 1) * (SV_Q_BYTES >> 4);
                 const bool turns = w.t0 + TOK < w.q.c;
-                if (!(ok = scores(qa, turns, true))) break;
+                ok = scores(qa, turns, true);
                 for (int i = 0; i < nt; i++) {
-                    if (i + 1 < nt && !(ok = scores(qa, turns, false))) break;
+                    if (i + 1 < nt) ok &= scores(qa, turns, false);
                     if (leader && i == max(nt - 2, 0)) sv_commit(&S->q_empty[seg & 1]);  // the last scores are under way
                     const uint32_t st = vt % KST;
-                    if (!(ok = sv_wait_all(&S->v_full[st], (vt / KST) & 1, &S->abort_))) break;
-                    if (!PAGED && !(ok = sv_wait_all(&S->v_ok[st], (vt / KST) & 1, &S->abort_))) break;
-                    if (i == 0 && segs > 0 && !(ok = sv_wait_all(&S->o_free[t], (segs - 1) & 1, &S->abort_))) break;
-                    if (!(ok = sv_wait_all(&S->p_full[t], np & 1, &S->abort_))) break;
+                    ok &= sv_wait(&S->v_full[st], (vt / KST) & 1, &S->abort_);
+                    if (!PAGED) ok &= sv_wait(&S->v_ok[st], (vt / KST) & 1, &S->abort_);
+                    if (i == 0 && segs > 0) ok &= sv_wait(&S->o_free[t], (segs - 1) & 1, &S->abort_);
+                    ok &= sv_wait(&S->p_full[t], np & 1, &S->abort_);
                     sv_fence_after();
                     if (leader) {
                         const uint32_t va = v_lo + st * (SV_TILE_BYTES >> 4);
@@ -826,6 +828,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                         sv_commit(&S->v_empty[st]);
                     }
                     np++, vt++;
+                    if (!(ok = __all_sync(0xffffffffu, ok))) break;
                 }
                 segs++;
             }
