@@ -39,7 +39,6 @@
 #define SV_SC 16         // slots of the pages' scales (more tiles than can be in flight)
 #define SV_TILE_BYTES (SV_KT * CUINF_HD * 2)
 #define SV_TMEM_COLS 512
-#define SV_TURN 64       // tries
 #define SV_P_COL 256     // S of row tile t at 128 t, P at 256 + 64 t, O at 384 + 64 t
 #define SV_O_COL 384
 
@@ -57,7 +56,7 @@ struct SvSmem {
     uint64_t s_full[2], s_free[2], p_full[2], o_full[2], o_free[2], epi[2], conv, done;
     uint32_t tmem;
     int abort_;
-    float sc[SV_SC][4];  // FP8: K scale of the tile's two pages (negative: absent), V scales
+    alignas(16) float sc[SV_SC][4];  // (read by float4) FP8: K scale of the tile's two pages (negative: absent), V scales
     int kind[SV_FST][2];  // FP8: what the tile's two groups are (SV_PAGE ...)
     int bad[2][3][CUINF_HD];  // by segment parity: first key whose value is +inf, -inf, NaN
     int any_bad[2];
@@ -544,20 +543,16 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 float* s = reinterpret_cast<float*>(sr);
                 sv_ld32(s_addr, sr), sv_ld32(s_addr + 32, sr + 32);
                 float kc[2] = {c2, c2}, vc[2] = {1.f, 1.f};
-                bool gone[2] = {false, false};
+                bool masked = i >= first_masked, gone[2] = {false, false};
                 if (PAGED) {
-                    const float* sc = S->sc[tiles % SV_SC];
-#pragma unroll
-                    for (int g = 0; g < 2; g++) {
-                        gone[g] = sc[g] < 0.f;
-                        kc[g] = c2 * sc[g];
-                        if (kc[g] == 0.f) kc[g] = 1e-30f;  // a page of zeros: -inf * 0 is no number
-                        vc[g] = SV_VEXP * sc[2 + g];
-                    }
+                    const float4 sc = *reinterpret_cast<const float4*>(S->sc[tiles % SV_SC]);
+                    kc[0] = c2 * sc.x, kc[1] = c2 * sc.y;
+                    vc[0] = SV_VEXP * sc.z, vc[1] = SV_VEXP * sc.w;
+                    gone[0] = sc.x < 0.f, gone[1] = sc.y < 0.f;
+                    masked |= gone[0] | gone[1];
                 }
                 sv_wait_ld();
                 sv_ld32(s_addr + 64, sr + 64), sv_ld32(s_addr + 96, sr + 96);
-                const bool masked = i >= first_masked;
                 const int lim = pos - i * SV_KT;  // last key of the tile that the row attends
                 float mx[2];
 #pragma unroll
@@ -569,15 +564,14 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                         if (lane == 0) mbar_arrive(&S->s_free[t]);  // the next scores may come while these are worked on
                     }
                     if (masked) {
+                        const int last = gone[g] ? -1 : lim;
 #pragma unroll
-                        for (int j = 64 * g; j < 64 * g + 64; j++) s[j] = j <= lim ? s[j] : -INFINITY;
-                        // a page's scale that is no number reaches only rows that attend the page
-                        if (PAGED && lim < 64 * g) kc[g] = c2, vc[g] = 0.f;
-                    }
-                    if (PAGED && gone[g]) {
-                        kc[g] = c2, vc[g] = 0.f;
-#pragma unroll
-                        for (int j = 0; j < 64; j++) s[64 * g + j] = -INFINITY;
+                        for (int j = 64 * g; j < 64 * g + 64; j++) s[j] = j <= last ? s[j] : -INFINITY;
+                        if (PAGED) {
+                            // a page's scale that is no number reaches only rows that attend the page
+                            if (last < 64 * g) kc[g] = c2, vc[g] = 0.f;
+                            if (kc[g] == 0.f) kc[g] = 1e-30f;  // a page of zeros: -inf * 0 is no number
+                        }
                     }
                     float a[8];
 #pragma unroll
@@ -600,7 +594,8 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     const float mn = fmaxf(m, x);
                     const float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
                     m = mn;
-                    l2[0] = f2_mul(l2[0], f2_pack(f, f)), l2[1] = f2_mul(l2[1], f2_pack(f, f));
+#pragma unroll
+                    for (int e = 0; e < 2; e++) l2[e] = f2_mul(l2[e], f2_pack(f, f));
 #pragma unroll 1
                     for (uint32_t j = 0; j < CUINF_HD; j += 16) {
                         uint32_t o[16];
@@ -764,20 +759,10 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             uint32_t seg = 0, kt = 0, vt = 0;
             uint32_t nq = 0, np = 0, segs = 0;  // products of this row tile so far; segments in which it is active
             bool ok = true;
-            uint32_t n1 = 0;  // (t = 0) products of row tile 1 in key tiles so far
-            auto scores = [&](uint32_t qa, bool turns, bool first) -> bool {
+            auto scores = [&](uint32_t qa) -> bool {
                 const uint32_t st = kt % KST;
                 bool fine = sv_wait(&S->k_full[st], (kt / KST) & 1, &S->abort_);
                 if (nq > 0) fine &= sv_wait(&S->s_free[t], (nq - 1) & 1, &S->abort_);
-                // The row tiles take turns: one's exponentials run beside the other's loads and maxima.  Only a
-                // matter of pace, so it is not insisted on (and a phase that has gone by unseen costs some tries).
-                if (t == 1) {
-                    for (int k = 0; k < SV_TURN && !mbar_test_wait(&S->s_free[0], kt & 1); k++) {}
-                } else if (turns) {
-                    if (!first)
-                        for (int k = 0; k < SV_TURN && !mbar_test_wait(&S->s_free[1], (n1 - 1) & 1); k++) {}
-                    n1++;
-                }
                 sv_fence_after();
                 if (leader) {
                     const uint32_t ka = k_lo + st * (SV_TILE_BYTES >> 4);
@@ -807,10 +792,9 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     continue;
                 }
                 const uint32_t qa = q_lo + (seg & 1) * (SV_Q_BYTES >> 4);
-                const bool turns = w.t0 + TOK < w.q.c;
-                ok = scores(qa, turns, true);
+                ok = scores(qa);
                 for (int i = 0; i < nt; i++) {
-                    if (i + 1 < nt) ok &= scores(qa, turns, false);
+                    if (i + 1 < nt) ok &= scores(qa);
                     if (leader && i == max(nt - 2, 0)) sv_commit(&S->q_empty[seg & 1]);  // the last scores are under way
                     const uint32_t st = vt % KST;
                     ok &= sv_wait(&S->v_full[st], (vt / KST) & 1, &S->abort_);
