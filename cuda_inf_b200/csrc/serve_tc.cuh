@@ -296,6 +296,12 @@ __device__ __forceinline__ void sv_note(SvSmem* S, int par, __half* p, int key, 
     atomicMin(&S->bad[par][isnan(f) ? 2 : f > 0.f ? 0 : 1][d], key);
     S->any_bad[par] = 1;
 }
+// output column d of a row at `pos` with the values that are no numbers
+__device__ __forceinline__ float sv_with_bad(const SvSmem* S, int par, int d, int pos, float x) {
+    if (S->bad[par][0][d] <= pos) x += INFINITY;
+    if (S->bad[par][1][d] <= pos) x -= INFINITY;
+    return S->bad[par][2][d] <= pos ? NAN : x;
+}
 // place of column d of row r in a 128-byte-swizzled tile of 64-value rows
 __device__ __forceinline__ __half* sv_at(unsigned char* tile, int r, int d) {
     return reinterpret_cast<__half*>(tile + r * 128 + (((d >> 3) ^ (r & 7)) << 4)) + (d & 7);
@@ -512,6 +518,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         const uint32_t o_addr = lane_base + SV_O_COL + t * CUINF_HD;
         const float c2 = A.scale * 1.44269504088896340736f;  // scores in powers of two
         const uint32_t s_addr = lane_base + t * 128, p_addr = lane_base + SV_P_COL + t * 64;
+        const int row_t = row / G, row_h = row - row_t * G;  // the row's token and head in the row tile
         uint32_t ops = 0, tiles = 0, seg = 0;
         bool ok = true;
         for (; ok; seg++) {
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 if (lane == 0) mbar_arrive(&S->epi[seg & 1]);
                 continue;
             }
-            const int tok = w.t0 + t * TOK + row / G;
+            const int tok = w.t0 + t * TOK + row_t;
             const bool live_row = row < TOK * G && tok < w.q.c;
             const int pos = live_row ? w.q.p0 + tok : -1;
             float m = -INFINITY;
@@ -643,35 +650,35 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             const bool whole = w.tb == 0 && w.te == w.n, any_bad = S->any_bad[seg & 1] != 0;
             const size_t slot = (size_t)blockIdx.x * 2 + (w.tb == 0);
             const float inv = whole ? (l == 0.f ? 0.f : vs / l) : vs;
-            __half* dst = A.out + ((size_t)(w.q.a + tok) * A.nh + w.h * G + row % G) * CUINF_HD;
+            __half* dst = A.out + ((size_t)(w.q.a + tok) * A.nh + w.h * G + row_h) * CUINF_HD;
             float* part = W.o + (slot * 256 + t * 128 + row) * CUINF_HD;
 #pragma unroll 1
-            for (int d0 = 0; d0 < CUINF_HD; d0 += 16) {
-                uint32_t o[16];
-                sv_ld16(o_addr + d0, o);
+            for (int d0 = 0; d0 < CUINF_HD; d0 += 32) {
+                uint32_t o[32];
+                sv_ld32(o_addr + d0, o);
                 sv_wait_ld();
-                float* of = reinterpret_cast<float*>(o);
-                if (any_bad) {
-                    const int(*bad)[CUINF_HD] = S->bad[seg & 1];
-#pragma unroll
-                    for (int d = 0; d < 16; d++) {
-                        if (bad[0][d0 + d] <= pos) of[d] += INFINITY;
-                        if (bad[1][d0 + d] <= pos) of[d] -= INFINITY;
-                        if (bad[2][d0 + d] <= pos) of[d] = NAN;
-                    }
-                }
+                const float* of = reinterpret_cast<const float*>(o);
                 if (!live_row) continue;
                 if (whole) {
 #pragma unroll
-                    for (int d = 0; d < 16; d += 8)
+                    for (int d = 0; d < 32; d += 8)
                         *reinterpret_cast<uint4*>(dst + d0 + d) =
                             make_uint4(sv_pack_h2(of[d] * inv, of[d + 1] * inv), sv_pack_h2(of[d + 2] * inv, of[d + 3] * inv),
                                        sv_pack_h2(of[d + 4] * inv, of[d + 5] * inv), sv_pack_h2(of[d + 6] * inv, of[d + 7] * inv));
                 } else {
 #pragma unroll
-                    for (int d = 0; d < 16; d += 4)
+                    for (int d = 0; d < 32; d += 4)
                         *reinterpret_cast<float4*>(part + d0 + d) =
                             make_float4(of[d] * inv, of[d + 1] * inv, of[d + 2] * inv, of[d + 3] * inv);
+                }
+            }
+            if (any_bad && live_row) {  // rare: the row once more, where it has gone
+#pragma unroll 1
+                for (int d = 0; d < CUINF_HD; d++) {
+                    if (whole)
+                        dst[d] = __float2half_rn(sv_with_bad(S, seg & 1, d, pos, __half2float(dst[d])));
+                    else
+                        part[d] = sv_with_bad(S, seg & 1, d, pos, part[d]);
                 }
             }
             sv_fence_before();
