@@ -209,25 +209,32 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
     const unsigned char *kd = x.kd, *vd = x.kd + FW_UNIT / 2;
     if (MASKED) fw_clean<TAIL>(x, S, note, lane);
     float s[NT][4];
+    // four score tiles at a time, so that a product does not wait for the one before it
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-        uint32_t w[8];
-        if (TAIL) {
-            const uint4* src = reinterpret_cast<const uint4*>(kd + (8 * t + g) * 128 + 32 * c);
-            const uint4 a = src[0], b = src[1];
-            w[0] = a.x, w[1] = a.y, w[2] = a.z, w[3] = a.w;
-            w[4] = b.x, w[5] = b.y, w[6] = b.z, w[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(kd + (8 * t + g) * 64 + 16 * c);
-            w[0] = sv_e4m3x2(a.x), w[1] = sv_e4m3x2(a.x >> 16);
-            w[2] = sv_e4m3x2(a.y), w[3] = sv_e4m3x2(a.y >> 16);
-            w[4] = sv_e4m3x2(a.z), w[5] = sv_e4m3x2(a.z >> 16);
-            w[6] = sv_e4m3x2(a.w), w[7] = sv_e4m3x2(a.w >> 16);
+    for (int t0 = 0; t0 < NT; t0 += 4) {
+        uint32_t w[4][8];
+#pragma unroll
+        for (int t = 0; t < 4; t++) {
+            if (TAIL) {
+                const uint4* src = reinterpret_cast<const uint4*>(kd + (8 * (t0 + t) + g) * 128 + 32 * c);
+                const uint4 a = src[0], b = src[1];
+                w[t][0] = a.x, w[t][1] = a.y, w[t][2] = a.z, w[t][3] = a.w;
+                w[t][4] = b.x, w[t][5] = b.y, w[t][6] = b.z, w[t][7] = b.w;
+            } else {
+                const uint4 a = *reinterpret_cast<const uint4*>(kd + (8 * (t0 + t) + g) * 64 + 16 * c);
+                w[t][0] = sv_e4m3x2(a.x), w[t][1] = sv_e4m3x2(a.x >> 16);
+                w[t][2] = sv_e4m3x2(a.y), w[t][3] = sv_e4m3x2(a.y >> 16);
+                w[t][4] = sv_e4m3x2(a.z), w[t][5] = sv_e4m3x2(a.z >> 16);
+                w[t][6] = sv_e4m3x2(a.w), w[t][7] = sv_e4m3x2(a.w >> 16);
+            }
         }
 #pragma unroll
+        for (int t = 0; t < 4; t++) s[t0 + t][0] = s[t0 + t][1] = s[t0 + t][2] = s[t0 + t][3] = 0.f;
+#pragma unroll
         for (int k = 0; k < 4; k++)
-            mma_16816(s[t], R.q[k][0], R.q[k][1], R.q[k][2], R.q[k][3], w[2 * k], w[2 * k + 1]);
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                mma_16816(s[t0 + t], R.q[k][0], R.q[k][1], R.q[k][2], R.q[k][3], w[t][2 * k], w[t][2 * k + 1]);
     }
     constexpr int NR = TWO ? 2 : 1;
     float kc[2], vc[2], top[2];
