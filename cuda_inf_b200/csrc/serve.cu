@@ -191,6 +191,7 @@ static int check_rows(const void* p, int64_t stride, int heads, const char* what
     do {                                                                                                       \
         REQUIRE((kp8) && (vp8) && (kps) && (vps) && (ktail) && (vtail) && (table), "null pointer");            \
         REQUIRE((n_pages) > 0 && (width) > 0, "n_pages and table_width must be positive");                     \
+        REQUIRE((width) <= 1 << 24, "table_width must be at most 2^24 (positions are 32 bits)");               \
         REQUIRE((((uintptr_t)(kp8) | (uintptr_t)(vp8) | (uintptr_t)(ktail) | (uintptr_t)(vtail)) & 15) == 0,   \
                 "pages and tails must be 16-byte aligned");                                                    \
         REQUIRE((((uintptr_t)(kps) | (uintptr_t)(vps)) & 1) == 0 && ((uintptr_t)(table) & 3) == 0,             \

@@ -23,7 +23,6 @@
 #define FW_UNIT 8192       // bytes of a unit: 4096 of keys, 4096 of values
 #define FW_TAIL 32         // tail tokens of a unit
 #define FW_IDLE (1u << 24) // turns (of 50 clocks and more) without a free stage that end the kernel
-#define FW_THR 3.f         // the reference follows the maximum when it has grown by 2^THR
 
 struct FwSmem {
     uint64_t full[FW_ST], empty[FW_ST], merge, merged;
@@ -260,7 +259,8 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * kc[r];
     }
-    if (__any_sync(0xffffffffu, top[0] > R.m[0] + FW_THR || (TWO && top[NR - 1] > R.m[NR - 1] + FW_THR))) {
+    const float growth = sv_growth(x.vs);
+    if (__any_sync(0xffffffffu, top[0] > R.m[0] + growth || (TWO && top[NR - 1] > R.m[NR - 1] + growth))) {
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             const float mn = fmaxf(R.m[r], top[r]);

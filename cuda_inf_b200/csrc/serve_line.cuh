@@ -8,10 +8,10 @@
 
 // ---- waits (bounded; the first that gives up raises the CTA's abort word, and
 // the kernel's end reports it) ----
-// A try that fails has taken between 90 ns and 4 us, so this many end after 45
-// ms to 2 s.  Counting them keeps the 30 waits of a kernel small: its roles run
+// A try that fails has taken between 90 ns and 4 us, so this many end after
+// 0.2 to 8 s.  Counting them keeps the 30 waits of a kernel small: its roles run
 // side by side from one instruction cache.
-#define SV_TRIES 500000u
+#define SV_TRIES 2000000u
 __device__ __forceinline__ bool sv_wait(uint64_t* bar, uint32_t parity, int* abort_) {
 #pragma unroll 1
     for (uint32_t k = 0; k < SV_TRIES; k++) {
@@ -49,10 +49,16 @@ __device__ __forceinline__ uint32_t sv_e4m3x2(uint32_t two) {  // low 16 bits: t
     asm("{\n .reg .b16 t;\n cvt.u16.u32 t, %1;\n cvt.rn.f16x2.e4m3x2 %0, t;\n}\n" : "=r"(r) : "r"(two));
     return r;
 }
-// FP8: the weights carry the page's value scale times this.  A scale is at most
-// 65504 / 448, so with weights up to 2^3 fp16 still holds them; a usual scale
-// (0.01) keeps weights above 4e-4 in fp16's normal range.
+// The reference that scores are taken from follows a row's maximum when that
+// has grown by more than 2^8 (fp16 holds such weights), so that sums and O are
+// seldom rescaled.
+//
+// FP8: the weights carry the page's value scale times SV_VEXP, so that a usual
+// scale (0.01) keeps weights above 4e-4 in fp16's normal range.  A scale is at
+// most 65504 / 448; from 15.9 on (values above 7000) the limit is 2^3, which
+// keeps scale x 16 x weight below 65504.
 #define SV_VEXP 16.f
+__device__ __forceinline__ float sv_growth(float value_scale) { return value_scale > 15.9f ? 3.f : 8.f; }
 
 // ---- sequences ----
 enum { SV_PACKED = 0, SV_MANY = 1, SV_FEW = 2 };  // packed prompts; paged, many or few rows of a sequence
@@ -166,11 +172,11 @@ static inline SvWs sv_ws(void* p, int ctas, int rows) {
 // of the attention began and did not finish; the other parts are slot 0 of the
 // CTAs behind it.  j < SV_JOIN_Y (with `many`): 32 rows each of the tensor-core
 // kernel's items, else the 16 of the single-token kernel's.  A thread holds 4
-// columns of a row and asks for 8 parts at a time (one after another, 20 parts
+// columns of a row and asks for 4 parts at a time (one after another, 20 parts
 // of a 32768-token context took 29 us).  Fixed order: the same bits every time.
 #define SV_JOIN_Y 8
-#define SV_JOIN 8
-__global__ void __launch_bounds__(256) k_serve_combine(const AttnArgs A, const SvWs Wm, const SvWs Wf, const int n_ctas,
+#define SV_JOIN 4
+__global__ void __launch_bounds__(256, 5) k_serve_combine(const AttnArgs A, const SvWs Wm, const SvWs Wf, const int n_ctas,
                                                        const int many) {
     pdl_wait();
     const bool few = !many || blockIdx.y == SV_JOIN_Y;

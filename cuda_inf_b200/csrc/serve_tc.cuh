@@ -13,7 +13,7 @@
 //                    operand) and written to TMEM
 //   O += P V         tcgen05.mma with P from TMEM, 128 x 64 x 128, fp32 in TMEM
 // The reference m follows the row's maximum only when that has grown by more
-// than 2^THR since, so O is rescaled seldom (P stays within fp16's range).
+// than 2^8 since, so O is rescaled seldom (P stays within fp16's range).
 //
 // A row tile's softmax gives its S back once the scores are in registers, so
 // the next scores come while it works and the kernel runs at the softmax's
@@ -284,7 +284,6 @@ struct SvCfg {
     // registers: 512 x 128 = 256 x 200 + 256 x 56; 384 x 168 = 256 x 208 + 128 x 88
     static constexpr int REG_HI = PAGED ? 200 : 208;
     static constexpr int REG_LO = PAGED ? 56 : 88;
-    static constexpr float THR = PAGED ? 3.f : 8.f;
 };
 
 // ---- paged: pages widened to fp16 tiles by four warps ----
@@ -550,11 +549,13 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 float* s = reinterpret_cast<float*>(sr);
                 sv_ld32(s_addr, sr), sv_ld32(s_addr + 32, sr + 32);
                 float kc[2] = {c2, c2}, vc[2] = {1.f, 1.f};
+                float growth = 8.f;
                 bool masked = i >= first_masked, gone[2] = {false, false};
                 if (PAGED) {
                     const float4 sc = *reinterpret_cast<const float4*>(S->sc[tiles % SV_SC]);
                     kc[0] = c2 * sc.x, kc[1] = c2 * sc.y;
                     vc[0] = SV_VEXP * sc.z, vc[1] = SV_VEXP * sc.w;
+                    growth = sv_growth(fmaxf(sc.z, sc.w));
                     gone[0] = sc.x < 0.f, gone[1] = sc.y < 0.f;
                     masked |= gone[0] | gone[1];
                 }
@@ -596,7 +597,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 }
                 if (i == tb) {
                     m = x;
-                } else if (__any_sync(0xffffffffu, x > m + C::THR)) {
+                } else if (__any_sync(0xffffffffu, x > m + growth)) {
                     // rare: the reference follows the maximum, sum and O with it
                     const float mn = fmaxf(m, x);
                     const float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);

@@ -51,6 +51,9 @@ CASES = [
     (append, dict(kp8=P + 4), b"pages and tails must be"), (append, dict(vtail=P + 8), b"pages and tails must be"),
     (append, dict(kps=P + 1), b"misaligned scales"), (append, dict(vs=8), b"v: 16-byte aligned"),
     (append, dict(nkv=0), HEADS),
+    (append, dict(width=1 << 25), b"table_width"), (paged, dict(width=1 << 25), b"table_width"),
+    (varlen, dict(rows=4096, wb=100), b"workspace"), (varlen, dict(rows=4096, ws=None), b"workspace"),
+    (paged, dict(width=64, wb=100), b"workspace"), (paged, dict(width=64, ws=P + 4), b"workspace"),
     (paged, dict(kv=None), b"null pointer"), (paged, dict(ktail=None), b"null pointer"),
     (paged, dict(max_q=0), b"max_q must be"), (paged, dict(scale=float("inf")), b"scale must be"),
     (paged, dict(nh=12), HEADS), (paged, dict(out=P + 4), b"out must be 16-byte"),

@@ -443,6 +443,78 @@ def test_paged_bad_lengths_are_reported(cuda):
     assert bool((out[1:60] == 5).all()) and not bool((out[0] == 5).any()) and not bool((out[60] == 5).any())
 
 
+def test_pages_of_zeros_and_infinite_scales(cuda):
+    """A page whose scale is 0 beside masked places, and pages with an infinite key or value (their scale is
+    infinite): rows that do not attend them stay as they are."""
+    for chunk in (1, 3, 200):
+        c = Cache(1, 2, 448, cuda)
+        k, v = rnd((300, 2, 64), 3, cuda), rnd((300, 2, 64), 4, cuda)
+        k[64:128] = 0
+        v[192:256] = 0
+        c.append(k, v, [300])
+        q = rnd((chunk, 8, 64), 7, cuda)
+        out = c.attend(q, [chunk], max_q=chunk)
+        c.check(q, [chunk], out)
+        o, tol = plain_rows(q, c.values(0, "k"), c.values(0, "v"), 300 - chunk, 0.125)
+        for x in (k, v):
+            x[200, 1, 5] = INF
+            c.lens = [0]
+            c.append(k, v, [300])
+            got = c.attend(q, [chunk], max_q=chunk)
+            first = max(0, min(chunk, 192 - (300 - chunk)))  # rows before the page
+            # the heads of the other kv head, and (to the bit where the values' scale, which the limit of the weights
+            # goes by, is the same) the rows before the page
+            assert torch.equal(got[:, :4], out[:, :4])
+            assert x is v or torch.equal(got[:first], out[:first])
+            close(got[:first], o[:first], tol[:first])
+            assert bool(got[first:, 4:].isnan().any(-1).all())
+            x[200, 1, 5] = 1.0
+            c.lens = [0]
+
+
+def test_large_values(cuda):
+    """Values up to fp16's largest: the weights carry the scale."""
+    c = Cache(2, 2, 448, cuda)
+    k, v = rnd((700, 2, 64), 3, cuda, 3.0), rnd((700, 2, 64), 4, cuda, 1.0).clamp(-3, 3) * 21000
+    k = k * torch.linspace(0.2, 1.5, 700, device=cuda).half()[:, None, None]
+    c.append(k, v, [350, 350])
+    for new in ([1, 1], [300, 290]):
+        q = rnd((sum(new), 8, 64), 7, cuda)
+        out = c.attend(q, new, max_q=max(new))
+        assert bool(out.isfinite().all())
+        c.check(q, new, out)
+
+
+def test_many_sequences(cuda):
+    """More sequences than a CTA has threads: their line is walked in two passes."""
+    lens = [(37 * i) % 90 for i in range(1300)]
+    t = sum(lens)
+    q, k, v = rnd((t, 4, 64), 1, cuda), rnd((t, 1, 64), 2, cuda), rnd((t, 1, 64), 3, cuda)
+    check_varlen(q, k, v, lens, ops.attn_varlen(q, k, v, cum(lens, cuda)))
+    c = Cache(1300, 1, 128, cuda)
+    c.append(k, v, lens)
+    new = [min(x, 1 + 39 * (i % 7 == 0)) for i, x in enumerate(lens)]
+    q = rnd((sum(new), 4, 64), 7, cuda)
+    c.check(q, new, c.attend(q, new, max_q=max(new)))
+    assert ops.paged_error() == 0
+
+
+def test_workspace_contents_do_not_matter(cuda):
+    c = Cache(3, 2, 4096, cuda)
+    fill(c, [4000, 700, 65], 3)
+    q, k, v = rnd((2000, 8, 64), 1, cuda), rnd((2000, 2, 64), 2, cuda), rnd((2000, 2, 64), 3, cuda)
+    ws = torch.empty(40 << 20, dtype=torch.uint8, device=cuda)
+    want = None
+    for byte in (0, 255, 1):
+        ws.fill_(byte)
+        got = (c.attend(q[:3], [1, 1, 1], max_q=1, workspace=ws), c.attend(q[:500], [400, 90, 10], workspace=ws),
+               ops.attn_varlen(q, k, v, cum([1500, 500], cuda), workspace=ws))
+        want = want or got
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(CuinfError, match="workspace"):
+        ops.attn_varlen(q, k, v, cum([1500, 500], cuda), workspace=ws[:1000])
+
+
 def test_shared_prefix_pages(cuda):
     c = Cache(2, 2, 640, cuda)
     fill(c, [512, 512], 3)
