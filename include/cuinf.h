@@ -178,7 +178,14 @@ int cuinf_moe_ffn(const void* xn, const void* gate, const void* expert_bias,
 /* (kps/vps [n_pages][nkv]); table (device int [n_seqs][table_width]) names    */
 /* the page of each whole 64-token group of a sequence; the tokens behind its  */
 /* last whole group are fp16 in ktail/vtail [n_seqs][nkv][64][64].  Sequences  */
-/* may share pages that are only read (a common prefix).                       */
+/* may share pages that are only read (a common prefix).  table_width is at    */
+/* most 2^24; page scales are never negative (the append makes none).          */
+/*                                                                             */
+/* Rows: a weight is exactly zero where the mask leaves a key out, whatever    */
+/* its key and value hold (infinities and NaN too).  A row that attends a NaN  */
+/* or infinite value, key or query gets results that are no numbers where the  */
+/* formula's are not (an infinity there may become NaN); a row without a key,  */
+/* or whose scores are all minus infinity, is zero.                            */
 /*                                                                             */
 /* All lengths are read on the device; nothing synchronizes, so the calls can  */
 /* be captured into a CUDA graph.  What the device finds wrong there it skips  */
