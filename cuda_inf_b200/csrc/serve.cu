@@ -284,7 +284,7 @@ static cudaLaunchConfig_t pdl_config(dim3 grid, int threads, size_t smem, cudaSt
     return cfg;
 }
 template <bool PAGED>
-static int launch_many(const AttnArgs& A, bool cuts, const SvWs& W, int ctas, cudaStream_t st) {
+static int launch_many(const AttnArgs& A, bool cuts, const SvWs& W, int ctas, bool beside, cudaStream_t st) {
     CUtensorMap qm, km, vm;
     const int G = A.nh / A.nkv;
     if (int rc = rows_map(&qm, A.q, A.q_stride, A.nh, A.rows.n_rows, G, 128 / G)) return rc;
@@ -295,23 +295,26 @@ static int launch_many(const AttnArgs& A, bool cuts, const SvWs& W, int ctas, cu
     }
     CUINF_TRY(cudaFuncSetAttribute(k_serve_attn<PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    (int)SV_SMEM_BYTES));
-    k_serve_attn<PAGED><<<ctas, SvCfg<PAGED>::WARPS * 32, SV_SMEM_BYTES, st>>>(qm, km, vm, A, cuts, W);
+    k_serve_attn<PAGED><<<ctas, SvCfg<PAGED>::WARPS * 32, SV_SMEM_BYTES, st>>>(qm, km, vm, A, cuts, beside, W);
     return cuinf_launch_status();
 }
-// `beside`: a chunks' kernel of the same call runs before (its results do not matter to this one)
+// `beside`: the chunks' kernel of the same call is launched before and runs beside this one (neither reads the other's
+// results)
 static int launch_few(const AttnArgs& A, bool cuts, const SvWs& W, int ctas, bool beside, cudaStream_t st) {
-    CUINF_TRY(cudaFuncSetAttribute(k_serve_few, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FW_SMEM_BYTES));
+    auto* kernel = beside ? k_serve_few<true> : k_serve_few<false>;
+    CUINF_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FW_SMEM_BYTES));
     cudaLaunchAttribute attr[1];
     cudaLaunchConfig_t cfg = pdl_config(dim3(ctas), (FW_WARPS + 1) * 32, FW_SMEM_BYTES, st, attr);
     cfg.numAttrs = beside ? 1 : 0;
-    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_few, A, (int)cuts, W));
+    CUINF_TRY(cudaLaunchKernelEx(&cfg, kernel, A, (int)cuts, W));
     return cuinf_launch_status();
 }
 static int launch_combine(const AttnArgs& A, const SvWs& Wm, const SvWs& Wf, int ctas, bool many, bool few,
                           cudaStream_t st) {
     cudaLaunchAttribute attr[1];
     const cudaLaunchConfig_t cfg = pdl_config(dim3(ctas, (many ? SV_JOIN_Y : 0) + (few ? 1 : 0)), 256, 0, st, attr);
-    CUINF_TRY(cudaLaunchKernelEx(&cfg, k_serve_combine, A, Wm, Wf, ctas, (int)many));
+    auto* kernel = !few ? k_serve_combine<true, false> : many ? k_serve_combine<true, true> : k_serve_combine<false, true>;
+    CUINF_TRY(cudaLaunchKernelEx(&cfg, kernel, A, Wm, Wf, ctas));
     return cuinf_launch_status();
 }
 
@@ -342,7 +345,7 @@ extern "C" int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k,
     int ctas;
     if (int rc = num_ctas(&ctas)) return rc;
     const SvWs W = sv_ws(workspace, ctas, 256);
-    if (int rc = launch_many<false>(A, cuts, W, ctas, ST(stream))) return rc;
+    if (int rc = launch_many<false>(A, cuts, W, ctas, false, ST(stream))) return rc;
     return cuts ? launch_combine(A, W, W, ctas, true, false, ST(stream)) : CUINF_OK;
 }
 
@@ -387,7 +390,7 @@ extern "C" int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_s
     const SvWs Wm = sv_ws(workspace, ctas, 256);
     const SvWs Wf = sv_ws((char*)workspace + (many && cuts ? sv_ws_bytes(ctas, 256) : 0), ctas, 16);
     if (many)
-        if (int rc = launch_many<true>(A, cuts, Wm, ctas, ST(stream))) return rc;
+        if (int rc = launch_many<true>(A, cuts, Wm, ctas, few, ST(stream))) return rc;
     if (few)
         if (int rc = launch_few(A, cuts, Wf, ctas, many, ST(stream))) return rc;
     return cuts ? launch_combine(A, Wm, Wf, ctas, many, few, ST(stream)) : CUINF_OK;

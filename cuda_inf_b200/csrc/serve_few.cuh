@@ -30,7 +30,6 @@
 #define FW_WARPS 11        // and one that copies: 3 a scheduler, at up to 168 registers a thread
 #define FW_ST 22           // stages; a multiple of FW_WARPS: a stage's phases are all seen by one warp
 #define FW_UNIT 8192       // bytes of a unit: 4096 of keys, 4096 of values
-#define FW_TAIL 32         // tail tokens of a unit
 #define FW_IDLE (1u << 24) // turns (of 50 clocks and more) without a free stage that end the kernel
 
 struct FwSmem {
@@ -46,10 +45,6 @@ struct FwSmem {
 };
 static constexpr size_t FW_SMEM_BYTES = 128 + (size_t)FW_ST * FW_UNIT + sizeof(FwSmem);
 
-// units of one kv head (at least one: rows without a key still become zero)
-__device__ __forceinline__ int fw_units(const SvSeq& q) {
-    return max(1, q.kv / SERVE_PAGE + (q.kv % SERVE_PAGE + FW_TAIL - 1) / FW_TAIL);
-}
 // A place on the line: unit u of the n of (sequence s, kv head h).  Kept by
 // steps (a 64-bit division per unit and lane: 83 us for 78).
 struct FwPos {
@@ -84,6 +79,7 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
     if (lane >= FW_ST) return;
     const int cnt = S->left;
     FwPos p, np;  // the unit to copy; the one after it (FW_ST further on)
+    int npage = -2;
     fw_first(A, S->share, p);
     fw_skip(A, p, lane);
     int page = lane < cnt ? fw_page(A, p) : -2;
@@ -95,9 +91,6 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
     };
     __half ks, vs;
     scales(p, page, ks, vs);
-    np = p;
-    if (lane + FW_ST < cnt) fw_skip(A, np, FW_ST);
-    int npage = lane + FW_ST < cnt ? fw_page(A, np) : -2;
     uint32_t k = 0;      // copies of this lane so far
     bool armed = false;  // copies of the last one are in flight
     int j = lane;
@@ -116,30 +109,39 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
         if (!go) continue;
         unsigned char* dst = ring + (size_t)lane * FW_UNIT;
         const int u = p.u, h = p.h, ng = p.q.kv / SERVE_PAGE;
-        S->sc[lane][0] = __half2float(ks), S->sc[lane][1] = __half2float(vs);
+        auto put = [&] { S->sc[lane][0] = __half2float(ks), S->sc[lane][1] = __half2float(vs); };
         armed = true;
         if (page == -2) {
             const int first = (u - ng) * FW_TAIL, rows = min(FW_TAIL, p.q.kv % SERVE_PAGE - first);
             if (rows > 0) {
                 const size_t at = ((size_t)p.s * A.nkv + h) * SERVE_PAGE_HEAD + (size_t)first * CUINF_HD;
+                put();
                 mbar_arrive_expect_tx(&S->full[lane], 2 * rows * CUINF_HD * 2);
                 tma_load_1d(dst, A.kv.ktail + at, rows * CUINF_HD * 2, &S->full[lane]);
                 tma_load_1d(dst + FW_UNIT / 2, A.kv.vtail + at, rows * CUINF_HD * 2, &S->full[lane]);
             } else {
+                put();
                 mbar_arrive(&S->full[lane]);
             }
         } else if (page >= 0 && page < A.kv.n_pages) {
             const size_t at = ((size_t)page * A.nkv + h) * SERVE_PAGE_HEAD;
-            mbar_arrive_expect_tx(&S->full[lane], FW_UNIT);
+            mbar_expect_tx(&S->full[lane], FW_UNIT);
             tma_load_1d(dst, A.kv.kp8 + at, FW_UNIT / 2, &S->full[lane]);
             tma_load_1d(dst + FW_UNIT / 2, A.kv.vp8 + at, FW_UNIT / 2, &S->full[lane]);
+            put();  // (the first copies do not wait for their scales)
+            mbar_arrive(&S->full[lane]);
         } else {
             atomicOr(A.err, SERVE_ERR_PAGE);
-            S->sc[lane][0] = -1.f;
+            S->sc[lane][0] = -1.f, S->sc[lane][1] = 1.f;
             mbar_arrive(&S->full[lane]);
         }
-        p = np, page = npage;
+        if (k == 0 && j + FW_ST < cnt) {  // (nor for the place of the second)
+            np = p;
+            fw_skip(A, np, FW_ST);
+            npage = fw_page(A, np);
+        }
         if (j + FW_ST < cnt) {
+            p = np, page = npage;
             scales(p, page, ks, vs);
             if (j + 2 * FW_ST < cnt) {
                 fw_skip(A, np, FW_ST);
@@ -327,6 +329,7 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
     }
 }
 
+template <bool BESIDE>  // (a kernel of its own: with the sums' code one token at 32768 took 20.1 us, without 19.7)
 __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
     k_serve_few(const AttnArgs A, const int split, const SvWs W) {
     extern __shared__ __align__(128) unsigned char fw_raw[];
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
     }
     for (int i = tid; i < 9 * CUINF_HD; i += blockDim.x) (&S->bad[0][0][0])[i] = 0x7fffffff;
     if (split && tid < 2) W.part[blockIdx.x * 2 + tid].valid = 0;
-    sv_share<SV_FEW>(A, &S->share, blockIdx.x, gridDim.x, [&](const SvSeq& q) { return (long long)fw_units(q) * A.nkv; });
+    sv_share<SV_FEW>(A, &S->share, blockIdx.x, gridDim.x, BESIDE, [&](const SvSeq& q) { return (long long)fw_units(q) * A.nkv; });
     if (tid == 0) {
         long long left = S->share.left;
         if (!split && left > 0) {

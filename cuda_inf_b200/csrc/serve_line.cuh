@@ -26,6 +26,9 @@ __device__ __forceinline__ bool sv_wait(uint64_t* bar, uint32_t parity, int* abo
 __device__ __forceinline__ bool sv_wait_all(uint64_t* bar, uint32_t parity, int* abort_) {
     return __all_sync(0xffffffffu, sv_wait(bar, parity, abort_));
 }
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 // Before the CTA ends: a phase that copies or products in flight complete.
 __device__ __forceinline__ void sv_drain(uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
@@ -89,41 +92,92 @@ __device__ __forceinline__ bool sv_seq(const AttnArgs& A, int s, SvSeq& q, bool 
     return q.c > 0;
 }
 
+// Many rows: the line's unit is a key, and an item (a block of tq rows of one
+// kv head) takes
+// the keys of its last row and SV_OVH more for its beginning and end, so the
+// blocks of a sequence form an arithmetic series and a place on the line is
+// found without a table.  Cuts fall on key tiles (sv_cut).
+#define SV_OVH 256
+__device__ __forceinline__ int sv_keys(const SvSeq& q, int end) {  // rows before `end`; a row without a key still
+    return max(1, q.p0 + end);                                     // has its zeros written
+}
+// units of the first k blocks of a head (none of them the last)
+__device__ __forceinline__ long long sv_prefix(const SvSeq& q, int tq, int k) {
+    const int z = q.p0 < 0 ? min(k, -q.p0 / tq) : 0;  // blocks without a key
+    return (long long)k * SV_OVH + z + (long long)(k - z) * q.p0 +
+           (long long)tq * (((long long)k * (k + 1) - (long long)z * (z + 1)) / 2);
+}
+__device__ __forceinline__ long long sv_head_units(const SvSeq& q, int tq) {
+    return sv_prefix(q, tq, (q.c + tq - 1) / tq - 1) + sv_keys(q, q.c) + SV_OVH;
+}
+#define FW_TAIL 32  // tail tokens of a unit
+// Few rows: units of one kv head (at least one: rows without a key still become zero)
+__device__ __forceinline__ int fw_units(const SvSeq& q) {
+    return max(1, q.kv / SERVE_PAGE + (q.kv % SERVE_PAGE + FW_TAIL - 1) / FW_TAIL);
+}
+
 // The CTA's share of the line (equal parts, to a unit).
 struct SvShare {
     int s;           // sequence in which it begins
     long long rem;   // units of that sequence before it
     long long left;  // its units (0: nothing to do)
     long long scan[32];
+    long long work[32][2];
 };
+// Where a call's sequences are of both kinds, the two kernels run beside one
+// another, each on a part of the SMs that follows its work (`beside`), and the
+// CTAs behind that end at once: the single tokens' kernel is bound by memory and
+// latencies, the chunks' by the softmax.  128 single tokens at contexts to 4096
+// beside a chunk of 64 tokens take 107 us (one kernel after the other: 130), 24
+// beside a chunk of 515 80 (86).  In keys of the chunks' kernel a unit of the
+// other takes SV_FEW_COST and an item's end SV_FEW_END units (8 instead of 14:
+// 109 and 99 us; 12: 105 and 82; 18: 120 and 85).
+#define SV_FEW_COST 14
+#define SV_FEW_END 11
 // All threads call; `units` gives a sequence's units.  One pass over the
 // sequences where the CTA has a thread for each, else one for the sum and one
 // for the place.
 template <int KIND, class F>
-__device__ __forceinline__ void sv_share(const AttnArgs& A, SvShare* S, int cta, int n_ctas, F units) {
+__device__ __forceinline__ void sv_share(const AttnArgs& A, SvShare* S, int cta, int n_ctas, int beside, F units) {
+    constexpr int OTHER = KIND == SV_FEW ? SV_MANY : SV_FEW;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nt = blockDim.x, nw = nt >> 5, n = A.rows.n_seqs;
-    long long total = 0, beg = 0, end = 0, base = 0;
+    auto cost = [&](int kind, const SvSeq& q) {  // of one kv head
+        return kind == SV_FEW ? (long long)(fw_units(q) + SV_FEW_END) * SV_FEW_COST
+                              : sv_head_units(q, 2 * (128 / (A.nh / A.nkv)));
+    };
+    long long total = 0, beg = 0, end = 0, base = 0, mine = 0, other = 0;
     if (tid == 0) S->left = 0;
     for (int pass = n <= nt ? 1 : 0; pass < 2; pass++) {
+        const bool sum = pass == 0 || n <= nt;
         for (int b = 0; b < n; b += nt) {
             const int s = b + tid;
             SvSeq q;
-            long long w = 0;
-            if (s < n && sv_seq<KIND>(A, s, q, (pass == 0 || n <= nt) && cta == 0)) w = units(q);
-            long long x = w;
+            long long w = 0, x, work[2] = {0, 0};
+            if (s < n && sv_seq<KIND>(A, s, q, sum && cta == 0)) w = units(q);
+            if (beside && sum) {
+                if (w)
+                    work[0] = cost(KIND, q);
+                else if (s < n && sv_seq<OTHER>(A, s, q, false))
+                    work[1] = cost(OTHER, q);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1)
+                    for (int k = 0; k < 2; k++) work[k] += __shfl_xor_sync(0xffffffffu, work[k], o);
+            }
+            x = w;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
                 const long long y = __shfl_up_sync(0xffffffffu, x, o);
                 if (lane >= o) x += y;
             }
             if (b > 0 || pass == 1) __syncthreads();
-            if (lane == 31) S->scan[warp] = x;
+            if (lane == 31) S->scan[warp] = x, S->work[warp][0] = work[0], S->work[warp][1] = work[1];
             __syncthreads();
             long long before = 0, all = 0;
             for (int i = 0; i < nw; i++) {
                 const long long y = S->scan[i];
                 if (i < warp) before += y;
                 all += y;
+                if (beside && sum) mine += S->work[i][0], other += S->work[i][1];
             }
             if (pass == 0) {
                 total += all;
@@ -131,6 +185,11 @@ __device__ __forceinline__ void sv_share(const AttnArgs& A, SvShare* S, int cta,
             }
             if (n <= nt) total = all;
             if (b == 0) {
+                if (mine > 0 && other > 0) {  // the single tokens' CTAs: the same number in both kernels
+                    const float f = (float)(KIND == SV_FEW ? mine : other) / (float)(mine + other);
+                    const int few = min(max(1, (int)(f * n_ctas + 0.5f)), n_ctas - 1);
+                    n_ctas = KIND == SV_FEW ? few : n_ctas - few;
+                }
                 const long long per = total / n_ctas, more = total - per * n_ctas;
                 beg = per * cta + min((long long)cta, more);
                 end = beg + per + (cta < more);
@@ -171,48 +230,60 @@ static inline SvWs sv_ws(void* p, int ctas, int rows) {
 // Joins the items that were cut: CTA (i, j) takes rows of the item that CTA i
 // of the attention began and did not finish; the other parts are slot 0 of the
 // CTAs behind it.  j < SV_JOIN_Y (with `many`): 32 rows each of the tensor-core
-// kernel's items, else the 16 of the single-token kernel's.  A thread holds 4
-// columns of a row and asks for 4 parts at a time (one after another, 20 parts
-// of a 32768-token context took 29 us; 8 at a time leave fewer CTAs on an SM,
-// and 12 prompts of up to 1500 tokens take 115 us for 112).  Fixed order: the
-// same bits every time.
+// kernel's items, else the up to 16 of the single-token kernel's.  A thread
+// holds 4 columns of a row and asks for SV_JOIN parts at a time, whether they
+// are there or not (an empty share's slot is read and left out: asking first
+// would double the time): 4, for 8 leave fewer CTAs on an SM (12 prompts of up to
+// 1500 tokens: 115 us for 112), or 8 in a decode step, with one CTA an SM.
+// Where the rows are few and the parts many, up to 256 /
+// (16 rows) neighbouring threads share the parts of one place.  The time is that of dependent loads:
+// one part after another, the 20 parts of a 32768-token context took 29 us in
+// all, shared out 20.  Fixed order: the same bits every time.
 #define SV_JOIN_Y 8
-#define SV_JOIN 4
-__global__ void __launch_bounds__(256, 5) k_serve_combine(const AttnArgs A, const SvWs Wm, const SvWs Wf, const int n_ctas,
-                                                       const int many) {
+template <bool MANY, bool FEW>
+__global__ void __launch_bounds__(256, !MANY ? 1 : FEW ? 4 : 5)
+    k_serve_combine(const AttnArgs A, const SvWs Wm, const SvWs Wf, const int n_ctas) {
+    constexpr int SV_JOIN = MANY ? 4 : 8;
     pdl_wait();
-    const bool few = !many || blockIdx.y == SV_JOIN_Y;
+    const bool few = FEW && (!MANY || blockIdx.y == SV_JOIN_Y);
     const SvWs& W = few ? Wf : Wm;
     const int rows = few ? 16 : 256, i = blockIdx.x, lane = threadIdx.x & 31;
+    auto last = [&](int k) {  // CTA k's first slot ends its item
+        if (k >= n_ctas) return false;
+        const int2 x = *reinterpret_cast<const int2*>(W.part + (size_t)k * 2);
+        return x.x && x.y;
+    };
     const SvPart p = W.part[i * 2 + 1];
+    bool hit = last(i + 1 + lane);
     if (!p.valid) return;
-    int end = n_ctas;  // the item's last part is CTA end - 1's
-    for (int k = i + 1; k < n_ctas; k += 32) {
-        const int at = k + lane;
-        const SvPart* q = W.part + (size_t)at * 2;
-        const unsigned hit = __ballot_sync(0xffffffffu, at < n_ctas && q->valid && q->last);
-        if (hit) {
-            end = k + __ffs(hit);
-            break;
-        }
-    }
-    const int G = A.nh / A.nkv, TOK = 128 / G, c = (threadIdx.x & 15) * 4;
-    for (int r = (few ? 0 : blockIdx.y * 32) + (threadIdx.x >> 4), z = 0; z < (few ? 1 : 2); z++, r += 16) {
+    int k = i + 1;
+    unsigned hits;
+    while (!(hits = __ballot_sync(0xffffffffu, hit)) && (k += 32) < n_ctas) hit = last(k + lane);
+    const int end = hits ? k + __ffs(hits) : n_ctas;  // the item's last part is CTA end - 1's
+    const int G = A.nh / A.nkv, TOK = 128 / G;
+    int lg = 0;  // 2^lg threads share a place's parts
+    if (few)
+        while (lg < 4 && SV_JOIN << lg < end - i && p.tokens * G << lg <= 8) lg++;
+    const int at = threadIdx.x >> lg, c = (at & 15) * 4, part0 = threadIdx.x & ((1 << lg) - 1);
+    for (int r = (few ? 0 : blockIdx.y * 32) + (at >> 4), z = 0; z < (few ? 1 : 2); z++, r += 16) {
         const int row = r & 127, tok = (r >> 7) * TOK + row / G;
-        if (row >= TOK * G || tok >= p.tokens) continue;
+        const bool live = row < TOK * G && tok < p.tokens;
         float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = i; k0 < end; k0 += SV_JOIN) {
+        for (int k0 = i + part0; k0 < end; k0 += SV_JOIN << lg) {
             float2 ml[SV_JOIN];
             float4 x[SV_JOIN];
 #pragma unroll
             for (int j = 0; j < SV_JOIN; j++) {
-                const int k = k0 + j;
+                const int k = k0 + (j << lg);
                 const size_t slot = (size_t)k * 2 + (k == i);
-                // (an empty share's slot holds nothing)
-                const bool there = k < end && (k == i || W.part[slot].valid);
-                ml[j] = there ? reinterpret_cast<const float2*>(W.ml)[slot * rows + r] : make_float2(-INFINITY, 0.f);
-                x[j] = there ? *reinterpret_cast<const float4*>(W.o + (slot * rows + r) * CUINF_HD + c)
-                             : make_float4(0.f, 0.f, 0.f, 0.f);
+                int valid = 0;
+                ml[j] = make_float2(-INFINITY, 0.f), x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (live && k < end) {
+                    valid = W.part[slot].valid;
+                    ml[j] = reinterpret_cast<const float2*>(W.ml)[slot * rows + r];
+                    x[j] = *reinterpret_cast<const float4*>(W.o + (slot * rows + r) * CUINF_HD + c);
+                }
+                if (!valid) ml[j] = make_float2(-INFINITY, 0.f), x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             float mn = m;
 #pragma unroll
@@ -228,6 +299,15 @@ __global__ void __launch_bounds__(256, 5) k_serve_combine(const AttnArgs A, cons
                 o[0] += x[j].x * f, o[1] += x[j].y * f, o[2] += x[j].z * f, o[3] += x[j].w * f;
             }
         }
+        for (int t = 1; t < 1 << lg; t *= 2) {
+            const float m2 = __shfl_xor_sync(0xffffffffu, m, t), mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+            const float f = m == -INFINITY ? 0.f : sv_exp2(m - ref), f2 = m2 == -INFINITY ? 0.f : sv_exp2(m2 - ref);
+            l = l * f + __shfl_xor_sync(0xffffffffu, l, t) * f2;  // (0 * NaN: NaN)
+#pragma unroll
+            for (int d = 0; d < 4; d++) o[d] = o[d] * f + __shfl_xor_sync(0xffffffffu, o[d], t) * f2;
+            m = mn;
+        }
+        if (!live || part0) continue;
         const float inv = l == 0.f ? 0.f : 1.f / l;
         *reinterpret_cast<uint2*>(A.out + ((size_t)(p.row0 + tok) * A.nh + p.h * G + row % G) * CUINF_HD + c) =
             make_uint2(sv_pack_h2(o[0] * inv, o[1] * inv), sv_pack_h2(o[2] * inv, o[3] * inv));

@@ -178,23 +178,7 @@ __device__ __forceinline__ void sv_tma_3d(void* dst, const CUtensorMap* map, int
 // ---------------------------------------------------------------------------
 // the line of key tiles
 // ---------------------------------------------------------------------------
-// The line's unit is a key: an item (a block of tq rows of one kv head) takes
-// the keys of its last row and SV_OVH more for its beginning and end, so the
-// blocks of a sequence form an arithmetic series and a place on the line is
-// found without a table.  Cuts fall on key tiles (sv_cut).
-#define SV_OVH 256
-__device__ __forceinline__ int sv_keys(const SvSeq& q, int end) {  // rows before `end`; a row without a key still
-    return max(1, q.p0 + end);                                     // has its zeros written
-}
-// units of the first k blocks of a head (none of them the last)
-__device__ __forceinline__ long long sv_prefix(const SvSeq& q, int tq, int k) {
-    const int z = q.p0 < 0 ? min(k, -q.p0 / tq) : 0;  // blocks without a key
-    return (long long)k * SV_OVH + z + (long long)(k - z) * q.p0 +
-           (long long)tq * (((long long)k * (k + 1) - (long long)z * (z + 1)) / 2);
-}
-__device__ __forceinline__ long long sv_head_units(const SvSeq& q, int tq) {
-    return sv_prefix(q, tq, (q.c + tq - 1) / tq - 1) + sv_keys(q, q.c) + SV_OVH;
-}
+// (its unit is a key; see sv_head_units)
 // first key tile of a part that begins x units into an item of n tiles and u units
 __device__ __forceinline__ int sv_cut(long long x, int u, int n) {
     return x >= u ? n : min(n, (int)max(0ll, x - SV_OVH + SV_KT / 2) / SV_KT);
@@ -202,8 +186,8 @@ __device__ __forceinline__ int sv_cut(long long x, int u, int n) {
 
 // The CTA's share and the item in which it begins (all threads call).
 template <int KIND>
-__device__ void sv_start(const AttnArgs& A, SvSmem* S, int tq, int n_ctas) {
-    sv_share<KIND>(A, &S->share, blockIdx.x, n_ctas,
+__device__ void sv_start(const AttnArgs& A, SvSmem* S, int tq, int n_ctas, int beside) {
+    sv_share<KIND>(A, &S->share, blockIdx.x, n_ctas, beside,
                    [&](const SvSeq& q) { return sv_head_units(q, tq) * A.nkv; });
     if (threadIdx.x == 0 && S->share.left > 0) {
         SvSeq q;
@@ -472,7 +456,8 @@ __device__ __forceinline__ bool sv_pages(const AttnArgs& A, SvSmem* S, const SvI
 template <bool PAGED>
 __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
     k_serve_attn(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap kmap,
-                 const __grid_constant__ CUtensorMap vmap, const AttnArgs A, const int split, const SvWs W) {
+                 const __grid_constant__ CUtensorMap vmap, const AttnArgs A, const int split, const int beside,
+                 const SvWs W) {
     using C = SvCfg<PAGED>;
     extern __shared__ __align__(1024) unsigned char sv_raw[];
     unsigned char* sm = sv_raw + ((1024 - (smem_u32(sv_raw) & 1023)) & 1023);
@@ -513,7 +498,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
     }
     if (split && tid < 2) W.part[blockIdx.x * 2 + tid].valid = 0;
-    sv_start<C::KIND>(A, S, tq, gridDim.x);
+    sv_start<C::KIND>(A, S, tq, gridDim.x, PAGED && beside);
     sv_fence_before();
     __syncthreads();
     sv_fence_after();
