@@ -18,8 +18,8 @@
 // the scores, its value scale the weights (one rounding of a weight to fp16).
 //
 // Measured on B200, 8 kv heads of 4 query heads, one token each: 64 contexts of
-// 2048 tokens 42 us and of 4096 63 us (269 MB, 4.3 TB/s), 64 of 128 to 8191
-// tokens 128 us (554 MB, 4.3 TB/s); one of 32768 23 us (33.6 MB).  From 2048
+// 2048 tokens 42 us and of 4096 64 us (269 MB, 4.2 TB/s), 128 of up to 8191
+// tokens 129 us (554 MB, 4.3 TB/s); one of 32768 20 us (33.6 MB).  From 2048
 // to 4096 tokens the added bytes go at 6.5 TB/s, the copy rate: the rest is a
 // part per call (the launch, the line, the first pages' latency, the join) and
 // per item (the warps' join).  8 warps took 56 us for the first, 11 (what the

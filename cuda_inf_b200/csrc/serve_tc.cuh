@@ -23,7 +23,7 @@
 // query and 8 kv heads: one prompt of 16384 tokens 1.286 ms, 855 TFLOP/s of
 // the 1648 that a library matrix product reaches (the exponentials' bound is
 // 1150 at 1.9 GHz); 12 prompts of up to 1500 tokens 112 us; over pages, 4 chunks of 1024 tokens
-// behind 8192: 482 us, 604 TFLOP/s.  At 4096 tokens the exponential unit is
+// behind 8192: 474 us, 615 TFLOP/s.  At 4096 tokens the exponential unit is
 // busy 60 % and the tensor pipe 30 % of the time, and the 8 softmax warps
 // issue on 41 % of the clocks: two warps a scheduler do not hide the TMEM
 // loads' and each other's latencies.  Replacing exponentials by polynomials on

@@ -499,6 +499,37 @@ def test_many_sequences(cuda):
     assert ops.paged_error() == 0
 
 
+@pytest.mark.parametrize("nh,nkv,new", [(1, 1, 1), (2, 1, 1), (3, 1, 1), (5, 1, 1), (4, 1, 2), (4, 1, 4), (8, 8, 9)])
+def test_long_context_joined_from_many_parts(cuda, nh, nkv, new):
+    """One sequence over all SMs: 1 to 16 rows, whose parts 1 to 16 threads share."""
+    c = Cache(1, nkv, 20000, cuda)
+    fill(c, [19990], 3)
+    q = rnd((new, nh, 64), 7, cuda, 2.0)
+    out = c.attend(q, [new], max_q=new)
+    c.check(q, [new], out)
+    assert torch.equal(out, c.attend(q, [new], max_q=new))
+
+
+@pytest.mark.parametrize("lens,new", [
+    ([6000] + [300] * 5, [1] + [200] * 5),
+    ([3000] * 40 + [70], [1] * 40 + [17]),
+    ([64, 5000], [1, 900]),
+    ([63, 130, 200, 255], [1, 130, 3, 60]),
+    ([1, 4000, 1], [1, 1, 1]),
+    ([2000, 0, 1500], [700, 0, 1500]),
+])
+def test_chunks_beside_single_tokens(cuda, lens, new):
+    """Both kernels at once, each on its part of the SMs, whatever the work's ratio."""
+    c = Cache(len(lens), 2, max(lens), cuda)
+    fill(c, lens, 5)
+    q = rnd((sum(new), 8, 64), 7, cuda)
+    out = c.attend(q, new)
+    c.check(q, new, out)
+    for _ in range(3):
+        assert torch.equal(out, c.attend(q, new))
+    assert ops.paged_error() == 0
+
+
 def test_workspace_contents_do_not_matter(cuda):
     c = Cache(3, 2, 4096, cuda)
     fill(c, [4000, 700, 65], 3)
