@@ -253,8 +253,6 @@ static int rows_map(CUtensorMap* m, const __half* base, int64_t stride, int head
     return CUINF_OK;
 }
 
-// One CTA per SM, at most this many: the workspace holds two partial results of each.
-#define SERVE_MAX_CTAS 148
 // Items of at most this many key tiles are not cut.
 #define SERVE_WHOLE_TILES 4
 static bool sv_cuts(long long most_keys) { return most_keys > SERVE_WHOLE_TILES * SV_KT; }

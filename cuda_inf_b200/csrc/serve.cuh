@@ -23,6 +23,8 @@ struct PagedKV {
     int width, n_pages, nkv;
 };
 
+// One CTA per SM, at most this many: the workspace holds two partial results of each.
+#define SERVE_MAX_CTAS 148
 // Paged: sequences of at most this many rows (new tokens x query heads per kv
 // head) go to the single-token kernel, longer ones to the tensor-core kernel.
 #define SERVE_FEW_ROWS 16

@@ -231,59 +231,66 @@ static inline SvWs sv_ws(void* p, int ctas, int rows) {
 // of the attention began and did not finish; the other parts are slot 0 of the
 // CTAs behind it.  j < SV_JOIN_Y (with `many`): 32 rows each of the tensor-core
 // kernel's items, else the up to 16 of the single-token kernel's.  A thread
-// holds 4 columns of a row and asks for SV_JOIN parts at a time, whether they
-// are there or not (an empty share's slot is read and left out: asking first
-// would double the time): 4, for 8 leave fewer CTAs on an SM (12 prompts of up to
-// 1500 tokens: 115 us for 112), or 8 in a decode step, with one CTA an SM.
-// Where the rows are few and the parts many, up to 256 /
-// (16 rows) neighbouring threads share the parts of one place.  The time is that of dependent loads:
-// one part after another, the 20 parts of a 32768-token context took 29 us in
-// all, shared out 20.  Fixed order: the same bits every time.
+// holds 4 columns of a row and asks for SV_JOIN parts at a time: 3 or 4, for 8
+// leave fewer CTAs on an SM (12 prompts of up to 1500 tokens: 115 us for 112.5),
+// or 8 in a decode step, with one CTA an SM.  Where the rows are few and the parts many,
+// up to 256 / (16 rows) neighbouring threads share the parts of one place.  The
+// time is that of dependent loads: one part after another, the 20 parts of a
+// 32768-token context took 29 us in all, shared out 20.  Fixed order: the same
+// bits every time.
 #define SV_JOIN_Y 8
 template <bool MANY, bool FEW>
 __global__ void __launch_bounds__(256, !MANY ? 1 : FEW ? 4 : 5)
     k_serve_combine(const AttnArgs A, const SvWs Wm, const SvWs Wf, const int n_ctas) {
-    constexpr int SV_JOIN = MANY ? 4 : 8;
+    constexpr int SV_JOIN = !MANY ? 8 : FEW ? 4 : 3;
     pdl_wait();
     const bool few = FEW && (!MANY || blockIdx.y == SV_JOIN_Y);
     const SvWs& W = few ? Wf : Wm;
     const int rows = few ? 16 : 256, i = blockIdx.x, lane = threadIdx.x & 31;
-    auto last = [&](int k) {  // CTA k's first slot ends its item
-        if (k >= n_ctas) return false;
-        const int2 x = *reinterpret_cast<const int2*>(W.part + (size_t)k * 2);
-        return x.x && x.y;
+    __shared__ unsigned char list[SERVE_MAX_CTAS];  // the CTAs that hold a part of the item (a share can be empty)
+    __shared__ int n_parts;
+    auto flags = [&](int k) {  // of CTA k's first slot: there, the item's last
+        return k < n_ctas ? *reinterpret_cast<const int2*>(W.part + (size_t)k * 2) : make_int2(0, 0);
     };
     const SvPart p = W.part[i * 2 + 1];
-    bool hit = last(i + 1 + lane);
+    int2 x = flags(i + 1 + lane);
     if (!p.valid) return;
-    int k = i + 1;
-    unsigned hits;
-    while (!(hits = __ballot_sync(0xffffffffu, hit)) && (k += 32) < n_ctas) hit = last(k + lane);
-    const int end = hits ? k + __ffs(hits) : n_ctas;  // the item's last part is CTA end - 1's
+    if (threadIdx.x < 32) {
+        int cnt = 1;
+        if (lane == 0) list[0] = i;
+        for (int k = i + 1;;) {
+            const unsigned last = __ballot_sync(0xffffffffu, x.x && x.y);
+            const unsigned there = __ballot_sync(0xffffffffu, x.x) & (last ^ (last - 1));  // up to the last (none: all)
+            if (there >> lane & 1) list[cnt + __popc(there & ((1u << lane) - 1))] = k + lane;
+            cnt += __popc(there);
+            if (last || (k += 32) >= n_ctas) break;
+            x = flags(k + lane);
+        }
+        if (lane == 0) n_parts = cnt;
+    }
+    __syncthreads();
+    const int parts = n_parts;
     const int G = A.nh / A.nkv, TOK = 128 / G;
     int lg = 0;  // 2^lg threads share a place's parts
     if (few)
-        while (lg < 4 && SV_JOIN << lg < end - i && p.tokens * G << lg <= 8) lg++;
+        while (lg < 4 && SV_JOIN << lg < parts && p.tokens * G << lg <= 8) lg++;
     const int at = threadIdx.x >> lg, c = (at & 15) * 4, part0 = threadIdx.x & ((1 << lg) - 1);
     for (int r = (few ? 0 : blockIdx.y * 32) + (at >> 4), z = 0; z < (few ? 1 : 2); z++, r += 16) {
         const int row = r & 127, tok = (r >> 7) * TOK + row / G;
         const bool live = row < TOK * G && tok < p.tokens;
         float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int k0 = i + part0; k0 < end; k0 += SV_JOIN << lg) {
+        for (int k0 = part0; k0 < parts; k0 += SV_JOIN << lg) {
             float2 ml[SV_JOIN];
             float4 x[SV_JOIN];
 #pragma unroll
             for (int j = 0; j < SV_JOIN; j++) {
                 const int k = k0 + (j << lg);
-                const size_t slot = (size_t)k * 2 + (k == i);
-                int valid = 0;
                 ml[j] = make_float2(-INFINITY, 0.f), x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (live && k < end) {
-                    valid = W.part[slot].valid;
+                if (live && k < parts) {
+                    const size_t slot = (size_t)list[k] * 2 + (k == 0);
                     ml[j] = reinterpret_cast<const float2*>(W.ml)[slot * rows + r];
                     x[j] = *reinterpret_cast<const float4*>(W.o + (slot * rows + r) * CUINF_HD + c);
                 }
-                if (!valid) ml[j] = make_float2(-INFINITY, 0.f), x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
             }
             float mn = m;
 #pragma unroll
