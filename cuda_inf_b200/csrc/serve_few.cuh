@@ -15,7 +15,8 @@
 // 356 clocks of its HBM time per SM).  The sum over the head's dims may run in
 // any order, so lane quad c takes dims 16 c .. 16 c + 15 of a key: one 16-byte
 // shared load per key.  E4M3 becomes fp16 exactly; the page's key scale joins
-// the scores, its value scale the weights (one rounding of a weight to fp16).
+// the scores, its value scale (in units of the row's largest, SV_UNIT0) the
+// weights: one rounding of a weight to fp16.
 //
 // Measured on B200, 8 kv heads of 4 query heads, one token each: 64 contexts of
 // 2048 tokens 42 us and of 4096 64 us (269 MB, 4.2 TB/s), 128 of up to 8191
@@ -159,6 +160,8 @@ struct FwRows {
     int pos[2];
     float c2;                    // score scale, in powers of two
     float m[2], l[2], o[8][4];   // reference, this lane's share of the sum, output columns 2 c, 2 c + 1 of 8 tiles
+    float per_unit;              // O counts in units (see SV_UNIT0) of the warp's pages so far: a row that does not
+                                 // attend a page attends none behind it either
 };
 struct FwUnit {
     const unsigned char* kd;
@@ -247,14 +250,16 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
                 mma_16816(s[t0 + t], R.q[k][0], R.q[k][1], R.q[k][2], R.q[k][3], w[t][2 * k], w[t][2 * k + 1]);
     }
     constexpr int NR = TWO ? 2 : 1;
-    float kc[2], vc[2], top[2];
+    float kc[2], top[2];
+    bool none[2] = {false, false};  // the row attends no key of the unit
 #pragma unroll
     for (int r = 0; r < NR; r++) {
-        kc[r] = R.c2 * x.ks, vc[r] = x.vs * SV_VEXP;
+        kc[r] = R.c2 * x.ks;
         if (MASKED) {
             if (kc[r] == 0.f) kc[r] = 1e-30f;  // a page of zeros: -inf * 0 is no number
             // a page's scale that is no number reaches only rows that attend the page
-            if (R.pos[r] < x.key0) kc[r] = R.c2, vc[r] = 0.f;
+            none[r] = R.pos[r] < x.key0;
+            if (none[r]) kc[r] = R.c2;
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
@@ -270,13 +275,15 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
         top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * kc[r];
     }
-    const float growth = sv_growth(x.vs);
-    if (__any_sync(0xffffffffu, top[0] > R.m[0] + growth || (TWO && top[NR - 1] > R.m[NR - 1] + growth))) {
+    const bool grown = top[0] > R.m[0] + SV_GROWTH || (TWO && top[NR - 1] > R.m[NR - 1] + SV_GROWTH);
+    if (__any_sync(0xffffffffu, grown || x.vs * R.per_unit >= SV_UNIT_TOP)) {
+        const float v = sv_in_units(x.vs, R.per_unit), step = v >= SV_UNIT_TOP ? sv_unit_step(v) : 1.f;
+        R.per_unit *= step;
 #pragma unroll
         for (int r = 0; r < NR; r++) {
             const float mn = fmaxf(R.m[r], top[r]);
-            const float f = R.m[r] == -INFINITY ? 0.f : sv_exp2(R.m[r] - mn);
-            R.m[r] = mn, R.l[r] *= f;
+            float f = R.m[r] == -INFINITY ? 0.f : sv_exp2(R.m[r] - mn);
+            R.m[r] = mn, R.l[r] *= f, f *= step;
 #pragma unroll
             for (int i = 0; i < 8; i++) R.o[i][2 * r] *= f, R.o[i][2 * r + 1] *= f;
         }
@@ -289,13 +296,13 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
             for (int t = 0; t < NT; t++) a[t / 2][2 * (t & 1) + 1] = 0;
             continue;
         }
-        const float ref = R.m[r] == -INFINITY ? 0.f : R.m[r];
+        const float ref = R.m[r] == -INFINITY ? 0.f : R.m[r], vu = none[r] ? 0.f : x.vs * R.per_unit;
         float l[2] = {0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             const float p0 = sv_exp2(fmaf(s[t][2 * r], kc[r], -ref)), p1 = sv_exp2(fmaf(s[t][2 * r + 1], kc[r], -ref));
             l[t & 1] += p0 + p1;
-            a[t / 2][2 * (t & 1) + r] = sv_pack_h2(p0 * vc[r], p1 * vc[r]);
+            a[t / 2][2 * (t & 1) + r] = sv_pack_h2(p0 * vu, p1 * vu);
         }
         R.l[r] += l[0] + l[1];
     }
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                     fw_skip(A, nx, te - tb);
                     load_q(nx);
                 }
-                R.c2 = c2;
+                R.c2 = c2, R.per_unit = SV_UNIT0;
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
                     R.pos[r] = p.q.p0 + (g + 8 * r) / G;
@@ -460,12 +467,13 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                     const int row = g + 8 * r;
                     if (c == 0) S->ml[warp][row][0] = R.m[r], S->ml[warp][row][1] = R.l[r];
                     if (row >= rows) continue;
+                    const float unit = sv_inverse(R.per_unit);
 #pragma unroll
                     for (int e = 0; e < 2; e++) {  // columns 2 c + e of tile i: dims 8 (2 c + e) + i
                         const int z = 2 * r + e;
                         float4* d = reinterpret_cast<float4*>(&S->o[warp][row][16 * c + 8 * e]);
-                        d[0] = make_float4(R.o[0][z], R.o[1][z], R.o[2][z], R.o[3][z]);
-                        d[1] = make_float4(R.o[4][z], R.o[5][z], R.o[6][z], R.o[7][z]);
+                        d[0] = make_float4(R.o[0][z] * unit, R.o[1][z] * unit, R.o[2][z] * unit, R.o[3][z] * unit);
+                        d[1] = make_float4(R.o[4][z] * unit, R.o[5][z] * unit, R.o[6][z] * unit, R.o[7][z] * unit);
                     }
                 }
                 // notes of the next item: last read two items ago, written only after this barrier
@@ -504,16 +512,14 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
                         }
                     }
                     if (whole) {
-                        const float inv = l == 0.f ? 0.f : 1.f / (SV_VEXP * l);
+                        const float inv = l == 0.f ? 0.f : 1.f / l;
                         uint2 r;
                         r.x = sv_pack_h2(x.x * inv, x.y * inv), r.y = sv_pack_h2(x.z * inv, x.w * inv);
                         *reinterpret_cast<uint2*>(A.out + ((size_t)(p.q.a + row / G) * A.nh + h * G + row % G) * CUINF_HD +
                                                   d) = r;
                     } else {
-                        const float v = 1.f / SV_VEXP;
                         if (d == 0) reinterpret_cast<float2*>(W.ml)[slot * 16 + row] = make_float2(m, l);
-                        *reinterpret_cast<float4*>(W.o + (slot * 16 + row) * CUINF_HD + d) =
-                            make_float4(x.x * v, x.y * v, x.z * v, x.w * v);
+                        *reinterpret_cast<float4*>(W.o + (slot * 16 + row) * CUINF_HD + d) = x;
                     }
                 }
                 if (!whole && tid == 0) {

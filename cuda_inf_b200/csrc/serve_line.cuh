@@ -53,15 +53,29 @@ __device__ __forceinline__ uint32_t sv_e4m3x2(uint32_t two) {  // low 16 bits: t
     return r;
 }
 // The reference that scores are taken from follows a row's maximum when that
-// has grown by more than 2^8 (fp16 holds such weights), so that sums and O are
-// seldom rescaled.
-//
-// FP8: the weights carry the page's value scale times SV_VEXP, so that a usual
-// scale (0.01) keeps weights above 4e-4 in fp16's normal range.  A scale is at
-// most 65504 / 448; from 15.9 on (values above 7000) the limit is 2^3, which
-// keeps scale x 16 x weight below 65504.
-#define SV_VEXP 16.f
-__device__ __forceinline__ float sv_growth(float value_scale) { return value_scale > 15.9f ? 3.f : 8.f; }
+// has grown by more than 2^SV_GROWTH (fp16 holds such weights), so that sums and
+// O are seldom rescaled.
+#define SV_GROWTH 8.f
+// FP8: a weight meets the values' codes times the page's value scale over the
+// row's unit, and O counts in that unit.  The unit is a power of two, 1/64 to
+// 1/128 of the largest scale among the pages that the row has attended, so
+// weights stay below 2^8 * 128 = 2^15 and, of the pages that count, in fp16's
+// normal range down to 2^-20 of the reference (2^-31 is the last that is not
+// lost), whatever the values' size.  A page of larger scale raises the unit in
+// the rare path that follows the maximum; O, in fp32, loses nothing by a power
+// of two.  An infinite scale does not count: its page's values are no numbers.
+#define SV_UNIT0 2147483648.f  // 1 / unit at first: below 2^-24, the smallest scale, so the first page sets it
+#define SV_UNIT_TOP 128.f
+__device__ __forceinline__ float sv_in_units(float scale, float per_unit) {
+    return scale <= 65504.f ? scale * per_unit : 0.f;
+}
+__device__ __forceinline__ float sv_inverse(float power_of_two) {
+    return __uint_as_float((254u << 23) - __float_as_uint(power_of_two));
+}
+// 64 over the power of two at or below x
+__device__ __forceinline__ float sv_unit_step(float x) {
+    return __uint_as_float(((127u + 127u + 6u) << 23) - (__float_as_uint(x) & 0x7f800000u));
+}
 
 // ---- sequences ----
 enum { SV_PACKED = 0, SV_MANY = 1, SV_FEW = 2 };  // packed prompts; paged, many or few rows of a sequence

@@ -13,8 +13,9 @@
 //                    operand) and written to TMEM
 //   O += P V         tcgen05.mma with P from TMEM, 128 x 64 x 128, fp32 in TMEM
 // The reference m follows the row's maximum only when that has grown by more
-// than 2^8 since (sv_growth), so O is rescaled seldom (P stays within fp16's
-// range).
+// than 2^8 since (SV_GROWTH), so O is rescaled seldom (P stays within fp16's
+// range).  Over pages P also carries the page's value scale, in units of the
+// row's largest (SV_UNIT0).
 //
 // A row tile's softmax gives its S back once the scores are in registers, so
 // the next scores come while it works and the kernel runs at the softmax's
@@ -338,6 +339,16 @@ struct SvConv {
         else
             tail(dst, g, tl, kind == SV_TAIL ? rest : 0);
     }
+    // This thread's values of the tail once more, times a power of two.
+    __device__ __forceinline__ void raise(unsigned char* dst, int g, float up) const {
+        const __half2 f = __float2half2_rn(up);
+#pragma unroll 1
+        for (int i = 0; i < 16; i++) {
+            const int u = tid + 128 * (i >> 2), r = 64 * g + (u >> 3);
+            __half2* p = reinterpret_cast<__half2*>(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4)) + (i & 3);
+            *p = __hmul2(*p, f);
+        }
+    }
     // In tiles with masked places, this thread's 32 values of the group once more: is one no number?
     __device__ __forceinline__ void note(unsigned char* dst, int g, int kind, int par, int key0) const {
         const bool pg = kind == SV_PAGE;
@@ -397,6 +408,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigne
                 cv.group(vd, g, kind[g], f + (2 + g) * SERVE_PAGE_HEAD, A.kv.vtail + tail, rest);
                 if (i >= first_masked) cv.note(vd, g, kind[g], par, i * SV_KT);
             }
+            if (kind[1] == SV_TAIL) cv.raise(vd, 1, sv_inverse(S->sc[kt % SV_SC][3]));
             asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
             __threadfence_block();
             __syncwarp();
@@ -405,6 +417,21 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigne
         __syncwarp();
         if (lane == 0) mbar_arrive(&S->epi[par]);
     }
+}
+// The scale of a tail's values beside a page: 2^-k where 2^k, at most 2^15, takes the largest of its `rows` rows below
+// 2^15.  The tail's rows are times 2^k in shared memory.  (With a scale of 1 the page's weights, in units of that
+// scale, would lose what values below 1/448 leave of them.)  All lanes of a warp call.
+__device__ __forceinline__ float sv_tail_scale(const __half* src, int rows, int lane) {
+    uint32_t mx = 0;  // of two halves' bits; infinities and NaN pass by
+#pragma unroll 4
+    for (int u = lane; u < rows * (CUINF_HD / 8); u += 32) {
+        const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * u);
+        const uint32_t w[4] = {x.x & 0x7fff7fffu, x.y & 0x7fff7fffu, x.z & 0x7fff7fffu, x.w & 0x7fff7fffu};
+#pragma unroll
+        for (int j = 0; j < 4; j++) mx = __vmaxu2(mx, w[j] & __vcmpltu2(w[j], 0x7c007c00u));
+    }
+    const uint32_t e = __reduce_max_sync(0xffffffffu, max(mx & 0xffffu, mx >> 16)) >> 10;  // its exponent, biased by 15
+    return __uint_as_float((127u - min(29u - min(e, 29u), 15u)) << 23);
 }
 // The tiles of an item, two pages each, by the copying warp; kt: tiles so far.  Lane l has the page index and the
 // scales of group l of 16 tiles.
@@ -431,6 +458,11 @@ __device__ __forceinline__ bool sv_pages(const AttnArgs& A, SvSmem* S, const SvI
             const uint32_t fs = kt % SV_FST;
             if (!sv_wait_all(&S->f_empty[fs], ((kt / SV_FST) & 1) ^ 1, &S->abort_)) return false;
             const bool mine = lane >> 1 == i;
+            if (2 * (c + i) + 1 == ng && w.q.kv % SERVE_PAGE) {  // a page and the tail
+                const float scale = sv_tail_scale(A.kv.vtail + ((size_t)w.s * A.nkv + w.h) * SERVE_PAGE_HEAD,
+                                                  w.q.kv % SERVE_PAGE, lane);
+                if (mine && kind == SV_TAIL) vs = scale;
+            }
             if (mine) {
                 S->sc[kt % SV_SC][lane & 1] = ks, S->sc[kt % SV_SC][2 + (lane & 1)] = vs;
                 S->kind[fs][lane & 1] = kind;
@@ -532,7 +564,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             const int tok = w.t0 + t * TOK + row_t;
             const bool live_row = row < TOK * G && tok < w.q.c;
             const int pos = live_row ? w.q.p0 + tok : -1;
-            float m = -INFINITY;
+            float m = -INFINITY, per_unit = SV_UNIT0;
             uint64_t l2[2] = {0, 0};  // four partial sums
             const int tb = w.tb, te = w.te;
             const int first_masked = (w.q.p0 + w.t0 + t * TOK + 1) >> 7;  // from here some row masks some key
@@ -544,13 +576,11 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 float* s = reinterpret_cast<float*>(sr);
                 sv_ld32(s_addr, sr), sv_ld32(s_addr + 32, sr + 32);
                 float kc[2] = {c2, c2}, vc[2] = {1.f, 1.f};
-                float growth = 8.f;
                 bool masked = i >= first_masked, gone[2] = {false, false};
                 if (PAGED) {
                     const float4 sc = *reinterpret_cast<const float4*>(S->sc[tiles % SV_SC]);
                     kc[0] = c2 * sc.x, kc[1] = c2 * sc.y;
-                    vc[0] = SV_VEXP * sc.z, vc[1] = SV_VEXP * sc.w;
-                    growth = sv_growth(fmaxf(sc.z, sc.w));
+                    vc[0] = sc.z, vc[1] = sc.w;
                     gone[0] = sc.x < 0.f, gone[1] = sc.y < 0.f;
                     masked |= gone[0] | gone[1];
                 }
@@ -590,17 +620,25 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     ok &= sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_);
                     sv_fence_after();
                 }
-                if (i == tb) {
+                if (i == tb && !PAGED) {
                     m = x;
-                } else if (__any_sync(0xffffffffu, x > m + growth)) {
-                    // rare: the reference follows the maximum, sum and O with it
+                } else if (i == tb || __any_sync(0xffffffffu, x > m + SV_GROWTH ||
+                                                 (PAGED && fmaxf(vc[0], vc[1]) * per_unit >= SV_UNIT_TOP))) {
+                    // rare: the reference follows the maximum (and the unit the scales), sum and O with it
                     const float mn = fmaxf(m, x);
-                    const float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
+                    float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
                     m = mn;
 #pragma unroll
                     for (int e = 0; e < 2; e++) l2[e] = f2_mul(l2[e], f2_pack(f, f));
+                    if (PAGED) {
+                        const float v = fmaxf(sv_in_units(vc[0], per_unit), sv_in_units(vc[1], per_unit));
+                        if (v >= SV_UNIT_TOP) {
+                            const float step = sv_unit_step(v);
+                            per_unit *= step, f *= step;
+                        }
+                    }
 #pragma unroll 1
-                    for (uint32_t j = 0; j < CUINF_HD; j += 16) {
+                    for (uint32_t j = i == tb ? CUINF_HD : 0; j < CUINF_HD; j += 16) {
                         uint32_t o[16];
                         sv_ld16(o_addr + j, o);
                         sv_wait_ld();
@@ -611,6 +649,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 }
                 const float ref = m == -INFINITY ? 0.f : m;
                 const uint64_t nm = f2_pack(-ref, -ref);
+                if (PAGED) vc[0] *= per_unit, vc[1] *= per_unit;
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const int g = j >> 1;
@@ -642,7 +681,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             float la, lb;
             f2_unpack(f2_add(l2[0], l2[1]), la, lb);
             const float l = la + lb;
-            const float vs = PAGED ? 1.f / SV_VEXP : 1.f;
+            const float vs = PAGED ? sv_inverse(per_unit) : 1.f;
             const bool whole = w.tb == 0 && w.te == w.n, any_bad = S->any_bad[seg & 1] != 0;
             const size_t slot = (size_t)blockIdx.x * 2 + (w.tb == 0);
             const float inv = whole ? (l == 0.f ? 0.f : vs / l) : vs;

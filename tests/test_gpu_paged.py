@@ -740,3 +740,108 @@ def test_refusals(cuda):
         ops.attn_paged(q, cu, kvl, *c.t[:6], c.vtail[:1])
     with pytest.raises(CuinfError, match="max_q"):
         ops.attn_paged(q, cu, kvl, *c.t, max_q=0)
+
+
+# ------------------------------------------------------------------ values of every size
+def plain_weights(q, k, v, first, scale=0.125):
+    """q [c,nh,64] at positions first.., k, v [nkv,l,64] (64 bits, finite): (out, bound on its error).
+
+    The bound in units of each row's own weights w (they sum to 1) and values: a weight is rounded once to 11 bits
+    (2^-11 of itself; its exponential, the scores' sums and the rescalings together stay below half of that), the
+    result to fp16 (2^-11 |o|, or 2^-25 below its normal range), and what a weight loses below fp16's range is at
+    most 2^-31 of the row's largest weight (2^-25 for the up to 63 keys of the tail) times its largest value."""
+    c, nh, _ = q.shape
+    k, v = (x.repeat_interleave(nh // k.shape[0], 0) for x in (k, v))
+    s = torch.einsum("chd,hld->hcl", q.double(), k) * scale
+    pos = first + torch.arange(c, device=q.device)
+    ok = (torch.arange(k.shape[1], device=q.device)[None] <= pos[:, None])[None]
+    w = torch.softmax(torch.where(ok, s, torch.full_like(s, -INF)), -1)
+    o, mag = torch.einsum("hcl,hld->chd", w, v), torch.einsum("hcl,hld->chd", w, v.abs())
+    top = (w.amax(-1) * v.abs().amax(-1).cummax(-1).values[:, pos]).T[..., None]
+    lost = (k.shape[1] * 2.0**-31 + 63 * 2.0**-25) * top
+    return o, 2.0**-11 * o.abs() + 1.5 * 2.0**-11 * mag + lost + 2.0**-25
+
+
+def check_weights(c, q, new, out):
+    a = 0
+    for i, x in enumerate(new):
+        close(out[a:a + x], *plain_weights(q[a:a + x], c.values(i, "k"), c.values(i, "v"), c.lens[i] - x))
+        a += x
+
+
+def first_key_heavy(c, lens, sizes, weight, seed):
+    """Fills the cache: keys of unit scores but for the first, which takes all but about n e^0.5 / e^weight of a
+    row's weight and whose value is small beside the others, and values of standard deviation sizes[i] in the i-th
+    equal part of a sequence."""
+    for i, n in enumerate(lens):
+        k, v = rnd((n, c.nkv, 64), seed + i, c.dev), rnd((n, c.nkv, 64), seed + 50 + i, c.dev, 1.0).float()
+        k[:, :, 0] = 0
+        k[0] = 0
+        k[0, :, 0] = weight
+        part = torch.arange(n, device=c.dev) * len(sizes) // n
+        v *= torch.tensor(sizes, device=c.dev)[part][:, None, None]
+        v[0] *= 0.02
+        new = [0] * len(lens)
+        new[i] = n
+        c.append(k, v.half(), new)
+
+
+def heavy_queries(t, nh, dev, seed):
+    q = rnd((t, nh, 64), seed, dev)
+    q[:, :, 0] = 8.0  # a score of 0.125 * 8 * weight on the first key
+    return q
+
+
+@pytest.mark.parametrize("sizes", [[1.0], [0.3], [0.1], [0.01], [0.001], [0.3, 0.001], [0.001, 0.3], [0.01, 300.0, 0.01]],
+                         ids=lambda x: "-".join(map(str, x)))
+@pytest.mark.parametrize("new", [1, 3, 40, 300])
+@pytest.mark.parametrize("total", [2048, 8192 + 64 + 37, 8192 + 5])
+def test_weights_beside_a_heavy_first_key(cuda, sizes, new, total):
+    """Most of the weight on one key of small value: what is left of the result are the many small weights."""
+    c = Cache(1, 2, total, cuda)
+    first_key_heavy(c, [total], sizes, 14.0, 3)
+    q = heavy_queries(new, 8, cuda, 7)
+    out = c.attend(q, [new], max_q=new)
+    assert ops.paged_error() == 0
+    check_weights(c, q, [new], out)
+
+
+def test_weights_beside_a_heavy_first_key_mixed(cuda):
+    lens, new = [3000, 700, 5000, 64, 129], [1, 200, 1, 3, 70]
+    c = Cache(5, 2, 5000, cuda)
+    first_key_heavy(c, lens, [0.03], 13.0, 3)
+    q = heavy_queries(sum(new), 8, cuda, 7)
+    out = c.attend(q, new)
+    check_weights(c, q, new, out)
+
+
+@pytest.mark.parametrize("late", [30, 64 + 30, 200])
+@pytest.mark.parametrize("new", [2, 100, 400])
+def test_small_values_before_large_ones(cuda, late, new):
+    """The newest tokens' values are 300 times the others'; rows before them do not attend them, and their weights
+    go by the values that they do attend."""
+    for total in (1000, 1030, 1100, 64 * 17 + late):
+        c = Cache(1, 2, total, cuda)
+        k, v = rnd((total, 2, 64), 3, cuda), rnd((total, 2, 64), 4, cuda, 0.01)
+        v[total - late:] *= 300
+        c.append(k, v, [total])
+        q = rnd((new, 8, 64), 7, cuda, 3.0)
+        out = c.attend(q, [new], max_q=new)
+        check_weights(c, q, [new], out)
+
+
+@pytest.mark.parametrize("new", [1, 3, 70])
+def test_page_scales_of_all_sizes(cuda, new):
+    """Pages whose value scales go from fp16's smallest to large ones, in every order, and a tail beside them."""
+    steps = [0.0, 3e-5, 1e-3, 0.0, 0.05, 2.0, 100.0, 5000.0, 60000.0]
+    for sizes in (steps, steps[::-1], steps[4:] + steps[:4]):
+        total = 64 * len(sizes) * 2 + 31
+        c = Cache(1, 2, total, cuda)
+        k, v = rnd((total, 2, 64), 3, cuda), rnd((total, 2, 64), 4, cuda).float().clamp(-1, 1)
+        v[:-31] *= torch.tensor(sizes, device=cuda).repeat_interleave(64).repeat(2)[:, None, None]
+        v[-31:] *= sizes[3]
+        c.append(k, v.half(), [total])
+        q = rnd((new, 8, 64), 7, cuda)
+        out = c.attend(q, [new], max_q=new)
+        assert bool(out.isfinite().all())
+        check_weights(c, q, [new], out)
