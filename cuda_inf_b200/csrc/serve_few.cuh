@@ -71,19 +71,20 @@ __device__ __forceinline__ void fw_skip(const AttnArgs& A, FwPos& p, int by) {
         p.n = fw_units(p.q);
     }
 }
-// Page of a unit: an index (unchecked), or -2 for a part of the tail.
+// Page of a unit: the table's entry, whatever it is (-1 for a part of the tail, which its place alone tells).
+__device__ __forceinline__ bool fw_tail(const FwPos& p) { return p.u >= p.q.kv / SERVE_PAGE; }
 __device__ __forceinline__ int fw_page(const AttnArgs& A, const FwPos& p) {
-    return p.u < p.q.kv / SERVE_PAGE ? __ldg(A.kv.table + (size_t)p.s * A.kv.width + p.u) : -2;
+    return fw_tail(p) ? -1 : __ldg(A.kv.table + (size_t)p.s * A.kv.width + p.u);
 }
 
 __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsigned char* ring, int lane) {
     if (lane >= FW_ST) return;
     const int cnt = S->left;
     FwPos p, np;  // the unit to copy; the one after it (FW_ST further on)
-    int npage = -2;
+    int npage = -1;
     fw_first(A, S->share, p);
     fw_skip(A, p, lane);
-    int page = lane < cnt ? fw_page(A, p) : -2;
+    int page = lane < cnt ? fw_page(A, p) : -1;
     auto scales = [&](const FwPos& x, int pg, __half& k, __half& v) {
         k = v = __float2half_rn(1.f);
         if (pg < 0 || pg >= A.kv.n_pages) return;
@@ -112,7 +113,7 @@ __device__ __forceinline__ void fw_producer(const AttnArgs& A, FwSmem* S, unsign
         const int u = p.u, h = p.h, ng = p.q.kv / SERVE_PAGE;
         auto put = [&] { S->sc[lane][0] = __half2float(ks), S->sc[lane][1] = __half2float(vs); };
         armed = true;
-        if (page == -2) {
+        if (fw_tail(p)) {
             const int first = (u - ng) * FW_TAIL, rows = min(FW_TAIL, p.q.kv % SERVE_PAGE - first);
             if (rows > 0) {
                 const size_t at = ((size_t)p.s * A.nkv + h) * SERVE_PAGE_HEAD + (size_t)first * CUINF_HD;

@@ -845,3 +845,25 @@ def test_page_scales_of_all_sizes(cuda, new):
         out = c.attend(q, [new], max_q=new)
         assert bool(out.isfinite().all())
         check_weights(c, q, [new], out)
+
+
+@pytest.mark.parametrize("new", [1, 2, 60])
+def test_every_page_index_outside_the_pool_counts_as_absent(cuda, new):
+    """Small negative numbers too, in every place of the table, beside a tail and without one."""
+    for total in (500, 512):
+        c = Cache(3, 2, 512, cuda)
+        fill(c, [total] * 3, 3)
+        q = rnd((3 * new, 8, 64), 7, cuda)
+        want = c.attend(q, [new] * 3, max_q=new)
+        assert ops.paged_error() == 0
+        for wrong in (-2, -3, -4, -63, -64, c.kp8.shape[0], c.kp8.shape[0] + 1):
+            for at in (0, 3, 5):  # (pages that all new rows attend in full)
+                keep = int(c.table[1, at])
+                c.table[1, at] = wrong
+                out = c.attend(q, [new] * 3, max_q=new)
+                assert ops.paged_error() == 2
+                c.table[1, at] = keep
+                assert torch.equal(out[:new], want[:new]) and torch.equal(out[2 * new:], want[2 * new:])
+                k, v = (torch.cat([x[:, :64 * at], x[:, 64 * at + 64:]], 1) for x in (c.values(1, "k"), c.values(1, "v")))
+                o, tol = plain_rows(q[new:2 * new], k, v, total - 64 - new, 0.125)
+                close(out[new:2 * new], o, tol)
