@@ -53,7 +53,9 @@ extern "C" int cuinf_paged_error(unsigned* flags) {
 //
 // CTA -> (sequence, group) without a plan: sequence s owns the slots from
 // (cu[s] + 62 s) / 64 + s on, which are at least the groups L new rows can
-// touch ((L + 62) / 64 + 1).
+// touch ((L + 62) / 64 + 1).  That needs ascending offsets: where they are not,
+// the largest offset so far takes the place of cu[s], and a sequence that begins
+// before it is skipped like one whose own offsets are out of order.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
     const __half *k, *v;
@@ -74,17 +76,28 @@ __device__ __forceinline__ uint32_t serve_e4m3x2(float lo, float hi) {
 __global__ void __launch_bounds__(256, 3) k_paged_append(const AppendArgs A) {
     extern __shared__ __align__(16) unsigned char append_raw[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int s = -1;
+    int s = -1, begin = 0;
+    bool disorder = false;
+    auto offset = [&](int i) { return min(max(A.rows.cu[i], 0), A.rows.n_rows); };
     for (int b = 0; b < A.rows.n_seqs; b += 256) {
         const int i = b + tid;
-        const bool mine = i < A.rows.n_seqs &&
-                          append_slot(min(max(A.rows.cu[i], 0), A.rows.n_rows), i) <= (long long)blockIdx.x;
+        const bool mine = i < A.rows.n_seqs && append_slot(offset(i), i) <= (long long)blockIdx.x;
+        disorder |= i < A.rows.n_seqs && A.rows.cu[i] > A.rows.cu[i + 1];
         s += __syncthreads_count(mine);
+    }
+    if (__syncthreads_or(disorder)) {
+        s = -1;
+#pragma unroll 1
+        for (int i = 0; i < A.rows.n_seqs; i++) {
+            const int most = max(begin, offset(i));
+            if (append_slot(most, i) > (long long)blockIdx.x) break;
+            begin = most, s = i;
+        }
     }
     if (s < 0) return;
     int a, b;
     const int ctx = A.ctx[s];
-    const bool fine = packed_range(A.rows, s, a, b) && ctx >= 0 && (long long)ctx + (b - a) < (1ll << 31);
+    const bool fine = packed_range(A.rows, s, a, b) && a >= begin && ctx >= 0 && (long long)ctx + (b - a) < (1ll << 31);
     if (!fine) {
         if (tid == 0) atomicOr(A.err, SERVE_ERR_RANGE);
         return;

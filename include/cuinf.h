@@ -206,7 +206,9 @@ int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k, int64_t k_
                       int nh, int nkv, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Append the packed new rows k, v [n_rows][nkv][64] to the paged cache:
- * sequence s holds ctx_lens[s] tokens (device int) before the call.  Every
+ * sequence s holds ctx_lens[s] tokens (device int) before the call.  Where the
+ * offsets are not ascending, a sequence that begins before an earlier offset is
+ * skipped and reported too.  Every
  * 64-token group that the call completes is quantized like
  * cuinf_kv_commit_group into page table[s][group] (scale = absmax/448 + 1e-12,
  * codes with the fp32 scale); the rows of the unfinished last group go to the

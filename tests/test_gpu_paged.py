@@ -867,3 +867,40 @@ def test_every_page_index_outside_the_pool_counts_as_absent(cuda, new):
                 k, v = (torch.cat([x[:, :64 * at], x[:, 64 * at + 64:]], 1) for x in (c.values(1, "k"), c.values(1, "v")))
                 o, tol = plain_rows(q[new:2 * new], k, v, total - 64 - new, 0.125)
                 close(out[new:2 * new], o, tol)
+
+
+def well_formed(cu, rows):
+    """Sequences whose two offsets are in range and in order and that begin at no less than every offset before."""
+    top, ok = 0, []
+    for s, (a, b) in enumerate(zip(cu, cu[1:])):
+        top = max(top, min(max(a, 0), rows))
+        if 0 <= a <= b <= rows and a >= top:
+            ok.append(s)
+    return ok
+
+
+DISORDER = [[0, 800, 1000, 0, 1000], [0, 1000, 1001, 50, 60], [0, 1000, 1001, 0, 0], [500, 100, 200, 300], [900, 1001, 0],
+            [0, 64, 63, 127, 200, 199, 500], [0, 2000, 10, 20], [-7, 30, 10, 900], [0, 100, 1500, 300, 400, 2**31 - 1],
+            [1001, -2**31, 5, 9], [0, 0, 0, 300, 299, 299, 800], list(range(0, 600, 2)) + [3, 4, 700]]
+
+
+@pytest.mark.parametrize("ctx", [0, 60, 640])
+@pytest.mark.parametrize("cu", DISORDER, ids=lambda x: "-".join(map(str, x[:5])))
+def test_append_offsets_out_of_order(cuda, cu, ctx):
+    """A sequence that is out of order is skipped and reported; the others are appended, and no other page, scale or
+    tail is touched."""
+    rows, n = 1001, len(cu) - 1
+    k, v = rnd((rows, 2, 64), 3, cuda), rnd((rows, 2, 64), 4, cuda)
+    got, want = (Cache(n, 2, ctx + rows, cuda, seed=5) for _ in range(2))
+    for c in (got, want):
+        fill(c, [ctx] * n, 7)
+    assert ops.paged_error() == 0
+    for s in well_formed(cu, rows):
+        a, b = cu[s], cu[s + 1]
+        want.append(k[a:b], v[a:b], [b - a if i == s else 0 for i in range(n)])
+        want.lens = [ctx] * n
+    assert ops.paged_error() == 0
+    ops.kv_paged_append(k, v, torch.tensor(cu, dtype=torch.int32, device=cuda), got.ints(), *got.t)
+    assert ops.paged_error() == 4
+    for x, y in zip(got.t, want.t):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
