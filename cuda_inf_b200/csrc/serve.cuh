@@ -30,8 +30,9 @@ struct PagedKV {
 #define SERVE_FEW_ROWS 16
 
 // New rows of packed sequences: sequence s holds rows cu[s]..cu[s+1]-1 of
-// n_rows.  Offsets outside [0, n_rows] or out of order are clamped (and
-// reported), so that no row outside the tensors is touched.
+// n_rows.  Offsets outside [0, n_rows] are clamped, and a sequence whose own two
+// are clamped or out of order is reported and skipped, so that no row outside
+// the tensors is touched.
 struct PackedRows {
     const int* cu;
     int n_seqs, n_rows;

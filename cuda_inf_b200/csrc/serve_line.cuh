@@ -89,7 +89,7 @@ template <int KIND>
 __device__ __forceinline__ bool sv_seq(const AttnArgs& A, int s, SvSeq& q, bool report) {
     int b;
     bool fine = packed_range(A.rows, s, q.a, b);
-    q.c = b - q.a;
+    q.c = fine ? b - q.a : 0;
     if (KIND != SV_PACKED) {
         q.kv = __ldg(A.kv_lens + s);
         if (q.c > 0 && (q.kv < 0 || q.kv / SERVE_PAGE > A.kv.width || q.c > A.max_q)) {

@@ -191,7 +191,8 @@ int cuinf_moe_ffn(const void* xn, const void* gate, const void* expert_bias,
 /* be captured into a CUDA graph.  What the device finds wrong there it skips  */
 /* and reports in a word per device (cuinf_paged_error): a page index outside  */
 /* the pool (its keys count as absent, its group is not stored), lengths or    */
-/* offsets outside their ranges (the sequence is skipped).                     */
+/* offsets outside their ranges or a sequence's two offsets out of order (the  */
+/* sequence is skipped).  A row that several sequences claim is undefined.      */
 /* ------------------------------------------------------------------------ */
 
 /* out[t,h,:] = softmax(scale * q[t,h] . k[j,h/(nh/nkv)]) v over the rows j of

@@ -904,3 +904,29 @@ def test_append_offsets_out_of_order(cuda, cu, ctx):
     assert ops.paged_error() == 4
     for x, y in zip(got.t, want.t):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("cu", [[0, 70], [-5, 20], [-5, 2], [20, 30, 51], [60, 70], [0, 20, 10, 40, 2**31 - 1], [-2**31, 50]],
+                         ids=str)
+def test_sequences_with_offsets_outside_are_skipped(cuda, cu):
+    """Reported, and none of their rows written; the others as ever."""
+    rows, n = 50, len(cu) - 1
+    q, k, v = rnd((rows, 4, 64), 1, cuda), rnd((rows, 1, 64), 2, cuda), rnd((rows, 1, 64), 3, cuda)
+    c = Cache(n, 1, 128, cuda)
+    fill(c, [100] * n, 5)
+    offsets = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    good = [(s, a, b) for s, (a, b) in enumerate(zip(cu, cu[1:])) if 0 <= a <= b <= rows]
+    assert ops.paged_error() == 0
+    calls = [(lambda out: ops.attn_varlen(q, k, v, offsets, out=out), lambda s, a, b: plain_rows(
+        q[a:b], k[a:b].double().transpose(0, 1), v[a:b].double().transpose(0, 1), 0, 0.125))]
+    calls += [(lambda out, m=m: ops.attn_paged(q, offsets, c.ints(), *c.t, max_q=m, out=out), lambda s, a, b: plain_rows(
+        q[a:b], c.values(s, "k"), c.values(s, "v"), 100 - (b - a), 0.125)) for m in (None, 50)]
+    for call, plain in calls:
+        out = torch.full_like(q, 9.0)
+        call(out)
+        assert ops.paged_error() == 4
+        for s, a, b in good:  # (a row that two of them claim is undefined)
+            one = [sum(x <= r < y for _, x, y in good) == 1 for r in range(a, b)]
+            o, tol = plain(s, a, b)
+            close(out[a:b][one], o[one], tol[one])
+        assert bool((out[[not any(x <= r < y for _, x, y in good) for r in range(rows)]] == 9).all())
