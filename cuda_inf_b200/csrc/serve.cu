@@ -16,18 +16,25 @@
         if (!(cond)) return cuinf_set_arg_error(msg); \
     } while (0)
 
-static __device__ unsigned g_serve_err;
+static __device__ unsigned g_serve_err, g_serve_taken;
 static int serve_err_ptr(unsigned** p) {
     CUINF_TRY(cudaGetSymbolAddress((void**)p, g_serve_err));
     return CUINF_OK;
 }
 
+// Read and cleared at once, so that a bit set meanwhile (by a call of another host thread) is kept for the next asking.
+__global__ void k_take_err() { g_serve_taken = atomicExch(&g_serve_err, 0u); }
+
 extern "C" int cuinf_paged_error(unsigned* flags) {
     REQUIRE(flags, "null pointer");
+    static std::mutex mu;  // of g_serve_taken
+    std::lock_guard<std::mutex> lock(mu);
+    // the default stream alone would not wait for non-blocking ones
+    CUINF_TRY(cudaDeviceSynchronize());
+    k_take_err<<<1, 1>>>();
+    if (int rc = cuinf_launch_status()) return rc;
     unsigned v = 0;
-    const unsigned zero = 0;
-    CUINF_TRY(cudaMemcpyFromSymbol(&v, g_serve_err, sizeof(v)));
-    if (v) CUINF_TRY(cudaMemcpyToSymbol(g_serve_err, &zero, sizeof(zero)));
+    CUINF_TRY(cudaMemcpyFromSymbol(&v, g_serve_taken, sizeof(v)));
     *flags = v;
     return CUINF_OK;
 }

@@ -428,7 +428,8 @@ def attn_paged(q, cu_seqlens, kv_lens, table, kp8, vp8, kps, vps, ktail, vtail, 
 
 def paged_error():
     """Read and clear the current device's error word of attn_varlen,
-    kv_paged_append and attn_paged (0 = none; the bits are in cuinf.h)."""
+    kv_paged_append and attn_paged (0 = none; the bits are in cuinf.h).  Waits
+    for all work of the device, on every stream."""
     flags = ctypes.c_uint(0)
     check(lib().cuinf_paged_error(ctypes.byref(flags)))
     return flags.value

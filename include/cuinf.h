@@ -233,9 +233,11 @@ int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_seqlens, con
                      const void* vtail, float scale, void* out, int nh, int nkv, void* workspace,
                      size_t workspace_bytes, void* stream);
 
-/* Read and clear the current device's error word of these operators
- * (synchronous): bit 0 a bounded wait gave up, bit 1 a page index outside the
- * pool, bit 2 lengths or offsets outside their ranges. */
+/* Read and clear the current device's error word of these operators.  Waits
+ * for all work of the device, on every stream, so not while a stream captures
+ * and not in every step of a server that overlaps streams.  Bit 0: a bounded
+ * wait gave up, bit 1: a page index outside the pool, bit 2: lengths or offsets
+ * outside their ranges. */
 int cuinf_paged_error(unsigned* flags);
 
 /* INT4 G=128 quantizer of tools/export_weights.py:64-79, bit-exact:

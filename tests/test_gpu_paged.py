@@ -930,3 +930,22 @@ def test_sequences_with_offsets_outside_are_skipped(cuda, cu):
             o, tol = plain(s, a, b)
             close(out[a:b][one], o[one], tol[one])
         assert bool((out[[not any(x <= r < y for _, x, y in good) for r in range(rows)]] == 9).all())
+
+
+def test_errors_are_seen_at_once_from_every_stream(cuda):
+    """paged_error right after calls on side streams that are still waiting for their turn."""
+    c = Cache(1, 1, 128, cuda)
+    fill(c, [100], 5)
+    q, one, bad, lens = rnd((1, 4, 64), 1, cuda), cum([1], cuda), cum([2], cuda), c.ints()
+    table = torch.full_like(c.table, -1)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(streams[0]):
+            torch.cuda._sleep(20_000_000)
+            ops.attn_varlen(q, q[:, :1], q[:, :1], bad)
+        with torch.cuda.stream(streams[1]):
+            torch.cuda._sleep(40_000_000)
+            ops.attn_paged(q, one, lens, table, *c.t[1:], max_q=1)
+        assert ops.paged_error() == 6
+        assert ops.paged_error() == 0
