@@ -468,6 +468,7 @@ __device__ __forceinline__ bool sv_pages(const AttnArgs& A, SvSmem* S, const SvI
                 S->kind[fs][lane & 1] = kind;
             }
             const uint32_t pages = __popc(__ballot_sync(0xffffffffu, mine && kind == SV_PAGE));
+            __syncwarp();  // scales and kinds before the arrival (a vote does not order memory)
             if (lane == 0) {
                 if (pages)
                     mbar_arrive_expect_tx(&S->f_full[fs], pages * 2 * SERVE_PAGE_HEAD);
