@@ -572,6 +572,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
             for (int i = tb; i < te; i++, ops++, tiles++) {
                 // (a wait that gave up ends the loop after the tile, for all lanes alike)
                 ok = sv_wait(&S->s_full[t], ops & 1, &S->abort_);
+                __syncwarp();  // lanes leave a wait one by one; TMEM accesses take the whole warp
                 sv_fence_after();
                 uint32_t sr[128];
                 float* s = reinterpret_cast<float*>(sr);
@@ -619,6 +620,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 // the last product has read P and written O
                 if (i > tb) {
                     ok &= sv_wait(&S->o_full[t], (ops - 1) & 1, &S->abort_);
+                    __syncwarp();
                     sv_fence_after();
                 }
                 if (i == tb && !PAGED) {
@@ -633,10 +635,8 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                     for (int e = 0; e < 2; e++) l2[e] = f2_mul(l2[e], f2_pack(f, f));
                     if (PAGED) {
                         const float v = fmaxf(sv_in_units(vc[0], per_unit), sv_in_units(vc[1], per_unit));
-                        if (v >= SV_UNIT_TOP) {
-                            const float step = sv_unit_step(v);
-                            per_unit *= step, f *= step;
-                        }
+                        const float step = v >= SV_UNIT_TOP ? sv_unit_step(v) : 1.f;
+                        per_unit *= step, f *= step;
                     }
 #pragma unroll 1
                     for (uint32_t j = i == tb ? CUINF_HD : 0; j < CUINF_HD; j += 16) {
@@ -691,6 +691,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
 #pragma unroll 1
             for (int d0 = 0; d0 < CUINF_HD; d0 += 32) {
                 uint32_t o[32];
+                __syncwarp();
                 sv_ld32(o_addr + d0, o);
                 sv_wait_ld();
                 const float* of = reinterpret_cast<const float*>(o);
