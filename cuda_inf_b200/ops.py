@@ -418,8 +418,7 @@ def attn_paged(q, cu_seqlens, kv_lens, table, kp8, vp8, kps, vps, ktail, vtail, 
     T = q.shape[0]
     if T == 0 or n == 0:
         return out
-    if max_q is None:
-        max_q = T
+    max_q = T if max_q is None else min(max_q, T)  # (a bound above 32 bits would wrap in the call)
     size = _scratch_bytes("cuinf_attn_paged_workspace_size", n, T, max_q, nh, nkv, cache[1])
     workspace, ws, nbytes = _scratch(workspace, size, q, index)
     _call(lib().cuinf_attn_paged, index, qp, qs, cu, kvl, n, T, max_q, *cache, scale, op, nh, nkv, ws, nbytes)

@@ -949,3 +949,15 @@ def test_errors_are_seen_at_once_from_every_stream(cuda):
             ops.attn_paged(q, one, lens, table, *c.t[1:], max_q=1)
         assert ops.paged_error() == 6
         assert ops.paged_error() == 0
+
+
+@pytest.mark.parametrize("bound", [61, 4096, 2**31 - 1, 2**31, 2**32, 2**32 + 1, 2**40])
+def test_any_bound_of_the_longest_sequence(cuda, bound):
+    """max_q is an upper bound, however large."""
+    c = Cache(3, 2, 256, cuda)
+    fill(c, [100, 200, 100], 3)
+    q = rnd((62, 8, 64), 7, cuda)
+    want = c.attend(q, [1, 60, 1], max_q=60)
+    got = c.attend(q, [1, 60, 1], max_q=bound)
+    assert ops.paged_error() == 0
+    assert torch.equal(got, want)
