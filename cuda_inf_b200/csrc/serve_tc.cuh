@@ -502,7 +502,6 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
     SvSmem* S = reinterpret_cast<SvSmem*>(Ks + 8 * SV_TILE_BYTES);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int G = A.nh / A.nkv, TOK = 128 / G, tq = 2 * TOK;
-    pdl_trigger();
 
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -529,6 +528,8 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                      "r"(SV_TMEM_COLS)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+        // not before: a dependent kernel that allocates TMEM would hold it and wait for this one to end
+        pdl_trigger();
     }
     if (split && tid < 2) W.part[blockIdx.x * 2 + tid].valid = 0;
     sv_start<C::KIND>(A, S, tq, gridDim.x, PAGED && beside);
