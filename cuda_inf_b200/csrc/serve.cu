@@ -345,7 +345,7 @@ extern "C" int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k,
                                  void* stream) {
     REQUIRE(q && k && v && cu_seqlens && out, "null pointer");
     REQUIRE(n_seqs > 0 && n_rows > 0, "n_seqs and n_rows must be positive");
-    REQUIRE(scale > 0.f && isfinite(scale), "scale must be positive and finite");
+    REQUIRE(scale > 0.f && isfinite(scale * SV_LOG2E), "scale must be positive and finite (times log2(e) too)");
     CHECK_HEADS(nh, nkv);
     CHECK_ROWS(q, q_stride, nh, "q");
     CHECK_ROWS(k, k_stride, nkv, "k");
@@ -385,7 +385,7 @@ extern "C" int cuinf_attn_paged(const void* q, int64_t q_stride, const int* cu_s
     REQUIRE(q && cu_seqlens && kv_lens && out, "null pointer");
     REQUIRE(n_seqs > 0 && n_rows > 0, "n_seqs and n_rows must be positive");
     REQUIRE(max_q > 0, "max_q must be positive");
-    REQUIRE(scale > 0.f && isfinite(scale), "scale must be positive and finite");
+    REQUIRE(scale > 0.f && isfinite(scale * SV_LOG2E), "scale must be positive and finite (times log2(e) too)");
     CHECK_HEADS(nh, nkv);
     CHECK_CACHE(kp8, vp8, kps, vps, ktail, vtail, table, table_width, n_pages);
     CHECK_ROWS(q, q_stride, nh, "q");

@@ -385,7 +385,7 @@ __global__ void __launch_bounds__((FW_WARPS + 1) * 32, 1)
             __syncwarp();
         } else {
             const int G = A.nh / A.nkv, g = lane >> 2, c = lane & 3;
-            const float c2 = A.scale * 1.44269504088896340736f;
+            const float c2 = A.scale * SV_LOG2E;
             FwPos p;
             fw_first(A, S->share, p);
             int j = 0;  // share's units before the item

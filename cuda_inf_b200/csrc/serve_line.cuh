@@ -37,6 +37,7 @@ __device__ __forceinline__ void sv_drain(uint64_t* bar, uint32_t parity) {
 }
 
 // ---- arithmetic ----
+#define SV_LOG2E 1.44269504088896340736f
 __device__ __forceinline__ float sv_exp2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));

@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
         const int t = warp >> 2, row = tid & 127;
         const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const uint32_t o_addr = lane_base + SV_O_COL + t * CUINF_HD;
-        const float c2 = A.scale * 1.44269504088896340736f;  // scores in powers of two
+        const float c2 = A.scale * SV_LOG2E;  // scores in powers of two
         const uint32_t s_addr = lane_base + t * 128, p_addr = lane_base + SV_P_COL + t * 64;
         const int row_t = row / G, row_h = row - row_t * G;  // the row's token and head in the row tile
         uint32_t ops = 0, tiles = 0, seg = 0;

@@ -197,10 +197,11 @@ int cuinf_moe_ffn(const void* xn, const void* gate, const void* expert_bias,
 
 /* out[t,h,:] = softmax(scale * q[t,h] . k[j,h/(nh/nkv)]) v over the rows j of
  * t's sequence up to t (causal).  q [n_rows][nh][64], k, v [n_rows][nkv][64],
- * out fp16 [n_rows][nh][64] contiguous; nh/nkv <= 128; scale > 0.  Softmax
- * statistics and sums in fp32.  workspace: device scratch of
- * cuinf_attn_varlen_workspace_size bytes, 16-byte aligned, any contents; calls
- * that may overlap need one each.  All q/k/v/out pointers 16-byte aligned. */
+ * out fp16 [n_rows][nh][64] contiguous; nh/nkv <= 128; scale > 0, and finite
+ * times log2(e).  Softmax statistics and sums in fp32.  workspace: device
+ * scratch of cuinf_attn_varlen_workspace_size bytes, 16-byte aligned, any
+ * contents; calls that may overlap need one each.  All q/k/v/out pointers
+ * 16-byte aligned. */
 size_t cuinf_attn_varlen_workspace_size(int n_seqs, int n_rows, int nh, int nkv);
 int cuinf_attn_varlen(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
                       int64_t v_stride, const int* cu_seqlens, int n_seqs, int n_rows, float scale, void* out,

@@ -86,3 +86,11 @@ def test_wrappers_refuse_cpu_tensors_and_types():
         ops.kv_paged_append(_t(4, 1, 64), _t(4, 1, 64), cu, cu[:1], cu[None], *(None,) * 6)
     with pytest.raises(TypeError, match="q must be"):
         ops.attn_paged(_t(4, 4, 64).float(), cu, cu[:1], cu[None], *(None,) * 6)
+
+
+@pytest.mark.parametrize("call", [varlen, paged])
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_scale_that_is_infinite_in_powers_of_two(call, scale):
+    """Scores are taken times log2(e): a scale that this makes infinite would give no numbers."""
+    rc, err = call(scale=scale)
+    assert rc == 1 and b"scale must be" in err, (rc, err)
