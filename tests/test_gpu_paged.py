@@ -765,7 +765,8 @@ def plain_weights(q, k, v, first, scale=0.125):
 def check_weights(c, q, new, out):
     a = 0
     for i, x in enumerate(new):
-        close(out[a:a + x], *plain_weights(q[a:a + x], c.values(i, "k"), c.values(i, "v"), c.lens[i] - x))
+        if x:
+            close(out[a:a + x], *plain_weights(q[a:a + x], c.values(i, "k"), c.values(i, "v"), c.lens[i] - x))
         a += x
 
 
