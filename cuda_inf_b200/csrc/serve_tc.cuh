@@ -626,9 +626,11 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 }
                 if (i == tb && !PAGED) {
                     m = x;
-                } else if (i == tb || __any_sync(0xffffffffu, x > m + SV_GROWTH ||
-                                                 (PAGED && fmaxf(vc[0], vc[1]) * per_unit >= SV_UNIT_TOP))) {
-                    // rare: the reference follows the maximum (and the unit the scales), sum and O with it
+                } else if (i == tb ||
+                           __any_sync(0xffffffffu, live_row && (x > m + SV_GROWTH ||
+                                                                (PAGED && fmaxf(vc[0], vc[1]) * per_unit >= SV_UNIT_TOP)))) {
+                    // (rows that are nobody's, another sequence's or left in shared memory, have no vote: a row's bits
+                    // go by its sequence alone)  rare: the reference follows the maximum (and the unit the scales), sum and O with it
                     const float mn = fmaxf(m, x);
                     float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
                     m = mn;

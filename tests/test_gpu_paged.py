@@ -962,3 +962,25 @@ def test_any_bound_of_the_longest_sequence(cuda, bound):
     got = c.attend(q, [1, 60, 1], max_q=bound)
     assert ops.paged_error() == 0
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("nh,nkv", [(32, 8), (12, 4), (5, 1), (12, 1), (48, 1)])
+def test_bits_go_by_the_sequence_alone(cuda, nh, nkv):
+    """With the lengths and the keys the same, a sequence's bits depend neither on its neighbours' queries nor on what
+    ran before."""
+    lens, new = [400, 700, 352, 300], [150, 77, 129, 31]
+    c = Cache(4, nkv, 700, cuda)
+    fill(c, lens, 3)
+    q = rnd((sum(new), nh, 64), 7, cuda, 2.0)
+    big = rnd((900, nh, 64), 8, cuda, 40.0)
+    kv = [rnd((sum(new), nkv, 64), 9 + i, cuda) for i in range(2)]
+    calls = [lambda q: c.attend(q, new, max_q=max(new)), lambda q: ops.attn_varlen(q, *kv, cum(new, cuda))]
+    for call in calls:
+        want = call(q)
+        for i in range(4):
+            a, b = sum(new[:i]), sum(new[:i + 1])
+            for scale in (0.0, 1.0, 30.0):
+                other = q * scale
+                other[a:b] = q[a:b]
+                ops.attn_varlen(big * scale, big[:, :nkv], big[:, :nkv], cum([900], cuda))
+                assert torch.equal(call(other)[a:b], want[a:b]), (i, scale)
