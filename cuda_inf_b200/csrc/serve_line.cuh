@@ -43,6 +43,7 @@ __device__ __forceinline__ float sv_exp2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
     return r;
 }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];\n" ::"l"(p)); }
 __device__ __forceinline__ uint32_t sv_pack_h2(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));

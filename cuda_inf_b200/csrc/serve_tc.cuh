@@ -343,10 +343,14 @@ struct SvConv {
     __device__ __forceinline__ void raise(unsigned char* dst, int g, float up) const {
         const __half2 f = __float2half2_rn(up);
 #pragma unroll 1
-        for (int i = 0; i < 16; i++) {
-            const int u = tid + 128 * (i >> 2), r = 64 * g + (u >> 3);
-            __half2* p = reinterpret_cast<__half2*>(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4)) + (i & 3);
-            *p = __hmul2(*p, f);
+        for (int i = 0; i < 4; i++) {
+            const int u = tid + 128 * i, r = 64 * g + (u >> 3);
+            uint4* p = reinterpret_cast<uint4*>(dst + r * 128 + (((u & 7) ^ (r & 7)) << 4));
+            uint4 x = *p;
+            __half2* e = reinterpret_cast<__half2*>(&x);
+#pragma unroll
+            for (int j = 0; j < 4; j++) e[j] = __hmul2(e[j], f);
+            *p = x;
         }
     }
     // In tiles with masked places, this thread's 32 values of the group once more: is one no number?
@@ -423,7 +427,7 @@ __device__ __forceinline__ void sv_convert(const AttnArgs& A, SvSmem* S, unsigne
 // scale, would lose what values below 1/448 leave of them.)  All lanes of a warp call.
 __device__ __forceinline__ float sv_tail_scale(const __half* src, int rows, int lane) {
     uint32_t mx = 0;  // of two halves' bits; infinities and NaN pass by
-#pragma unroll 4
+#pragma unroll 8
     for (int u = lane; u < rows * (CUINF_HD / 8); u += 32) {
         const uint4 x = *reinterpret_cast<const uint4*>(src + 8 * u);
         const uint32_t w[4] = {x.x & 0x7fff7fffu, x.y & 0x7fff7fffu, x.z & 0x7fff7fffu, x.w & 0x7fff7fffu};
@@ -437,7 +441,13 @@ __device__ __forceinline__ float sv_tail_scale(const __half* src, int rows, int 
 // scales of group l of 16 tiles.
 __device__ __forceinline__ bool sv_pages(const AttnArgs& A, SvSmem* S, const SvItem& w, unsigned char* Fs, uint32_t& kt,
                                          int lane) {
-    const int ng = w.q.kv / SERVE_PAGE, te = w.te;
+    const int ng = w.q.kv / SERVE_PAGE, te = w.te, rest = w.q.kv % SERVE_PAGE;
+    const size_t tail = ((size_t)w.s * A.nkv + w.h) * SERVE_PAGE_HEAD;
+    if (te == w.n)  // the tail's lines, here and by the converters read at once where they are needed
+        for (int r = lane; r < rest; r += 32) {
+            prefetch_l2(A.kv.vtail + tail + r * CUINF_HD);
+            prefetch_l2(A.kv.ktail + tail + r * CUINF_HD);
+        }
     for (int c = w.tb; c < te; c += 16) {
         const int g = 2 * c + lane;
         int kind = g < ng ? SV_PAGE : g == ng && w.q.kv % SERVE_PAGE ? SV_TAIL : SV_NONE;
@@ -458,9 +468,8 @@ __device__ __forceinline__ bool sv_pages(const AttnArgs& A, SvSmem* S, const SvI
             const uint32_t fs = kt % SV_FST;
             if (!sv_wait_all(&S->f_empty[fs], ((kt / SV_FST) & 1) ^ 1, &S->abort_)) return false;
             const bool mine = lane >> 1 == i;
-            if (2 * (c + i) + 1 == ng && w.q.kv % SERVE_PAGE) {  // a page and the tail
-                const float scale = sv_tail_scale(A.kv.vtail + ((size_t)w.s * A.nkv + w.h) * SERVE_PAGE_HEAD,
-                                                  w.q.kv % SERVE_PAGE, lane);
+            if (2 * (c + i) + 1 == ng && rest) {  // a page and the tail
+                const float scale = sv_tail_scale(A.kv.vtail + tail, rest, lane);
                 if (mine && kind == SV_TAIL) vs = scale;
             }
             if (mine) {
