@@ -50,8 +50,8 @@ extern "C" int cuinf_paged_error(unsigned* flags) {
 // 28 KB of straight code, which a CTA's one pass spent its time fetching).
 // The maximum is reduced over the warp and the codes written once, a head's
 // page block being one run of 4096 bytes.  Bound by HBM: 256 bytes in and 128
-// out per token and head; 4 x 16384 tokens of 8 kv heads (201 MB) take 36.9 us,
-// 5.46 TB/s, 83 % of a copy's rate (62 us with the rows in registers and a
+// out per token and head; 4 x 16384 tokens of 8 kv heads (201 MB) take 35.0 us,
+// 5.75 TB/s, 88 % of a copy's rate (62 us with the rows in registers and a
 // division per value).
 //
 // The rows of the unfinished last group go to the tail.  The warp of the

@@ -19,11 +19,12 @@
 // weights: one rounding of a weight to fp16.
 //
 // Measured on B200, 8 kv heads of 4 query heads, one token each: 64 contexts of
-// 2048 tokens 42 us and of 4096 64 us (269 MB, 4.2 TB/s), 128 of up to 8191
-// tokens 129 us (554 MB, 4.3 TB/s); one of 32768 20 us (33.6 MB).  From 2048
-// to 4096 tokens the added bytes go at 6.5 TB/s, the copy rate: the rest is a
-// part per call (the launch, the line, the first pages' latency, the join) and
-// per item (the warps' join).  8 warps took 56 us for the first, 11 (what the
+// 2048 tokens 40 us and of 4096 61 us (269 MB, 4.4 TB/s), 128 of up to 8191
+// tokens 128 us (554 MB, 4.3 TB/s); one of 32768 18 us (33.6 MB).  From 2048
+// to 4096 tokens the added bytes go at 6.3 TB/s, near the copy rate: the rest is
+// a part per call (the launch, the line, the first pages' latency, the join: 8.5
+// us for 63 tokens) and per item (the warps' join: the same 269 MB as 512
+// contexts of 512 take 102 us, 1.7 us per further item of a CTA).  8 warps took 56 us for the first, 11 (what the
 // registers allow) 53; most of the rest came of smaller code (128 to 83 KB).
 #pragma once
 #include "serve_line.cuh"

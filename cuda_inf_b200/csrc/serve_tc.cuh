@@ -20,15 +20,16 @@
 // A row tile's softmax gives its S back once the scores are in registers, so
 // the next scores come while it works and the kernel runs at the softmax's
 // pace.  With head_dim 64 the exponentials alone (128 x 128 of them at 16 a
-// clock: 1024 clocks) take twice the products' 512.  Measured on B200, 32
-// query and 8 kv heads: one prompt of 16384 tokens 1.286 ms, 855 TFLOP/s of
-// the 1648 that a library matrix product reaches (the exponentials' bound is
-// 1150 at 1.9 GHz); 12 prompts of up to 1500 tokens 112 us; over pages, 4 chunks of 1024 tokens
-// behind 8192: 474 us, 615 TFLOP/s.  At 4096 tokens the exponential unit is
-// busy 60 % and the tensor pipe 30 % of the time, and the 8 softmax warps
-// issue on 41 % of the clocks: two warps a scheduler do not hide the TMEM
-// loads' and each other's latencies.  Replacing exponentials by polynomials on
-// the FMA pipes therefore gained nothing (1/8 to 1/2 of them).
+// clock: 1024 clocks) take twice the products' 512.  Measured on B200, 32 query
+// and 8 kv heads: one prompt of 16384 tokens 1.275 ms, 862 TFLOP/s (back to
+// back, under the 1 kW power cap, 1.39 to 1.41 ms) of the 1648 that a library
+// matrix product reaches (the exponentials' bound is 1150 at 1.9 GHz); 12
+// prompts of up to 1500 tokens 110 us; over pages, 4 chunks of 1024 tokens
+// behind 8192: 464 us, 628 TFLOP/s.  At 4096 tokens the exponential unit is
+// busy 60 % and the tensor pipe 30 % of the time, and the 8 softmax warps issue
+// on 41 % of the clocks: two warps a scheduler do not hide the TMEM loads' and
+// each other's latencies.  Replacing exponentials by polynomials on the FMA
+// pipes therefore gained nothing (1/8 to 1/2 of them).
 //
 // The row blocks' key tiles of all sequences are laid end to end, and each CTA
 // takes an equal share of that line (or, where items are short, the items that
