@@ -24,8 +24,9 @@
 // to 4096 tokens the added bytes go at 6.3 TB/s, near the copy rate: the rest is
 // a part per call (the launch, the line, the first pages' latency, the join: 8.5
 // us for 63 tokens) and per item (the warps' join: the same 269 MB as 512
-// contexts of 512 take 102 us, 1.7 us per further item of a CTA).  8 warps took 56 us for the first, 11 (what the
-// registers allow) 53; most of the rest came of smaller code (128 to 83 KB).
+// contexts of 512 take 102 us, 1.7 us per further item of a CTA).  8 warps took
+// 56 us for the first, 11 (what the registers allow) 53; most of the rest came of
+// smaller code (128 to 83 KB).
 #pragma once
 #include "serve_line.cuh"
 
@@ -283,7 +284,7 @@ __device__ __forceinline__ void fw_unit(const FwUnit& x, FwRows& R, FwSmem* S, i
         R.per_unit *= step;
 #pragma unroll
         for (int r = 0; r < NR; r++) {
-            const float mn = fmaxf(R.m[r], top[r]);
+            const float mn = top[r] > R.m[r] + SV_GROWTH ? top[r] : R.m[r];  // (each row for itself)
             float f = R.m[r] == -INFINITY ? 0.f : sv_exp2(R.m[r] - mn);
             R.m[r] = mn, R.l[r] *= f, f *= step;
 #pragma unroll

@@ -25,7 +25,7 @@
 // back, under the 1 kW power cap, 1.39 to 1.41 ms) of the 1648 that a library
 // matrix product reaches (the exponentials' bound is 1150 at 1.9 GHz); 12
 // prompts of up to 1500 tokens 110 us; over pages, 4 chunks of 1024 tokens
-// behind 8192: 464 us, 628 TFLOP/s.  At 4096 tokens the exponential unit is
+// behind 8192: 469 us, 621 TFLOP/s.  At 4096 tokens the exponential unit is
 // busy 60 % and the tensor pipe 30 % of the time, and the 8 softmax warps issue
 // on 41 % of the clocks: two warps a scheduler do not hide the TMEM loads' and
 // each other's latencies.  Replacing exponentials by polynomials on the FMA
@@ -637,11 +637,11 @@ __global__ void __launch_bounds__(SvCfg<PAGED>::WARPS * 32, 1)
                 if (i == tb && !PAGED) {
                     m = x;
                 } else if (i == tb ||
-                           __any_sync(0xffffffffu, live_row && (x > m + SV_GROWTH ||
-                                                                (PAGED && fmaxf(vc[0], vc[1]) * per_unit >= SV_UNIT_TOP)))) {
-                    // (rows that are nobody's, another sequence's or left in shared memory, have no vote: a row's bits
-                    // go by its sequence alone)  rare: the reference follows the maximum (and the unit the scales), sum and O with it
-                    const float mn = fmaxf(m, x);
+                           __any_sync(0xffffffffu, x > m + SV_GROWTH ||
+                                                       (PAGED && fmaxf(vc[0], vc[1]) * per_unit >= SV_UNIT_TOP))) {
+                    // rare: the reference follows the maximum (and the unit the scales), sum and O with it; each row for
+                    // itself, so that its bits do not go by the others of the warp, which may be nobody's
+                    const float mn = x > m + SV_GROWTH ? x : m;
                     float f = m == -INFINITY ? 0.f : sv_exp2(m - mn);
                     m = mn;
 #pragma unroll

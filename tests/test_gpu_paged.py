@@ -984,3 +984,21 @@ def test_bits_go_by_the_sequence_alone(cuda, nh, nkv):
                 other[a:b] = q[a:b]
                 ops.attn_varlen(big * scale, big[:, :nkv], big[:, :nkv], cum([900], cuda))
                 assert torch.equal(call(other)[a:b], want[a:b]), (i, scale)
+
+
+@pytest.mark.parametrize("nh,nkv", [(32, 8), (5, 1), (12, 4)])
+@pytest.mark.parametrize("new", [2, 3, 4, 100])
+def test_bits_go_by_the_row_alone(cuda, nh, nkv, new):
+    """The other new tokens' queries do not change a row's bits, whether its sequence is drafted tokens or a chunk."""
+    c = Cache(1, nkv, 3000, cuda)
+    fill(c, [2900], 3)
+    q = rnd((new, nh, 64), 7, cuda, 2.0)
+    kv = [rnd((new, nkv, 64), 9 + i, cuda) for i in range(2)]
+    calls = [lambda q: c.attend(q, [new], max_q=new), lambda q: ops.attn_varlen(q, *kv, cum([new], cuda))]
+    for call in calls:
+        want = call(q)
+        for row in (0, new // 2, new - 1):
+            for scale in (0.0, 20.0):
+                other = q * scale
+                other[row] = q[row]
+                assert torch.equal(call(other)[row], want[row]), (row, scale)
